@@ -25,8 +25,8 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-shared", "-fPIC", "-ffp
 # the training-layer operators, a library of their own (a multiplication and an addition may be one operation there, except where a
 # source says otherwise)
 LAYER_LIB = os.path.join(HERE, "libace_layer.so")
-LAYER_SOURCES = [os.path.join(HERE, "csrc", name) for name in ("layer_norm.hip", "layer_attend.hip", "layer_adamw.hip")]
-LAYER_HEADERS = [os.path.join(HERE, "csrc", "layer_common.h"), os.path.join(ROOT, "include", "ace_layer.h"), os.path.join(ROOT, "include", "ace_eval.h")]
+LAYER_SOURCES = [os.path.join(HERE, "csrc", name) for name in ("layer_norm.hip", "layer_norm_back.hip", "layer_attend.hip", "layer_adamw.hip")]
+LAYER_HEADERS = [os.path.join(HERE, "csrc", "layer_common.h"), os.path.join(HERE, "csrc", "layer_norm.h"), os.path.join(ROOT, "include", "ace_layer.h"), os.path.join(ROOT, "include", "ace_eval.h")]
 
 # walks plan objects for the one-call-at-a-time API: a CPython extension module, host code only (no contraction: see above)
 OBJECTS_SOURCE = os.path.join(HERE, "csrc", "ace_objects.cpp")

@@ -42,9 +42,9 @@ __device__ inline uint32_t half_wave_max(uint32_t bits) {
 
 struct None {};
 template <class C> __device__ inline void store_copy(C *to, int64_t at, const float *p, int n) {
-    Raw8<C> r;
+    vec8<C> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = (C)p[i];
+    for (int i = 0; i < 8; ++i) r[i] = (C)p[i];
     store_some(to + at, r, n);
 }
 template <> __device__ inline void store_copy<None>(None *, int64_t, const float *, int) {}
@@ -64,45 +64,45 @@ template <int BITS, class G, class C> __global__ void __launch_bounds__(LANES) a
         /* (a block with no element of the tensor is nobody's: nothing of it is read or written) */
         if (BITS == 8 ? left + (threadIdx.x & 31) * 8 <= 0 : left <= 0) break;
         const int n = left > 8 ? 8 : (int)left;
-        const Raw8<float> p0 = load_some(t.d_param + at, n);
-        const Raw8<G> g0 = load_some(grad + at, n);
+        const vec8<float> p0 = load_some(t.d_param + at, n);
+        const vec8<G> g0 = load_some(grad + at, n);
         float m[8], v[8], u[8], p[8];
         if (BITS == 32) {
-            const Raw8<float> m0 = load_some((const float *)a.m + t.state_at + at, n), v0 = load_some((const float *)a.v + t.state_at + at, n);
+            const vec8<float> m0 = load_some((const float *)a.m + t.state_at + at, n), v0 = load_some((const float *)a.v + t.state_at + at, n);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m[i] = m0.v[i], v[i] = v0.v[i];
+            for (int i = 0; i < 8; ++i) m[i] = m0[i], v[i] = v0[i];
         } else {
             /* (whole blocks: the moments' storage is padded to them) */
-            const Raw8<int8_t> mc = load8((const int8_t *)a.m + t.state_at + at);
-            const Raw8<uint8_t> vc = load8((const uint8_t *)a.v + t.state_at + at);
+            const vec8<int8_t> mc = load8((const int8_t *)a.m + t.state_at + at);
+            const vec8<uint8_t> vc = load8((const uint8_t *)a.v + t.state_at + at);
             const float ms = a.m_scale[(t.state_at + at) / ACE_ADAMW_BLOCK], vs = a.v_scale[(t.state_at + at) / ACE_ADAMW_BLOCK];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                m[i] = (float)mc.v[i] * ms;
-                const float root = (float)vc.v[i] * vs;
+                m[i] = (float)mc[i] * ms;
+                const float root = (float)vc[i] * vs;
                 v[i] = root * root;
                 if (i >= n) m[i] = v[i] = 0.0f;
             }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float g = (float)g0.v[i] * gs;
+            const float g = (float)g0[i] * gs;
             m[i] = m[i] * a.beta1 + g * a.one_minus_beta1;
             v[i] = v[i] * a.beta2 + (g * g) * a.one_minus_beta2;
             if (BITS == 8 && i >= n) m[i] = v[i] = 0.0f;
             u[i] = __builtin_sqrtf(v[i]);
             /* (the parameter is rounded once more anyway: a reciprocal that is right to its last bit or the one before it) */
-            p[i] = p0.v[i] * a.decay - m[i] * a.step_size * __builtin_amdgcn_rcpf(u[i] * a.root_scale + a.eps);
+            p[i] = p0[i] * a.decay - m[i] * a.step_size * __builtin_amdgcn_rcpf(u[i] * a.root_scale + a.eps);
         }
-        Raw8<float> out;
+        vec8<float> out;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out.v[i] = p[i];
+        for (int i = 0; i < 8; ++i) out[i] = p[i];
         store_some(t.d_param + at, out, n);
         store_copy(copy, at, p, n);
         if (BITS == 32) {
-            Raw8<float> mo, vo;
+            vec8<float> mo, vo;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mo.v[i] = m[i], vo.v[i] = v[i];
+            for (int i = 0; i < 8; ++i) mo[i] = m[i], vo[i] = v[i];
             store_some((float *)a.m + t.state_at + at, mo, n);
             store_some((float *)a.v + t.state_at + at, vo, n);
         } else {
@@ -114,14 +114,14 @@ template <int BITS, class G, class C> __global__ void __launch_bounds__(LANES) a
             }
             const float m_top = __uint_as_float(half_wave_max(m_bits)), u_top = __uint_as_float(half_wave_max(u_bits));
             const bool m_fine = m_top < __builtin_inff(), u_fine = u_top < __builtin_inff();
-            const float m_by = m_fine ? 127.0f / fmaxf(m_top, 1e-30f) : 0.0f, u_by = u_fine ? 255.0f / fmaxf(u_top, 1e-30f) : 0.0f;
-            Raw8<int8_t> mc;
-            Raw8<uint8_t> vc;
+            const float m_by = m_fine ? 1.0f / fmaxf(m_top, 1e-30f) * 127.0f : 0.0f, u_by = u_fine ? 1.0f / fmaxf(u_top, 1e-30f) * 255.0f : 0.0f;
+            vec8<int8_t> mc;
+            vec8<uint8_t> vc;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                mc.v[i] = m_fine ? (int8_t)(int)__builtin_rintf(m[i] * m_by) : (int8_t)0;
+                mc[i] = m_fine ? (int8_t)(int)__builtin_rintf(m[i] * m_by) : (int8_t)0;
                 const int code = u_fine ? (int)__builtin_rintf(u[i] * u_by) : 0;
-                vc.v[i] = (uint8_t)(u[i] > 0.0f && code < 1 ? 1 : code);
+                vc[i] = (uint8_t)(u[i] > 0.0f && code < 1 ? 1 : code);
             }
             store8((int8_t *)a.m + t.state_at + at, mc);
             store8((uint8_t *)a.v + t.state_at + at, vc);
@@ -137,15 +137,15 @@ template <int BITS, class G, class C> __global__ void __launch_bounds__(LANES) a
 __global__ void __launch_bounds__(LANES) moments_kernel(const int8_t *m, const uint8_t *v, const float *m_scale, const float *v_scale, int64_t vectors, float *m_out,
                                                         float *v_out) {
     for (int64_t k = (int64_t)blockIdx.x * LANES + threadIdx.x; k < vectors; k += (int64_t)gridDim.x * LANES) {
-        const Raw8<int8_t> mc = load8(m + k * 8);
-        const Raw8<uint8_t> vc = load8(v + k * 8);
+        const vec8<int8_t> mc = load8(m + k * 8);
+        const vec8<uint8_t> vc = load8(v + k * 8);
         const float ms = m_scale[k / (ACE_ADAMW_BLOCK / 8)], vs = v_scale[k / (ACE_ADAMW_BLOCK / 8)];
-        Raw8<float> mo, vo;
+        vec8<float> mo, vo;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            mo.v[i] = (float)mc.v[i] * ms;
-            const float root = (float)vc.v[i] * vs;
-            vo.v[i] = root * root;
+            mo[i] = (float)mc[i] * ms;
+            const float root = (float)vc[i] * vs;
+            vo[i] = root * root;
         }
         store8(m_out + k * 8, mo);
         store8(v_out + k * 8, vo);

@@ -26,33 +26,33 @@ typedef _Float16 f16;
 
 /* Eight consecutive elements as they lie in memory.  Addresses are multiples of the element's size only: the loads and stores
  * below are full-width at any alignment (unaligned access is on for every process of this platform). */
-template <class T> struct Raw8 { T v[8]; };
+template <class T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
+template <class T> using vec8 = typename Vec8<T>::type;
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 
-template <class T> __device__ inline Raw8<T> load8(const T *p) {
-    Raw8<T> r;
+template <class T> __device__ inline vec8<T> load8(const T *p) {
+    vec8<T> r;
     __builtin_memcpy(&r, p, sizeof r);
     return r;
 }
-template <class T> __device__ inline void store8(T *p, const Raw8<T> &r) { __builtin_memcpy(p, &r, sizeof r); }
+template <class T> __device__ inline void store8(T *p, vec8<T> r) { __builtin_memcpy(p, &r, sizeof r); }
 
 /* of a row's last vector only the first n elements are there; the rest is zero */
-template <class T> __device__ inline Raw8<T> load_some(const T *p, int n) {
-    Raw8<T> r;
+template <class T> __device__ inline vec8<T> load_some(const T *p, int n) {
     if (n >= 8) return load8(p);
+    vec8<T> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = i < n ? p[i] : (T)0.0f;
+    for (int i = 0; i < 8; ++i) r[i] = i < n ? p[i] : (T)0;
     return r;
 }
-template <class T> __device__ inline void store_some(T *p, const Raw8<T> &r, int n) {
+template <class T> __device__ inline void store_some(T *p, vec8<T> r, int n) {
     if (n >= 8) {
         store8(p, r);
         return;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (i < n) p[i] = r.v[i];
+        if (i < n) p[i] = r[i];
 }
-
-template <class T> __device__ inline T narrow(float f) { return (T)f; }
 
 #endif
