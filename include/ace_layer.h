@@ -69,8 +69,8 @@ typedef struct ace_attend {
     int32_t window, sinks;                                /* window 0: all earlier keys */
     float scale;
     const int32_t *d_start, *d_length;                    /* int32[batch]; NULL: keys - queries, keys */
-    /* elements between consecutive sequences, tokens and heads (a head's elements are adjacent); all multiples of 8, and every
-     * tensor starts at a multiple of 16 bytes */
+    /* elements between consecutive sequences, tokens and heads (a head's elements are adjacent); all multiples of 8, between
+     * tokens 0 to 2^23 - 8, and every tensor starts at a multiple of 16 bytes */
     int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
     const void *d_q, *d_k, *d_v;
     void *d_out;                                          /* [batch][queries][heads][dim] by out_stride */
@@ -81,9 +81,10 @@ size_t ace_attend_workspace_bytes(const ace_attend_t *a);
 int ace_attend_forward(const ace_attend_t *a, void *d_workspace, size_t workspace_bytes, void *stream);
 
 /* dq [batch][queries][heads][dim], dk and dv [batch][keys][kv_heads][dim], contiguous; d_gout: gradient of out, by
- * gout_stride.  d_out and d_lse of `a` are read.  d_delta: float[batch][heads][queries], scratch. */
-int ace_attend_backward(const ace_attend_t *a, const void *d_gout, const int64_t gout_stride[3], float *d_delta, void *d_dq, void *d_dk,
-                        void *d_dv, void *stream);
+ * gout_stride.  d_out and d_lse of `a` are read.  d_workspace: ace_attend_backward_workspace_bytes(a) bytes. */
+size_t ace_attend_backward_workspace_bytes(const ace_attend_t *a);
+int ace_attend_backward(const ace_attend_t *a, const void *d_gout, const int64_t gout_stride[3], void *d_dq, void *d_dk, void *d_dv,
+                        void *d_workspace, size_t workspace_bytes, void *stream);
 
 /* ---- AdamW over many tensors -------------------------------------------------------------------------------------------
  *     g = grad_scale * grad;  m = m b1 + g (1 - b1);  v = v b2 + g^2 (1 - b2)

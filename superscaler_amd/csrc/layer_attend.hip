@@ -11,10 +11,11 @@
  * row-major tiles by transposing LDS reads of four rows each.  No value passes through LDS on its way from one product to the
  * next.
  *
- * Tiles go from memory to LDS without registers between, 16 bytes per lane.  A tile's 16-byte pieces are exchanged within
- * their row, piece c of row r at c ^ swizzle(r): both kinds of reads, eight rows at one piece and four rows at two pieces, then
- * fall on different banks.  Rows past the sequence's length (and pieces past the head's size) are read from a page of zeros:
- * whatever stands there in memory, a number or not, takes no part.
+ * Tiles go from memory to LDS without registers between, 16 bytes per lane, through a buffer descriptor of the tile's rows: a lane's
+ * place in a tile is the same for every tile, and rows past the sequence's length (and pieces past the head's size) are out of
+ * the descriptor's range and arrive as zeros.  Whatever stands there in memory, a number or not, takes no part.  A tile's
+ * 16-byte pieces are exchanged within their row, piece c of row r at c ^ swizzle(r), so that what LDS serves at a time in
+ * either kind of read, sixteen rows at one piece or four rows at four pieces, lies in all of its 64 banks.
  */
 #include "layer_common.h"
 
@@ -31,9 +32,9 @@ struct Args {
     void *dq, *dk, *dv;
     float *part_o, *part_ml;             /* attend_split: [splits][rows][width], [splits][rows][2] */
     int splits, row_blocks;
+    float *far;                          /* attend_far: [batch][kv_heads][far_blocks][far_parts][2][width][32] */
+    int far_blocks, far_parts;
 };
-
-__device__ uint4 zero_page[1];
 
 typedef __attribute__((address_space(3))) char *lds_ptr;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -51,18 +52,21 @@ template <> struct Mma<f16> {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ inline int swizzle(int row) { return 2 * (row & 3) + ((row >> 2) & 1); }
+/* LDS serves a 16-byte read of a wavefront by sixteen lanes at a time (0-3, 12-15, 20-23, 24-27; then the others alike), an 8-byte
+ * read by lanes 0-31 and 32-63.  Rows of 256 bytes lie in all banks: the sixteen rows need sixteen places, the four rows of a
+ * transposing read four groups of four.  Rows of 128 bytes: two rows share the banks, the rest alike. */
+template <int PITCH> __device__ inline int swizzle(int row) { return PITCH == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3); }
 
 __device__ inline uint32_t lds_offset(const void *p) { return (uint32_t)(uintptr_t)(lds_ptr)p; }
 
-/* 16 bytes per lane from `from` to LDS at `to` + 16 lane (`to`: the same for the wavefront).  The LDS write is complete when the
- * wavefront's vector-memory counter says so (wait_tiles).  m0, the destination, needs one state before it is used; nothing else in
- * these kernels uses it. */
-__device__ inline void to_lds16(const void *from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
+/* 16 bytes per lane from place `at` of the rows to LDS at `to` + 16 lane (`to`: the same for the wavefront).  The LDS write is complete
+ * when the wavefront's vector-memory counter says so (wait_tiles).  m0, the destination, needs one state before it is used; nothing
+ * else in these kernels uses it. */
+__device__ inline void to_lds16(u32x4 rows, uint32_t at, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(rows) : "memory");
 }
-__device__ inline void to_lds4(const void *from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "memory");
+__device__ inline void to_lds4(u32x4 rows, uint32_t at, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(at), "s"(rows) : "memory");
 }
 template <int LEFT> __device__ inline void wait_tiles() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory"); }
 __device__ inline void meet() {
@@ -70,37 +74,64 @@ __device__ inline void meet() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
+/* registers that loads fill are complete here: nothing later waits for them together with what was asked for since */
+template <class V> __device__ inline void arrived(V &v) { asm volatile("" : "+v"(v)); }
 
-/* ROWS rows of a tile by LANES lanes; rows at or past `end` and elements past `dim` come from the page of zeros. */
-template <class T, int PITCH, int ROWS, int LANES> __device__ inline void load_tile(uint32_t to, const T *base, int64_t stride, int row0, int end, int dim, int lane) {
-    constexpr int PER = PITCH / 8;
+/* A buffer descriptor of `bytes` bytes from `p` on, both the same for the wavefront. */
+__device__ inline u32x4 buffer(const void *p, int64_t bytes) {
+    const uint64_t at = (uint64_t)(uintptr_t)p;
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xffff),
+                 (uint32_t)__builtin_amdgcn_readfirstlane(bytes < 0 ? 0 : (int)bytes), 0x00027000u};
+}
+
+/* A tile's rows in memory and where the lanes find their pieces of them: ROWS rows of PITCH elements by LANES lanes. */
+template <class T, int PITCH, int ROWS, int LANES> struct Tile {
+    static constexpr int PER = PITCH / 8, LOADS = ROWS * PER / LANES;
     static_assert(ROWS * PER % LANES == 0, "whole loads");
-    const uint32_t wave_at = __builtin_amdgcn_readfirstlane(to + (lane & ~63) * 16);
+    const T *base;
+    int64_t stride;
+    int dim;
+    uint32_t at[LOADS], to;
+    __device__ inline Tile(const T *b, int64_t s, int d, int lane) : base(b), stride(s), dim(d) {
 #pragma unroll
-    for (int i = 0; i < ROWS * PER / LANES; ++i) {
-        const int p = i * LANES + lane, row = p / PER, piece = (p % PER) ^ (swizzle(row) & (PER - 1));
-        const bool there = row0 + row < end && piece * 8 < dim;
-        const void *from = there ? (const void *)(base + (int64_t)(row0 + row) * stride + piece * 8) : (const void *)zero_page;
-        to_lds16(from, wave_at + i * LANES * 16);
+        for (int i = 0; i < LOADS; ++i) {
+            const int p = i * LANES + lane, row = p / PER, piece = (p % PER) ^ (swizzle<PITCH>(row) & (PER - 1));
+            at[i] = piece * 8 < d ? (uint32_t)(row * (int)s + piece * 8) * 2u : 0x80000000u;   /* (past every descriptor's end) */
+        }
+        to = (lane & ~63) * 16;
     }
-}
+    __device__ inline void ask(uint32_t lds, int row0, int end) const {
+        const int rows = end - row0 < ROWS ? end - row0 : ROWS;
+        const u32x4 b = buffer(base + (int64_t)row0 * stride, rows > 0 ? ((int64_t)(rows - 1) * stride + dim) * 2 : 0);
+        const uint32_t at_lds = __builtin_amdgcn_readfirstlane(lds + to);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) to_lds16(b, at[i], at_lds + i * LANES * 16);
+    }
+};
 
-/* Where a lane reads its part of an operand whose rows are the tile's rows: row `row`, pieces 2 s + h. */
-template <class T, int PITCH> __device__ inline typename Mma<T>::frag row_frag(const char *tile, int row0, int s, int lane) {
-    const int row = row0 + (lane & 31), piece = (2 * s + (lane >> 5)) ^ (swizzle(lane & 31) & (PITCH / 8 - 1));
-    return *(const typename Mma<T>::frag *)(tile + row * PITCH * 2 + piece * 16);
-}
+template <class V> __device__ inline V lds_load(uint32_t at) { return *(const __attribute__((address_space(3))) V *)at; }
 
-/* The transposed operand: rows are elements 32 t + lane % 32 of the head, k the sixteen tile rows from row0 on. */
-template <class T, int PITCH> __device__ inline typename Mma<T>::frag column_frag(const char *tile, int row0, int t, int lane) {
-    const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2);
-    const int piece = (4 * t + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ (swizzle(r) & (PITCH / 8 - 1));
-    const char *at = tile + (row0 + r) * PITCH * 2 + piece * 16 + (i & 1) * 8;
-    union { s16x4 half[2]; typename Mma<T>::frag whole; } u;
-    u.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(lds_ptr)at);
-    u.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(lds_ptr)(at + 8 * PITCH * 2));
-    return u.whole;
-}
+/* Where a lane finds its part of operands in a tile of rows of PITCH elements; a tile begins at a multiple of a row.  Pieces of other
+ * steps differ in bits that are exchanged, never carried, so a place is one base with bits flipped, plus a constant. */
+template <class T, int PITCH> struct Operands {
+    typedef typename Mma<T>::frag frag;
+    uint32_t row, column;
+    __device__ inline explicit Operands(int lane) {
+        const int half = lane >> 5, i = lane & 15, r = 4 * half + (i >> 2);
+        row = (lane & 31) * PITCH * 2 + (half ^ (swizzle<PITCH>(lane & 31) & (PITCH / 8 - 1))) * 16;
+        column = r * PITCH * 2 + ((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ (swizzle<PITCH>(r) & (PITCH / 8 - 1))) * 16 + (i & 1) * 8;
+    }
+    /* rows are the tile's rows row0 + lane % 32, k the elements 16 s to 16 s + 15 */
+    __device__ inline frag rows(uint32_t tile, int row0, int s) const { return lds_load<frag>(((tile + row) ^ (s << 5)) + row0 * PITCH * 2); }
+    /* rows are the elements 32 t + lane % 32, k the tile's rows row0 to row0 + 15 (row0: a multiple of sixteen) */
+    __device__ inline frag columns(uint32_t tile, int row0, int t) const {
+        union { s16x4 half[2]; frag whole; } u;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            u.half[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(lds_ptr)(((tile + column) ^ (t << 6 | k << 5)) + (row0 + 8 * k) * PITCH * 2));
+        return u.whole;
+    }
+};
 
 template <class T> __device__ inline typename Mma<T>::frag pack8(const float *p) {
     typename Mma<T>::frag r;
@@ -140,15 +171,37 @@ template <int SIZE> __device__ inline Tiles tiles_of(const Args &a, const Sequen
     return {first, at, first + to - at};
 }
 
-__device__ inline bool sees(const Args &a, int length, int p, int key) {
-    return key < length && key <= p && (a.window == 0 || p - key < a.window || key < a.sinks);
-}
 /* whether positions lo..hi all see (or all do not see) keys from..to - 1 */
 __device__ inline bool all_see(const Args &a, int length, int lo, int hi, int from, int to) {
     return to <= length && to - 1 <= lo && (a.window == 0 || hi - from < a.window || to <= a.sinks);
 }
 __device__ inline bool none_see(const Args &a, int length, int lo, int hi, int from, int to) {
     return from >= length || from > hi || (a.window > 0 && lo - (to - 1) >= a.window && from >= a.sinks);
+}
+
+/* What a query sees: `count` keys from `from` on, and those below `first`. */
+struct Sight {
+    int from, first;
+    uint32_t count;
+    __device__ inline Sight(const Args &a, int length, int p) {
+        const int end = p + 1 < length ? p + 1 : length;
+        from = a.window > 0 ? p - a.window + 1 : 0;
+        count = end > from ? end - from : 0;
+        first = a.window > 0 ? (a.sinks < end ? a.sinks : end) : 0;
+    }
+};
+/* Values of keys key0 + result_row(i) that are not seen become `otherwise`.  `sinks`: some of the keys are first ones. */
+__device__ inline void hide(float *s, const Sight &sight, int key0, int half, bool sinks, float otherwise) {
+    const int t = key0 + 4 * half - sight.from, u = key0 + 4 * half;
+    if (sinks) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if ((uint32_t)(t + 8 * (i / 4) + i % 4) >= sight.count && u + 8 * (i / 4) + i % 4 >= sight.first) s[i] = otherwise;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if ((uint32_t)(t + 8 * (i / 4) + i % 4) >= sight.count) s[i] = otherwise;
+    }
 }
 
 /* Work in an order that keeps a head's blocks, which read the same keys, on one of the eight dies and its cache: workgroups go to
@@ -176,8 +229,8 @@ __device__ inline float other_half(float x) { return __shfl_xor(x, 32); }
 /* One block of 32 keys times NB more for 32 queries: scores, softmax, weighted values.  The maximum that exponentials are taken
  * around moves only when a score passes it by 8 powers of two: the sums stay far from their range's end, and most blocks
  * need no rescaling. */
-template <class T, int DP, int PITCH, int NB> __device__ inline void block_step(Running<DP / 32> &run, const typename Mma<T>::frag *qf, const char *ktile, const char *vtile,
-                                                                                const Args &a, int length, int p, int key0, bool masked, int lane) {
+template <class T, int DP, int PITCH, int NB> __device__ inline void block_step(Running<DP / 32> &run, const typename Mma<T>::frag *qf, const Operands<T, PITCH> &ops, uint32_t ktile, uint32_t vtile,
+                                                                                const Args &a, const Sight &sight, int key0, bool masked, int lane) {
     const int half = lane >> 5;
     float s[NB][16];
     float top = -__builtin_inff();
@@ -185,17 +238,13 @@ template <class T, int DP, int PITCH, int NB> __device__ inline void block_step(
     for (int n = 0; n < NB; ++n) {
         f32x16 acc = {};
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) acc = Mma<T>::go(row_frag<T, PITCH>(ktile, n * 32, k, lane), qf[k], acc);
+        for (int k = 0; k < DP / 16; ++k) acc = Mma<T>::go(ops.rows(ktile, n * 32, k), qf[k], acc);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][i] = acc[i];
     }
-    if (masked) {
+    if (masked)
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (!sees(a, length, p, key0 + n * 32 + result_row(i, half))) s[n][i] = -__builtin_inff();
-    }
+        for (int n = 0; n < NB; ++n) hide(s[n], sight, key0 + n * 32, half, key0 < a.sinks, -__builtin_inff());
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -230,7 +279,7 @@ template <class T, int DP, int PITCH, int NB> __device__ inline void block_step(
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int t = 0; t < DP / 32; ++t) run.o[t] = Mma<T>::go(column_frag<T, PITCH>(vtile, n * 32 + k * 16, t, lane), pf[n][k], run.o[t]);
+            for (int t = 0; t < DP / 32; ++t) run.o[t] = Mma<T>::go(ops.columns(vtile, n * 32 + k * 16, t), pf[n][k], run.o[t]);
 }
 
 /* Four neighbouring elements of a result, rounded. */
@@ -245,7 +294,7 @@ constexpr int WAVES = 4, LANES = WAVES * 64, QUERIES = WAVES * 32, KEYS = 64;
 
 /* Prompts: a workgroup takes 128 queries of a head, 32 per wavefront, and walks over its keys in tiles of 64, the next tile on its
  * way while one is worked on. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_forward(const Args a) {
+template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_forward(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
     const int blocks = (a.queries + QUERIES - 1) / QUERIES, count = a.batch * a.heads * blocks;
@@ -259,19 +308,23 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_forwa
     const T *k = (const T *)a.k + b * a.k_stride[0] + head / a.shared * a.k_stride[2], *v = (const T *)a.v + b * a.v_stride[0] + head / a.shared * a.v_stride[2];
     const Tiles tiles = tiles_of<KEYS>(a, seq, seq.start + q0, seq.start + last);
     const uint32_t lds0 = lds_offset(lds);
+    const Operands<T, PITCH> ops(lane);
+    const Tile<T, PITCH, KEYS, LANES> ktiles(k, a.k_stride[1], a.dim, threadIdx.x), vtiles(v, a.v_stride[1], a.dim, threadIdx.x);
     auto ask = [&](int t) {
         const uint32_t to = lds0 + (t & 1) * 2 * TILE;
         const int at = tiles.tile(t) * KEYS;
-        load_tile<T, PITCH, KEYS, LANES>(to, k, a.k_stride[1], at, seq.length, a.dim, threadIdx.x);
-        load_tile<T, PITCH, KEYS, LANES>(to + TILE, v, a.v_stride[1], at, seq.length, a.dim, threadIdx.x);
+        ktiles.ask(to, at, seq.length), vtiles.ask(to + TILE, at, seq.length);
     };
     if (tiles.count > 0) ask(0);
     const T *qrow = (const T *)a.q + b * a.q_stride[0] + (int64_t)query * a.q_stride[1] + head * a.q_stride[2];
     typename Mma<T>::frag qf[DP / 16];
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) qf[s] = global_frag<T>(qrow, s * 16 + half * 8, a.dim, query < a.queries);
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) arrived(qf[s]);
     Running<DP / 32> run;
     run.clear();
+    const Sight sight(a, seq.length, seq.start + query);
     const int lo = seq.start + mine, hi = seq.start + (mine + 31 < a.queries ? mine + 31 : a.queries - 1);
     for (int t = 0; t < tiles.count; ++t) {
         wait_tiles<0>();
@@ -279,8 +332,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_forwa
         if (t + 1 < tiles.count) ask(t + 1);
         const int at = tiles.tile(t) * KEYS;
         if (mine >= a.queries || none_see(a, seq.length, lo, hi, at, at + KEYS)) continue;
-        const char *ktile = lds + (t & 1) * 2 * TILE;
-        block_step<T, DP, PITCH, KEYS / 32>(run, qf, ktile, ktile + TILE, a, seq.length, seq.start + query, at, !all_see(a, seq.length, lo, hi, at, at + KEYS), lane);
+        const uint32_t ktile = lds0 + (t & 1) * 2 * TILE;
+        block_step<T, DP, PITCH, KEYS / 32>(run, qf, ops, ktile, ktile + TILE, a, sight, at, !all_see(a, seq.length, lo, hi, at, at + KEYS), lane);
     }
     const float total = run.total + other_half(run.total);
     if (query >= a.queries) return;
@@ -312,19 +365,22 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split
     const Tiles tiles = tiles_of<SPLIT_KEYS>(a, seq, lo, hi);
     const int worker = split * WAVES + wave, workers = a.splits * WAVES;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds) + wave * 4 * TILE);
-    char *own = lds + wave * 4 * TILE;
+    const Operands<T, PITCH> ops(lane);
+    const Tile<T, PITCH, SPLIT_KEYS, 64> ktiles(k, a.k_stride[1], a.dim, lane), vtiles(v, a.v_stride[1], a.dim, lane);
     auto ask = [&](int t, int buffer) {
         const uint32_t to = lds0 + buffer * 2 * TILE;
         const int at = tiles.tile(t) * SPLIT_KEYS;
-        load_tile<T, PITCH, SPLIT_KEYS, 64>(to, k, a.k_stride[1], at, seq.length, a.dim, lane);
-        load_tile<T, PITCH, SPLIT_KEYS, 64>(to + TILE, v, a.v_stride[1], at, seq.length, a.dim, lane);
+        ktiles.ask(to, at, seq.length), vtiles.ask(to + TILE, at, seq.length);
     };
     const T *qrow = (const T *)a.q + b * a.q_stride[0] + (int64_t)query * a.q_stride[1] + head * a.q_stride[2];
     typename Mma<T>::frag qf[DP / 16];
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) qf[s] = global_frag<T>(qrow, s * 16 + half * 8, a.dim, row < rows);
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) arrived(qf[s]);
     Running<DP / 32> run;
     run.clear();
+    const Sight sight(a, seq.length, seq.start + query);
     int buffer = 0;
     if (worker < tiles.count) ask(worker, 0);
     for (int t = worker; t < tiles.count; t += workers, buffer ^= 1) {
@@ -336,8 +392,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split
         } else
             wait_tiles<0>();
         const int at = tiles.tile(t) * SPLIT_KEYS;
-        const char *ktile = own + buffer * 2 * TILE;
-        block_step<T, DP, PITCH, 1>(run, qf, ktile, ktile + TILE, a, seq.length, seq.start + query, at, !all_see(a, seq.length, lo, hi, at, at + SPLIT_KEYS), lane);
+        const uint32_t ktile = lds0 + buffer * 2 * TILE;
+        block_step<T, DP, PITCH, 1>(run, qf, ops, ktile, ktile + TILE, a, sight, at, !all_see(a, seq.length, lo, hi, at, at + SPLIT_KEYS), lane);
     }
     run.total += other_half(run.total);
     /* join the wavefronts: element d of a row's sum lies at [wave][d][row] */
@@ -405,9 +461,11 @@ template <class T> __global__ void __launch_bounds__(LANES) attend_join(const Ar
     if (lane == 0) a.lse[row] = total == 0.0f ? -__builtin_inff() : top * a.scale + __logf(total);
 }
 
+constexpr int FEW_TILES = 3;
+
 /* dQ: queries in registers, keys in tiles as in attend_forward; per block of 32 keys S^T = K Q^T, dP^T = V dO^T,
  * dQ^T += K^T dS^T.  It also leaves delta = sum dO O of every query for attend_dkv. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_dq(const Args a) {
+template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dq(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
     const int blocks = (a.queries + QUERIES - 1) / QUERIES, count = a.batch * a.heads * blocks;
@@ -421,11 +479,12 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_dq(co
     const T *k = (const T *)a.k + b * a.k_stride[0] + head / a.shared * a.k_stride[2], *v = (const T *)a.v + b * a.v_stride[0] + head / a.shared * a.v_stride[2];
     const Tiles tiles = tiles_of<KEYS>(a, seq, seq.start + q0, seq.start + last);
     const uint32_t lds0 = lds_offset(lds);
+    const Operands<T, PITCH> ops(lane);
+    const Tile<T, PITCH, KEYS, LANES> ktiles(k, a.k_stride[1], a.dim, threadIdx.x), vtiles(v, a.v_stride[1], a.dim, threadIdx.x);
     auto ask = [&](int t) {
         const uint32_t to = lds0 + (t & 1) * 2 * TILE;
         const int at = tiles.tile(t) * KEYS;
-        load_tile<T, PITCH, KEYS, LANES>(to, k, a.k_stride[1], at, seq.length, a.dim, threadIdx.x);
-        load_tile<T, PITCH, KEYS, LANES>(to + TILE, v, a.v_stride[1], at, seq.length, a.dim, threadIdx.x);
+        ktiles.ask(to, at, seq.length), vtiles.ask(to + TILE, at, seq.length);
     };
     if (tiles.count > 0) ask(0);
     const bool there = query < a.queries;
@@ -442,46 +501,63 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_dq(co
 #pragma unroll
         for (int i = 0; i < 8; ++i) delta += (float)gf[s][i] * (float)of[i];
     }
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) arrived(qf[s]), arrived(gf[s]);
     delta += other_half(delta);
     const int64_t flat = ((int64_t)b * a.heads + head) * a.queries + query;
-    if (there && half == 0) a.delta[flat] = delta;
-    const float lse2 = there ? a.lse[flat] * LOG2E : 0.0f;
+    float lse2 = there ? a.lse[flat] * LOG2E : 0.0f;
     f32x16 dq[DP / 32];
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) dq[t] = f32x16{};
-    const int lo = seq.start + mine, hi = seq.start + (mine + 31 < a.queries ? mine + 31 : a.queries - 1), p = seq.start + query;
-    for (int t = 0; t < tiles.count; ++t) {
-        wait_tiles<0>();
-        meet();
-        if (t + 1 < tiles.count) ask(t + 1);
-        const int at = tiles.tile(t) * KEYS;
-        if (mine >= a.queries) continue;
-        const char *ktile = lds + (t & 1) * 2 * TILE, *vtile = ktile + TILE;
+    arrived(lse2);
+    const int lo = seq.start + mine, hi = seq.start + (mine + 31 < a.queries ? mine + 31 : a.queries - 1);
+    const Sight sight(a, seq.length, seq.start + query);
+    /* With few keys the rounding of the forward pass's answer, which delta goes by, is no small part of dS: there delta is the sum of
+     * P dP itself, in a walk before the walk. */
+    const bool few = tiles.count <= FEW_TILES;
+    float sum = 0.0f;
+    for (int walk = few ? 0 : 1; walk < 2; ++walk) {
+        if (walk == 1) {
+            if (few) delta = sum + other_half(sum);
+            if (there && half == 0) a.delta[flat] = delta;
+        }
+        if (few && walk == 1) {
+            meet();   /* (every wavefront is through with the first walk's last tile) */
+            if (tiles.count > 0) ask(0);
+        }
+        for (int t = 0; t < tiles.count; ++t) {
+            wait_tiles<0>();
+            meet();
+            if (t + 1 < tiles.count) ask(t + 1);
+            const int at = tiles.tile(t) * KEYS;
+            if (mine >= a.queries) continue;
+            const uint32_t buffer_at = lds0 + (t & 1) * 2 * TILE;
+#pragma unroll 1
+            for (int n = 0; n < KEYS / 32; ++n) {
+                const int key0 = at + n * 32;
+                const uint32_t ktile = buffer_at + n * 32 * PITCH * 2, vtile = ktile + TILE;
+                if (none_see(a, seq.length, lo, hi, key0, key0 + 32)) continue;
+                f32x16 s = {}, dp = {};
 #pragma unroll
-        for (int n = 0; n < KEYS / 32; ++n) {
-            const int key0 = at + n * 32;
-            if (none_see(a, seq.length, lo, hi, key0, key0 + 32)) continue;
-            f32x16 s = {}, dp = {};
+                for (int j = 0; j < DP / 16; ++j) s = Mma<T>::go(ops.rows(ktile, 0, j), qf[j], s);
 #pragma unroll
-            for (int j = 0; j < DP / 16; ++j) s = Mma<T>::go(row_frag<T, PITCH>(ktile, n * 32, j, lane), qf[j], s);
+                for (int j = 0; j < DP / 16; ++j) dp = Mma<T>::go(ops.rows(vtile, 0, j), gf[j], dp);
+                float ds[16];
+                const float less = walk == 0 ? 0.0f : delta;
 #pragma unroll
-            for (int j = 0; j < DP / 16; ++j) dp = Mma<T>::go(row_frag<T, PITCH>(vtile, n * 32, j, lane), gf[j], dp);
-            const bool masked = !all_see(a, seq.length, lo, hi, key0, key0 + 32);
-            float ds[16];
+                for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse2)) * (dp[i] - less);
+                if (!all_see(a, seq.length, lo, hi, key0, key0 + 32)) hide(ds, sight, key0, half, key0 < a.sinks, 0.0f);
+                if (walk == 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float prob = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse2));
-                ds[i] = prob * (dp[i] - delta);
-            }
-            if (masked)
+                    for (int i = 0; i < 16; ++i) sum += ds[i];
+                    continue;
+                }
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!there || !sees(a, seq.length, p, key0 + result_row(i, half))) ds[i] = 0.0f;
+                for (int j = 0; j < 2; ++j) {
+                    const typename Mma<T>::frag f = pack8<T>(ds + 8 * j);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const typename Mma<T>::frag f = pack8<T>(ds + 8 * j);
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) dq[d] = Mma<T>::go(column_frag<T, PITCH>(ktile, n * 32 + j * 16, d, lane), f, dq[d]);
+                    for (int d = 0; d < DP / 32; ++d) dq[d] = Mma<T>::go(ops.columns(ktile, j * 16, d), f, dq[d]);
+                }
             }
         }
     }
@@ -496,12 +572,80 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_dq(co
         }
 }
 
-/* dK and dV: a workgroup takes 128 keys of a key head, 32 per wavefront in registers, and walks over the queries that see them, of
- * every head that shares the key head, in tiles of 64: S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS.  A key's sums stay
- * with one workgroup: no atomic additions, the same bits every time. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_dkv(const Args a) {
+/* dK and dV: 32 keys of a key head in a wavefront's registers, 32 queries at a time: S = Q K^T, dP = dO V^T, dV^T += dO^T P,
+ * dK^T += Q^T dS.  A key's sums stay with one wavefront: no atomic additions, the same bits every time. */
+template <class T, int DP> struct KeyGrads {
+    static constexpr int PITCH = Shape<DP>::PITCH;
+    typename Mma<T>::frag kf[DP / 16], vf[DP / 16];
+    f32x16 dk[DP / 32], dv[DP / 32];
+    __device__ inline void start(const T *krow, const T *vrow, int dim, bool there, int half) {
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) kf[s] = global_frag<T>(krow, s * 16 + half * 8, dim, there), vf[s] = global_frag<T>(vrow, s * 16 + half * 8, dim, there);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) arrived(kf[s]), arrived(vf[s]);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
+    }
+    /* `t`: the first query's position from the first one that sees this lane's key; the `count` from there on see it */
+    __device__ inline void step(const Operands<T, PITCH> &ops, uint32_t qtile, uint32_t gtile, uint32_t lse, uint32_t delta, float scale2, int t, uint32_t count, bool masked,
+                                int half) {
+        f32x16 s = {}, dp = {};
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j) s = Mma<T>::go(ops.rows(qtile, 0, j), kf[j], s);
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j) dp = Mma<T>::go(ops.rows(gtile, 0, j), vf[j], dp);
+        float prob[16], ds[16];
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const f32x4 l = lds_load<f32x4>(lse + 16 * half + 8 * i), d = lds_load<f32x4>(delta + 16 * half + 8 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                prob[i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + e], scale2, -l[e] * LOG2E));
+                ds[i + e] = prob[i + e] * (dp[i + e] - d[e]);
+            }
+        }
+        if (masked)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if ((uint32_t)(t + result_row(i, half)) >= count) prob[i] = ds[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const typename Mma<T>::frag pf = pack8<T>(prob + 8 * j), df = pack8<T>(ds + 8 * j);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) {
+                dv[d] = Mma<T>::go(ops.columns(gtile, j * 16, d), pf, dv[d]);
+                dk[d] = Mma<T>::go(ops.columns(qtile, j * 16, d), df, dk[d]);
+            }
+        }
+    }
+};
+
+/* Tiles of queries: rows of q and of the answer's gradient, then log-sums and deltas, by LANES lanes. */
+template <class T, int PITCH, int ROWS, int LANES> struct QueryTiles {
+    static constexpr int BYTES = ROWS * PITCH * 2, STAGE = 2 * BYTES + 2 * 256, LOADS = 2 * Tile<T, PITCH, ROWS, LANES>::LOADS + (LANES == 64 ? 2 : 1);
+    Tile<T, PITCH, ROWS, LANES> q, g;
+    const float *lse, *delta;
+    __device__ inline QueryTiles(const Args &a, int b, int lane)
+        : q((const T *)a.q + b * a.q_stride[0], a.q_stride[1], a.dim, lane), g((const T *)a.g + b * a.g_stride[0], a.g_stride[1], a.dim, lane),
+          lse(a.lse + (int64_t)b * a.heads * a.queries), delta(a.delta + (int64_t)b * a.heads * a.queries) {}
+    /* (a workgroup's four wavefronts: each asks for as many loads, the last two for those of the first two again) */
+    __device__ inline void ask(const Args &a, uint32_t lds, int head, int row, int wave, int lane) const {
+        Tile<T, PITCH, ROWS, LANES> qh = q, gh = g;
+        qh.base += head * a.q_stride[2], gh.base += head * a.g_stride[2];
+        qh.ask(lds, row, a.queries), gh.ask(lds + BYTES, row, a.queries);
+        const int64_t at = (int64_t)head * a.queries + row;
+        const int64_t bytes = (int64_t)(a.queries - row < ROWS ? a.queries - row : ROWS) * 4;
+        if (LANES == 64 || (wave & 1) == 0) to_lds4(buffer(lse + at, bytes), lane * 4, __builtin_amdgcn_readfirstlane(lds + 2 * BYTES));
+        if (LANES == 64 || (wave & 1) == 1) to_lds4(buffer(delta + at, bytes), lane * 4, __builtin_amdgcn_readfirstlane(lds + 2 * BYTES + 256));
+    }
+};
+
+/* The pairs of a window: a workgroup takes 128 keys and walks over the queries whose window they are in, of every head that shares the
+ * key head, in tiles of 64. */
+template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dkv(const Args a) {
     extern __shared__ char lds[];
-    constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2, STAGE = 2 * TILE + 512;
+    constexpr int PITCH = Shape<DP>::PITCH;
+    typedef QueryTiles<T, PITCH, KEYS, LANES> Queries;
     const int blocks = (a.keys + QUERIES - 1) / QUERIES, count = a.batch * a.kv_heads * blocks;
     const int work = place(count);
     if (work >= count) return;
@@ -509,81 +653,60 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_dkv(c
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Sequence seq = sequence(a, b);
     const int k0 = block * QUERIES, mine = k0 + wave * 32, key = mine + (lane & 31);
-    const bool there = key < seq.length;
     const T *krow = (const T *)a.k + b * a.k_stride[0] + (int64_t)key * a.k_stride[1] + kv * a.k_stride[2];
     const T *vrow = (const T *)a.v + b * a.v_stride[0] + (int64_t)key * a.v_stride[1] + kv * a.v_stride[2];
-    typename Mma<T>::frag kf[DP / 16], vf[DP / 16];
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) kf[s] = global_frag<T>(krow, s * 16 + half * 8, a.dim, there), vf[s] = global_frag<T>(vrow, s * 16 + half * 8, a.dim, there);
-    f32x16 dk[DP / 32], dv[DP / 32];
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
-    /* queries that see one of the keys: from position k0 on, and up to the last key's window unless one of them is a first key */
+    /* queries from the first key's position on, up to the last key's window */
     int from = k0 - seq.start, to = a.queries;
-    if (a.window > 0 && k0 >= a.sinks) {
+    if (a.window > 0) {
         const int64_t most = (int64_t)k0 + QUERIES - 1 + a.window - seq.start;
         to = most < to ? (int)most : to;
     }
     from = from < 0 ? 0 : from;
     const int first = from / KEYS, per_head = k0 < seq.length && to > from ? (to + KEYS - 1) / KEYS - first : 0, steps = per_head * a.shared;
     const uint32_t lds0 = lds_offset(lds);
+    const Operands<T, PITCH> ops(lane);
+    const Queries queries(a, b, threadIdx.x);
+    int head = kv * a.shared, tile = first;      /* of the next step to be asked for */
     auto ask = [&](int t) {
-        const uint32_t at = lds0 + (t & 1) * STAGE;
-        const int head = kv * a.shared + t / per_head, q = (first + t % per_head) * KEYS;
-        load_tile<T, PITCH, KEYS, LANES>(at, (const T *)a.q + b * a.q_stride[0] + head * a.q_stride[2], a.q_stride[1], q, a.queries, a.dim, threadIdx.x);
-        load_tile<T, PITCH, KEYS, LANES>(at + TILE, (const T *)a.g + b * a.g_stride[0] + head * a.g_stride[2], a.g_stride[1], q, a.queries, a.dim, threadIdx.x);
-        if (wave < 2) {
-            const float *row = (wave == 0 ? a.lse : a.delta) + ((int64_t)b * a.heads + head) * a.queries;
-            to_lds4(q + lane < a.queries ? (const void *)(row + q + lane) : (const void *)zero_page, __builtin_amdgcn_readfirstlane(at + 2 * TILE + wave * 256));
-        }
+        queries.ask(a, lds0 + (t & 1) * Queries::STAGE, head, tile * KEYS, wave, lane);
+        if (++tile == first + per_head) tile = first, ++head;
     };
+    KeyGrads<T, DP> grads;
+    grads.start(krow, vrow, a.dim, key < seq.length, half);
+    /* this lane's key is seen from its own position on, for a window's length, by queries that there are */
+    const int64_t left = (int64_t)seq.start + a.queries - key;
+    const uint32_t sight = key >= seq.length || left <= 0 ? 0 : a.window > 0 && a.window < left ? a.window : (uint32_t)left;
     if (steps > 0) ask(0);
+    int q = first * KEYS;
     for (int t = 0; t < steps; ++t) {
         wait_tiles<0>();
         meet();
         if (t + 1 < steps) ask(t + 1);
-        if (mine >= seq.length) continue;
-        const char *qtile = lds + (t & 1) * STAGE, *gtile = qtile + TILE;
-        const float *lse = (const float *)(gtile + TILE), *delta = lse + 64;
-#pragma unroll
-        for (int n = 0; n < KEYS / 32; ++n) {
-            const int q = (first + t % per_head) * KEYS + n * 32;
-            const int lo = seq.start + q, hi = seq.start + (q + 31 < a.queries ? q + 31 : a.queries - 1);
-            if (q >= a.queries || none_see(a, seq.length, lo, hi, mine, mine + 32)) continue;
-            f32x16 s = {}, dp = {};
-#pragma unroll
-            for (int j = 0; j < DP / 16; ++j) s = Mma<T>::go(row_frag<T, PITCH>(qtile, n * 32, j, lane), kf[j], s);
-#pragma unroll
-            for (int j = 0; j < DP / 16; ++j) dp = Mma<T>::go(row_frag<T, PITCH>(gtile, n * 32, j, lane), vf[j], dp);
-            const bool masked = q + 32 > a.queries || !all_see(a, seq.length, lo, hi, mine, mine + 32);
-            float prob[16], ds[16];
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const f32x4 l = *(const f32x4 *)(lse + n * 32 + result_row(i, half)), d = *(const f32x4 *)(delta + n * 32 + result_row(i, half));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    prob[i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + e], a.scale2, -l[e] * LOG2E));
-                    ds[i + e] = prob[i + e] * (dp[i + e] - d[e]);
-                }
+        const uint32_t buffer_at = lds0 + (t & 1) * Queries::STAGE;
+        if (mine < seq.length)
+#pragma unroll 1
+            for (int n = 0; n < KEYS / 32; ++n) {
+                const int lo = seq.start + q + n * 32, hi = lo + 31;
+                if (q + n * 32 >= a.queries || hi < mine || (a.window > 0 && lo - (mine + 31) >= a.window)) continue;
+                const bool masked = q + n * 32 + 32 > a.queries || mine + 32 > seq.length || lo < mine + 31 || (a.window > 0 && hi - mine >= a.window);
+                const uint32_t qtile = buffer_at + n * 32 * PITCH * 2, lse = buffer_at + 2 * Queries::BYTES + n * 32 * 4;
+                grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + 256, a.scale2, lo - key, sight, masked, half);
             }
-            if (masked)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at = q + result_row(i, half);
-                    if (at >= a.queries || !sees(a, seq.length, seq.start + at, key)) prob[i] = ds[i] = 0.0f;
-                }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const typename Mma<T>::frag pf = pack8<T>(prob + 8 * j), df = pack8<T>(ds + 8 * j);
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
-                    dv[d] = Mma<T>::go(column_frag<T, PITCH>(gtile, n * 32 + j * 16, d, lane), pf, dv[d]);
-                    dk[d] = Mma<T>::go(column_frag<T, PITCH>(qtile, n * 32 + j * 16, d, lane), df, dk[d]);
-                }
-            }
-        }
+        q = q + KEYS < (first + per_head) * KEYS ? q + KEYS : first * KEYS;
     }
     if (key >= a.keys) return;
+    /* what queries beyond the window have left for a first key */
+    if (a.far_parts > 0 && mine < a.sinks) {
+        const float *part = a.far + ((((int64_t)b * a.kv_heads + kv) * a.far_blocks + mine / 32) * a.far_parts) * (2 * 32 * DP) + (lane & 31);
+        for (int c = 0; c < a.far_parts; ++c, part += 2 * 32 * DP)
+#pragma unroll
+            for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int d = t * 32 + result_row(i, half);
+                    grads.dk[t][i] += part[d * 32], grads.dv[t][i] += part[(DP + d) * 32];
+                }
+    }
     T *dkrow = (T *)a.dk + (((int64_t)b * a.keys + key) * a.kv_heads + kv) * a.dim, *dvrow = (T *)a.dv + (((int64_t)b * a.keys + key) * a.kv_heads + kv) * a.dim;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t)
@@ -591,9 +714,62 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_dkv(c
         for (int i = 0; i < 16; i += 4) {
             const int d = t * 32 + result_row(i, half);
             if (d >= a.dim) continue;
-            store4(dkrow + d, dk[t][i] * a.scale, dk[t][i + 1] * a.scale, dk[t][i + 2] * a.scale, dk[t][i + 3] * a.scale);
-            store4(dvrow + d, dv[t][i], dv[t][i + 1], dv[t][i + 2], dv[t][i + 3]);
+            store4(dkrow + d, grads.dk[t][i] * a.scale, grads.dk[t][i + 1] * a.scale, grads.dk[t][i + 2] * a.scale, grads.dk[t][i + 3] * a.scale);
+            store4(dvrow + d, grads.dv[t][i], grads.dv[t][i + 1], grads.dv[t][i + 2], grads.dv[t][i + 3]);
         }
+}
+
+/* The first keys and the queries beyond their window: every later query of every head sees those few keys, so the work is split
+ * over the queries.  A wavefront walks over tiles of 32 queries with buffers of its own; a workgroup's sums, element d of key j at
+ * [dk, dv][d][j], are one part, and attend_dkv adds the parts in order. */
+template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_far(const Args a) {
+    extern __shared__ char lds[];
+    constexpr int PITCH = Shape<DP>::PITCH;
+    typedef QueryTiles<T, PITCH, 32, 64> Queries;
+    const int part = blockIdx.x, block = blockIdx.y % a.far_blocks, kv = blockIdx.y / a.far_blocks, b = blockIdx.z;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const Sequence seq = sequence(a, b);
+    const int k0 = block * 32, key = k0 + (lane & 31);
+    const T *krow = (const T *)a.k + b * a.k_stride[0] + (int64_t)key * a.k_stride[1] + kv * a.k_stride[2];
+    const T *vrow = (const T *)a.v + b * a.v_stride[0] + (int64_t)key * a.v_stride[1] + kv * a.v_stride[2];
+    KeyGrads<T, DP> grads;
+    grads.start(krow, vrow, a.dim, key < seq.length, half);
+    const int64_t begin = (int64_t)k0 + a.window - seq.start;      /* the first query beyond the first key's window */
+    const int first = begin <= 0 ? 0 : begin < a.queries ? (int)begin / 32 : 0;
+    const int per_head = k0 < seq.length && begin < a.queries ? (a.queries + 31) / 32 - first : 0, items = per_head * a.shared;
+    const int worker = part * WAVES + wave, workers = a.far_parts * WAVES;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_offset(lds) + wave * 2 * Queries::STAGE);
+    const Operands<T, PITCH> ops(lane);
+    const Queries queries(a, b, lane);
+    auto ask = [&](int i, int buffer) { queries.ask(a, lds0 + buffer * Queries::STAGE, kv * a.shared + i / per_head, (first + i % per_head) * 32, 0, lane); };
+    const int64_t left = (int64_t)seq.start + a.queries - key - a.window;
+    const uint32_t sight = key >= seq.length || key >= a.sinks || left <= 0 ? 0 : (uint32_t)left;
+    int buffer = 0;
+    if (worker < items) ask(worker, 0);
+    for (int i = worker; i < items; i += workers, buffer ^= 1) {
+        if (i + workers < items) {
+            /* (the other buffer's last reads have returned: their results went into the products before this) */
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            ask(i + workers, buffer ^ 1);
+            wait_tiles<Queries::LOADS>();
+        } else
+            wait_tiles<0>();
+        const uint32_t qtile = lds0 + buffer * Queries::STAGE, lse = qtile + 2 * Queries::BYTES;
+        grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + 256, a.scale2, seq.start + (first + i % per_head) * 32 - key - a.window, sight, true, half);
+    }
+    float *sums = (float *)lds;
+    constexpr int HALF = DP * 32;
+    float *to = a.far + ((((int64_t)b * a.kv_heads + kv) * a.far_blocks + block) * a.far_parts + part) * (2 * HALF);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[wave * HALF + (t * 32 + result_row(i, half)) * 32 + (lane & 31)] = which ? grads.dv[t][i] : grads.dk[t][i];
+        __syncthreads();
+        for (int e = threadIdx.x; e < HALF; e += LANES) to[which * HALF + e] = sums[e] + sums[HALF + e] + sums[2 * HALF + e] + sums[3 * HALF + e];
+    }
 }
 
 int check(const ace_attend_t *a) {
@@ -601,6 +777,9 @@ int check(const ace_attend_t *a) {
     if (a->dim < 8 || a->dim % 8 || a->window < 0 || a->sinks < 0 || (a->dtype != ACE_T_BF16 && a->dtype != ACE_T_F16)) return ACE_EINVAL;
     if (!(a->scale > 0.0f) || a->scale > 1e30f) return ACE_EINVAL;
     if (a->dim > 128 || a->queries > (1 << 30) || a->keys > (1 << 30)) return ACE_ETOOBIG;
+    /* (a tile of 64 rows is named by 32-bit places) */
+    const int64_t widest = (int64_t)1 << 23;
+    if (a->q_stride[1] >= widest || a->k_stride[1] >= widest || a->v_stride[1] >= widest || a->q_stride[1] < 0 || a->k_stride[1] < 0 || a->v_stride[1] < 0) return ACE_ETOOBIG;
     for (int i = 0; i < 3; ++i)
         if (a->q_stride[i] % 8 || a->k_stride[i] % 8 || a->v_stride[i] % 8 || a->out_stride[i] % 8) return ACE_EINVAL;
     if (a->batch == 0 || a->queries == 0) return ACE_OK;
@@ -659,17 +838,38 @@ template <class T, int DP> int forward(Args &k, const ace_attend_t *a, hipStream
     return layer_launched();
 }
 
+/* Blocks of 32 first keys, and over how many workgroups the queries beyond their window go: about two for every CU, at least four
+ * tiles of queries for a wavefront. */
+void far_of(const ace_attend_t *a, Args &k) {
+    const int64_t sinks = a->window > 0 ? (a->sinks < a->keys ? a->sinks : a->keys) : 0;
+    k.far_blocks = (int)((sinks + 31) / 32), k.far_parts = 0;
+    if (sinks == 0 || a->batch == 0 || a->queries == 0) return;
+    const int64_t groups = (int64_t)a->batch * a->kv_heads * k.far_blocks, tiles = (int64_t)(a->heads / a->kv_heads) * ((a->queries + 31) / 32);
+    int64_t parts = (512 + groups - 1) / groups;
+    const int64_t most = (tiles + WAVES * 4 - 1) / (WAVES * 4);
+    parts = parts < most ? parts : most;
+    k.far_parts = parts < 1 ? 1 : parts > 32 ? 32 : (int)parts;
+}
+int width_of(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
+int64_t delta_floats(const ace_attend_t *a) { return ((int64_t)a->batch * a->heads * a->queries + 3) / 4 * 4; }
+
 template <class T, int DP> int backward(const Args &k, hipStream_t stream) {
-    constexpr int PITCH = Shape<DP>::PITCH, LDS = 4 * KEYS * PITCH * 2, LDS2 = LDS + 1024;
-    static const int ready = with_lds(attend_dq<T, DP>, LDS), ready2 = with_lds(attend_dkv<T, DP>, LDS2);
-    if (ready != ACE_OK || ready2 != ACE_OK) return ACE_EHIP;
+    constexpr int PITCH = Shape<DP>::PITCH, DQ = 4 * KEYS * PITCH * 2, DKV = 2 * QueryTiles<T, PITCH, KEYS, LANES>::STAGE;
+    constexpr int FAR_TILES = WAVES * 2 * QueryTiles<T, PITCH, 32, 64>::STAGE, FAR_JOIN = WAVES * DP * 32 * 4, FAR = FAR_TILES > FAR_JOIN ? FAR_TILES : FAR_JOIN;
+    static const int ready = with_lds(attend_dq<T, DP>, DQ), ready2 = with_lds(attend_dkv<T, DP>, DKV), ready3 = with_lds(attend_far<T, DP>, FAR);
+    if (ready != ACE_OK || ready2 != ACE_OK || ready3 != ACE_OK) return ACE_EHIP;
+    int rc = ACE_OK;
     if (k.queries > 0) {
-        attend_dq<T, DP><<<places((int64_t)k.batch * k.heads * ((k.queries + QUERIES - 1) / QUERIES)), LANES, LDS, stream>>>(k);
-        const int rc = layer_launched();
-        if (rc != ACE_OK) return rc;
+        attend_dq<T, DP><<<places((int64_t)k.batch * k.heads * ((k.queries + QUERIES - 1) / QUERIES)), LANES, DQ, stream>>>(k);
+        if ((rc = layer_launched()) != ACE_OK) return rc;
     }
     if (k.keys == 0) return ACE_OK;
-    attend_dkv<T, DP><<<places((int64_t)k.batch * k.kv_heads * ((k.keys + QUERIES - 1) / QUERIES)), LANES, LDS2, stream>>>(k);
+    if (k.far_parts > 0) {
+        if (k.batch > 65535 || (int64_t)k.kv_heads * k.far_blocks > 65535) return ACE_ETOOBIG;
+        attend_far<T, DP><<<dim3(k.far_parts, k.kv_heads * k.far_blocks, k.batch), LANES, FAR, stream>>>(k);
+        if ((rc = layer_launched()) != ACE_OK) return rc;
+    }
+    attend_dkv<T, DP><<<places((int64_t)k.batch * k.kv_heads * ((k.keys + QUERIES - 1) / QUERIES)), LANES, DKV, stream>>>(k);
     return layer_launched();
 }
 
@@ -695,18 +895,28 @@ extern "C" int ace_attend_forward(const ace_attend_t *a, void *d_workspace, size
     return a->dim <= 64 ? forward<f16, 64>(k, a, s) : a->dim <= 96 ? forward<f16, 96>(k, a, s) : forward<f16, 128>(k, a, s);
 }
 
-extern "C" int ace_attend_backward(const ace_attend_t *a, const void *d_gout, const int64_t gout_stride[3], float *d_delta, void *d_dq, void *d_dk,
-                                   void *d_dv, void *stream) {
+extern "C" size_t ace_attend_backward_workspace_bytes(const ace_attend_t *a) {
+    if (check(a) != ACE_OK || a->batch == 0) return 0;
+    Args k = {};
+    far_of(a, k);
+    return (size_t)(delta_floats(a) + (int64_t)a->batch * a->kv_heads * k.far_blocks * k.far_parts * 2 * 32 * width_of(a->dim)) * sizeof(float);
+}
+
+extern "C" int ace_attend_backward(const ace_attend_t *a, const void *d_gout, const int64_t gout_stride[3], void *d_dq, void *d_dk, void *d_dv, void *d_workspace,
+                                   size_t workspace_bytes, void *stream) {
     const int rc = check(a);
     if (rc != ACE_OK || a->batch == 0) return rc;
-    if ((a->queries > 0 && (!d_gout || !gout_stride || !d_delta || !d_dq)) || (a->keys > 0 && (!d_dk || !d_dv))) return ACE_EINVAL;
-    if (((uintptr_t)d_gout | (uintptr_t)d_dq | (uintptr_t)d_dk | (uintptr_t)d_dv) & 15) return ACE_EINVAL;
+    if ((a->queries > 0 && (!d_gout || !gout_stride || !d_dq || !d_workspace)) || (a->keys > 0 && (!d_dk || !d_dv))) return ACE_EINVAL;
+    if (workspace_bytes < ace_attend_backward_workspace_bytes(a)) return ACE_EINVAL;
+    if (((uintptr_t)d_gout | (uintptr_t)d_dq | (uintptr_t)d_dk | (uintptr_t)d_dv | (uintptr_t)d_workspace) & 15) return ACE_EINVAL;
     Args k = args_of(a);
-    k.g = d_gout, k.delta = d_delta, k.dq = d_dq, k.dk = d_dk, k.dv = d_dv;
+    far_of(a, k);
+    k.g = d_gout, k.delta = (float *)d_workspace, k.far = k.delta + delta_floats(a), k.dq = d_dq, k.dk = d_dk, k.dv = d_dv;
     for (int i = 0; gout_stride && i < 3; ++i) {
         if (gout_stride[i] % 8) return ACE_EINVAL;
         k.g_stride[i] = gout_stride[i];
     }
+    if (k.g_stride[1] < 0 || k.g_stride[1] >= (int64_t)1 << 23) return ACE_ETOOBIG;
     const hipStream_t s = (hipStream_t)stream;
     if (a->dtype == ACE_T_BF16) return a->dim <= 64 ? backward<bf16, 64>(k, s) : a->dim <= 96 ? backward<bf16, 96>(k, s) : backward<bf16, 128>(k, s);
     return a->dim <= 64 ? backward<f16, 64>(k, s) : a->dim <= 96 ? backward<f16, 96>(k, s) : backward<f16, 128>(k, s);

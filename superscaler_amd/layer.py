@@ -25,7 +25,8 @@ _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libace_lay
 _lib = None
 
 EXPORTS = ["ace_layer_abi_version", "ace_layer_strerror", "ace_layer_last_hip_error", "ace_block_norm_forward", "ace_block_norm_workspace_bytes",
-           "ace_block_norm_backward", "ace_attend_workspace_bytes", "ace_attend_forward", "ace_attend_backward", "ace_adamw_step", "ace_adamw_moments"]
+           "ace_block_norm_backward", "ace_attend_workspace_bytes", "ace_attend_forward", "ace_attend_backward_workspace_bytes",
+           "ace_attend_backward", "ace_adamw_step", "ace_adamw_moments"]
 ABI_VERSION = 1
 MAX_WIDTH = 32768       # ACE_NORM_MAX_WIDTH
 MAX_HEAD = 128
@@ -64,7 +65,7 @@ def load_library():
         getattr(lib, name).restype = ctypes.c_int
     for name in ("ace_layer_strerror", "ace_layer_last_hip_error"):
         getattr(lib, name).restype = ctypes.c_char_p
-    for name in ("ace_block_norm_workspace_bytes", "ace_attend_workspace_bytes"):
+    for name in ("ace_block_norm_workspace_bytes", "ace_attend_workspace_bytes", "ace_attend_backward_workspace_bytes"):
         getattr(lib, name).restype = ctypes.c_size_t
     lib.ace_layer_strerror.argtypes = [ctypes.c_int]
     lib.ace_block_norm_forward.argtypes = [_vp] * 5
@@ -72,7 +73,8 @@ def load_library():
     lib.ace_block_norm_backward.argtypes = [_vp] * 12 + [ctypes.c_size_t, _vp]
     lib.ace_attend_workspace_bytes.argtypes = [_vp]
     lib.ace_attend_forward.argtypes = [_vp, _vp, ctypes.c_size_t, _vp]
-    lib.ace_attend_backward.argtypes = [_vp] * 8
+    lib.ace_attend_backward_workspace_bytes.argtypes = [_vp]
+    lib.ace_attend_backward.argtypes = [_vp] * 7 + [ctypes.c_size_t, _vp]
     lib.ace_adamw_step.argtypes = [_vp] * 4 + [_f32] * 8 + [_vp]
     lib.ace_adamw_moments.argtypes = [_vp] * 4 + [_i64, _vp, _vp, _vp]
     if lib.ace_layer_abi_version() != ABI_VERSION:
@@ -230,7 +232,8 @@ def _heads(t, what, like=None):
     if like is not None and t.device != like.device:
         raise ValueError(f"{what} is on {t.device}, q on {like.device}")
     stride = t.stride()
-    if (t.shape[3] > 1 and stride[3] != 1) or any(n > 1 and s % 8 for n, s in zip(t.shape[:3], stride)) or t.data_ptr() % 16:
+    if (t.shape[3] > 1 and stride[3] != 1) or any(n > 1 and s % 8 for n, s in zip(t.shape[:3], stride)) or t.data_ptr() % 16 or \
+            (t.shape[1] > 1 and stride[1] >= 1 << 23):
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -301,9 +304,9 @@ def window_attention_backward(d_out, q, k, v, out, lse, *, window=None, sinks=0,
         raise ValueError("lse: what window_attention returned expected")
     a.out_stride, a.d_out, a.d_lse = _strides(out), out.data_ptr(), lse.data_ptr()
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    delta = torch.empty_like(lse)
-    stride = _strides(d_out)
-    _call(q.device, "ace_attend_backward", ctypes.byref(a), d_out.data_ptr(), stride, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+    size = load_library().ace_attend_backward_workspace_bytes(ctypes.byref(a))
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _call(q.device, "ace_attend_backward", ctypes.byref(a), d_out.data_ptr(), _strides(d_out), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), size)
     return dq, dk, dv
 
 
