@@ -74,7 +74,8 @@ __device__ inline void meet() {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
-/* registers that loads fill are complete here: nothing later waits for them together with what was asked for since */
+/* The registers of a value, whole, here: loads that fill them are complete (nothing later waits for them together with what was asked
+ * for since), and sums leave a loop in the registers that they have in it. */
 template <class V> __device__ inline void arrived(V &v) { asm volatile("" : "+v"(v)); }
 
 /* A buffer descriptor of `bytes` bytes from `p` on, both the same for the wavefront. */
@@ -335,6 +336,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_fo
         const uint32_t ktile = lds0 + (t & 1) * 2 * TILE;
         block_step<T, DP, PITCH, KEYS / 32>(run, qf, ops, ktile, ktile + TILE, a, sight, at, !all_see(a, seq.length, lo, hi, at, at + KEYS), lane);
     }
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) arrived(run.o[t]);
     const float total = run.total + other_half(run.total);
     if (query >= a.queries) return;
     const float by = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total;   /* (nothing visible: zero; not a number: that) */
@@ -395,6 +398,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split
         const uint32_t ktile = lds0 + buffer * 2 * TILE;
         block_step<T, DP, PITCH, 1>(run, qf, ops, ktile, ktile + TILE, a, sight, at, !all_see(a, seq.length, lo, hi, at, at + SPLIT_KEYS), lane);
     }
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) arrived(run.o[t]);
     run.total += other_half(run.total);
     /* join the wavefronts: element d of a row's sum lies at [wave][d][row] */
     float *sums = (float *)lds, *tops = sums + WAVES * DP * 32;
@@ -561,6 +566,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dq
             }
         }
     }
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) arrived(dq[t]);
     if (!there) return;
     T *to = (T *)a.dq + (((int64_t)b * a.queries + query) * a.heads + head) * a.dim;
 #pragma unroll
@@ -585,6 +592,10 @@ template <class T, int DP> struct KeyGrads {
         for (int s = 0; s < DP / 16; ++s) arrived(kf[s]), arrived(vf[s]);
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
+    }
+    __device__ inline void stop() {
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) arrived(dk[t]), arrived(dv[t]);
     }
     /* `t`: the first query's position from the first one that sees this lane's key; the `count` from there on see it */
     __device__ inline void step(const Operands<T, PITCH> &ops, uint32_t qtile, uint32_t gtile, uint32_t lse, uint32_t delta, float scale2, int t, uint32_t count, bool masked,
@@ -694,6 +705,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dk
             }
         q = q + KEYS < (first + per_head) * KEYS ? q + KEYS : first * KEYS;
     }
+    grads.stop();
     if (key >= a.keys) return;
     /* what queries beyond the window have left for a first key */
     if (a.far_parts > 0 && mine < a.sinks) {
@@ -757,6 +769,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_far(c
         const uint32_t qtile = lds0 + buffer * Queries::STAGE, lse = qtile + 2 * Queries::BYTES;
         grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + 256, a.scale2, seq.start + (first + i % per_head) * 32 - key - a.window, sight, true, half);
     }
+    grads.stop();
     float *sums = (float *)lds;
     constexpr int HALF = DP * 32;
     float *to = a.far + ((((int64_t)b * a.kv_heads + kv) * a.far_blocks + block) * a.far_parts + part) * (2 * HALF);
