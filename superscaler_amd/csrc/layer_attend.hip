@@ -157,6 +157,20 @@ __device__ inline Sequence sequence(const Args &a, int b) {
     return {start < -far ? -far : start > far ? far : start, length < 0 ? 0 : length > a.keys ? a.keys : length};
 }
 
+/* The order of a run of PRODUCTS matrix products whose operands come from LDS in READS reads each: operands of LEAD products are on
+ * their way before the first, and those of one more are asked for with each.  (Left to itself the compiler waits for every
+ * operand right behind its read, four times as long as the product takes.) */
+template <int PRODUCTS, int READS, int LEAD> __device__ inline void in_step() {
+    __builtin_amdgcn_sched_group_barrier(0x100, LEAD * READS, 0);
+#pragma unroll
+    for (int i = 0; i < PRODUCTS - LEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, LEAD, 0);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 /* The keys that positions lo..hi see, in tiles of SIZE: `first` tiles from 0 on (first keys), then those from `at` to `to`. */
 struct Tiles {
     int first, at, count;
@@ -225,7 +239,17 @@ template <int DT> struct Running {
     }
 };
 
-__device__ inline float other_half(float x) { return __shfl_xor(x, 32); }
+/* of a lane's value and that of the lane 32 further on, the other half of its query's keys */
+__device__ inline float sum_halves(float x) {
+    const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const uint32_t a = two[0], b = two[1];
+    return __uint_as_float(a) + __uint_as_float(b);
+}
+__device__ inline float max_halves(float x) {
+    const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const uint32_t a = two[0], b = two[1];
+    return fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
 
 /* One block of 32 keys times NB more for 32 queries: scores, softmax, weighted values.  The maximum that exponentials are taken
  * around moves only when a score passes it by 8 powers of two: the sums stay far from their range's end, and most blocks
@@ -237,12 +261,15 @@ template <class T, int DP, int PITCH, int NB> __device__ inline void block_step(
     float top = -__builtin_inff();
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
+        if (n == 0) __builtin_amdgcn_s_setprio(1), __builtin_amdgcn_sched_barrier(0);
         f32x16 acc = {};
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) acc = Mma<T>::go(ops.rows(ktile, n * 32, k), qf[k], acc);
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[n][i] = acc[i];
     }
+    in_step<NB * DP / 16, 1, 4>();
+    __builtin_amdgcn_s_setprio(0);
     if (masked)
 #pragma unroll
         for (int n = 0; n < NB; ++n) hide(s[n], sight, key0 + n * 32, half, key0 < a.sinks, -__builtin_inff());
@@ -250,7 +277,7 @@ template <class T, int DP, int PITCH, int NB> __device__ inline void block_step(
     for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
-    top = fmaxf(top, other_half(top));
+    top = max_halves(top);
     const bool more = (top - run.top) * a.scale2 > 8.0f;   /* (also from no key at all, -inf, to any) */
     if (__any(more)) {
         const float to = more ? top : run.top;
@@ -275,12 +302,16 @@ template <class T, int DP, int PITCH, int NB> __device__ inline void block_step(
         run.total += sum;
         pf[n][0] = pack8<T>(s[n]), pf[n][1] = pack8<T>(s[n] + 8);
     }
+    __builtin_amdgcn_s_setprio(1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t) run.o[t] = Mma<T>::go(ops.columns(vtile, n * 32 + k * 16, t), pf[n][k], run.o[t]);
+    in_step<NB * 2 * DP / 32, 2, 3>();
+    __builtin_amdgcn_s_setprio(0);
 }
 
 /* Four neighbouring elements of a result, rounded. */
@@ -295,7 +326,7 @@ constexpr int WAVES = 4, LANES = WAVES * 64, QUERIES = WAVES * 32, KEYS = 64;
 
 /* Prompts: a workgroup takes 128 queries of a head, 32 per wavefront, and walks over its keys in tiles of 64, the next tile on its
  * way while one is worked on. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_forward(const Args a) {
+template <class T, int DP> __global__ void __launch_bounds__(LANES) __attribute__((amdgpu_waves_per_eu(2, 2))) attend_forward(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
     const int blocks = (a.queries + QUERIES - 1) / QUERIES, count = a.batch * a.heads * blocks;
@@ -338,7 +369,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_fo
     }
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(run.o[t]);
-    const float total = run.total + other_half(run.total);
+    const float total = sum_halves(run.total);
     if (query >= a.queries) return;
     const float by = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total;   /* (nothing visible: zero; not a number: that) */
     T *to = (T *)a.out + b * a.out_stride[0] + (int64_t)query * a.out_stride[1] + head * a.out_stride[2];
@@ -400,7 +431,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split
     }
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(run.o[t]);
-    run.total += other_half(run.total);
+    run.total = sum_halves(run.total);
     /* join the wavefronts: element d of a row's sum lies at [wave][d][row] */
     float *sums = (float *)lds, *tops = sums + WAVES * DP * 32;
     __syncthreads();
@@ -470,7 +501,7 @@ constexpr int FEW_TILES = 3;
 
 /* dQ: queries in registers, keys in tiles as in attend_forward; per block of 32 keys S^T = K Q^T, dP^T = V dO^T,
  * dQ^T += K^T dS^T.  It also leaves delta = sum dO O of every query for attend_dkv. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dq(const Args a) {
+template <class T, int DP> __global__ void __launch_bounds__(LANES) __attribute__((amdgpu_waves_per_eu(2, 2))) attend_dq(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
     const int blocks = (a.queries + QUERIES - 1) / QUERIES, count = a.batch * a.heads * blocks;
@@ -508,7 +539,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dq
     }
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) arrived(qf[s]), arrived(gf[s]);
-    delta += other_half(delta);
+    delta = sum_halves(delta);
     const int64_t flat = ((int64_t)b * a.heads + head) * a.queries + query;
     float lse2 = there ? a.lse[flat] * LOG2E : 0.0f;
     f32x16 dq[DP / 32];
@@ -523,7 +554,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dq
     float sum = 0.0f;
     for (int walk = few ? 0 : 1; walk < 2; ++walk) {
         if (walk == 1) {
-            if (few) delta = sum + other_half(sum);
+            if (few) delta = sum_halves(sum);
             if (there && half == 0) a.delta[flat] = delta;
         }
         if (few && walk == 1) {
@@ -542,11 +573,15 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dq
                 const int key0 = at + n * 32;
                 const uint32_t ktile = buffer_at + n * 32 * PITCH * 2, vtile = ktile + TILE;
                 if (none_see(a, seq.length, lo, hi, key0, key0 + 32)) continue;
+                __builtin_amdgcn_s_setprio(1);
+                __builtin_amdgcn_sched_barrier(0);
                 f32x16 s = {}, dp = {};
 #pragma unroll
                 for (int j = 0; j < DP / 16; ++j) s = Mma<T>::go(ops.rows(ktile, 0, j), qf[j], s);
 #pragma unroll
                 for (int j = 0; j < DP / 16; ++j) dp = Mma<T>::go(ops.rows(vtile, 0, j), gf[j], dp);
+                in_step<DP / 8, 1, 4>();
+                __builtin_amdgcn_s_setprio(0);
                 float ds[16];
                 const float less = walk == 0 ? 0.0f : delta;
 #pragma unroll
@@ -557,12 +592,15 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dq
                     for (int i = 0; i < 16; ++i) sum += ds[i];
                     continue;
                 }
+                const typename Mma<T>::frag df[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
+                __builtin_amdgcn_s_setprio(1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const typename Mma<T>::frag f = pack8<T>(ds + 8 * j);
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) dq[d] = Mma<T>::go(ops.columns(ktile, j * 16, d), f, dq[d]);
-                }
+                    for (int d = 0; d < DP / 32; ++d) dq[d] = Mma<T>::go(ops.columns(ktile, j * 16, d), df[j], dq[d]);
+                in_step<DP / 16, 2, 3>();
+                __builtin_amdgcn_s_setprio(0);
             }
         }
     }
@@ -600,11 +638,15 @@ template <class T, int DP> struct KeyGrads {
     /* `t`: the first query's position from the first one that sees this lane's key; the `count` from there on see it */
     __device__ inline void step(const Operands<T, PITCH> &ops, uint32_t qtile, uint32_t gtile, uint32_t lse, uint32_t delta, float scale2, int t, uint32_t count, bool masked,
                                 int half) {
+        __builtin_amdgcn_s_setprio(1);
+        __builtin_amdgcn_sched_barrier(0);
         f32x16 s = {}, dp = {};
 #pragma unroll
         for (int j = 0; j < DP / 16; ++j) s = Mma<T>::go(ops.rows(qtile, 0, j), kf[j], s);
 #pragma unroll
         for (int j = 0; j < DP / 16; ++j) dp = Mma<T>::go(ops.rows(gtile, 0, j), vf[j], dp);
+        in_step<DP / 8, 1, 4>();
+        __builtin_amdgcn_s_setprio(0);
         float prob[16], ds[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
@@ -619,15 +661,18 @@ template <class T, int DP> struct KeyGrads {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if ((uint32_t)(t + result_row(i, half)) >= count) prob[i] = ds[i] = 0.0f;
+        const typename Mma<T>::frag pf[2] = {pack8<T>(prob), pack8<T>(prob + 8)}, df[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
+        __builtin_amdgcn_s_setprio(1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const typename Mma<T>::frag pf = pack8<T>(prob + 8 * j), df = pack8<T>(ds + 8 * j);
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d) {
-                dv[d] = Mma<T>::go(ops.columns(gtile, j * 16, d), pf, dv[d]);
-                dk[d] = Mma<T>::go(ops.columns(qtile, j * 16, d), df, dk[d]);
+                dv[d] = Mma<T>::go(ops.columns(gtile, j * 16, d), pf[j], dv[d]);
+                dk[d] = Mma<T>::go(ops.columns(qtile, j * 16, d), df[j], dk[d]);
             }
-        }
+        in_step<DP / 8, 2, 2>();
+        __builtin_amdgcn_s_setprio(0);
     }
 };
 
@@ -653,7 +698,7 @@ template <class T, int PITCH, int ROWS, int LANES> struct QueryTiles {
 
 /* The pairs of a window: a workgroup takes 128 keys and walks over the queries whose window they are in, of every head that shares the
  * key head, in tiles of 64. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES, 2) attend_dkv(const Args a) {
+template <class T, int DP> __global__ void __launch_bounds__(LANES) __attribute__((amdgpu_waves_per_eu(2, 2))) attend_dkv(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH;
     typedef QueryTiles<T, PITCH, KEYS, LANES> Queries;
