@@ -85,28 +85,37 @@ __device__ inline u32x4 buffer(const void *p, int64_t bytes) {
                  (uint32_t)__builtin_amdgcn_readfirstlane(bytes < 0 ? 0 : (int)bytes), 0x00027000u};
 }
 
-/* A tile's rows in memory and where the lanes find their pieces of them: ROWS rows of PITCH elements by LANES lanes. */
-template <class T, int PITCH, int ROWS, int LANES> struct Tile {
-    static constexpr int PER = PITCH / 8, LOADS = ROWS * PER / LANES;
-    static_assert(ROWS * PER % LANES == 0, "whole loads");
+/* A tile's rows in memory and where the lanes find their pieces of them: ROWS rows of PITCH elements by LANES lanes.  A lane keeps a
+ * place per load; with ONE, for kernels without registers for that, one for all of them (a load takes a multiple of sixteen
+ * rows then, after which swizzles repeat) and each load has a descriptor of its own rows, some ten scalar operations (which cost
+ * attend_forward 15%). */
+template <class T, int PITCH, int ROWS, int LANES, bool ONE = false> struct Tile {
+    static constexpr int PER = PITCH / 8, LOADS = ROWS * PER / LANES, STEP = LANES / PER, PLACES = ONE ? 1 : LOADS;
+    static_assert(ROWS * PER % LANES == 0 && (!ONE || STEP % 16 == 0), "whole loads");
     const T *base;
     int64_t stride;
     int dim;
-    uint32_t at[LOADS], to;
+    uint32_t at[PLACES], to;
     __device__ inline Tile(const T *b, int64_t s, int d, int lane) : base(b), stride(s), dim(d) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
+        for (int i = 0; i < PLACES; ++i) {
             const int p = i * LANES + lane, row = p / PER, piece = (p % PER) ^ (swizzle<PITCH>(row) & (PER - 1));
             at[i] = piece * 8 < d ? (uint32_t)(row * (int)s + piece * 8) * 2u : 0x80000000u;   /* (past every descriptor's end) */
         }
         to = (lane & ~63) * 16;
     }
+    __device__ inline u32x4 rows(int row0, int end, int most) const {
+        const int n = end - row0 < most ? end - row0 : most;
+        return buffer(base + (int64_t)row0 * stride, n > 0 ? ((int64_t)(n - 1) * stride + dim) * 2 : 0);
+    }
     __device__ inline void ask(uint32_t lds, int row0, int end) const {
-        const int rows = end - row0 < ROWS ? end - row0 : ROWS;
-        const u32x4 b = buffer(base + (int64_t)row0 * stride, rows > 0 ? ((int64_t)(rows - 1) * stride + dim) * 2 : 0);
         const uint32_t at_lds = __builtin_amdgcn_readfirstlane(lds + to);
+        u32x4 b;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) to_lds16(b, at[i], at_lds + i * LANES * 16);
+        for (int i = 0; i < LOADS; ++i) {
+            if (i == 0 || ONE) b = ONE ? rows(row0 + i * STEP, end, STEP) : rows(row0, end, ROWS);
+            to_lds16(b, at[ONE ? 0 : i], at_lds + i * LANES * 16);
+        }
     }
 };
 
@@ -322,11 +331,15 @@ template <class T> __device__ inline void store4(T *to, float a, float b, float 
 
 template <int DP> struct Shape { static constexpr int PITCH = DP <= 64 ? 64 : 128; };
 
+/* How many wavefronts of a SIMD a kernel is scheduled for: exactly as many as its registers allow, so that what is left of them goes to
+ * operands on their way. */
+#define RESIDENT(DP) __attribute__((amdgpu_waves_per_eu((DP) <= 64 ? 3 : 2, (DP) <= 64 ? 3 : 2)))
+
 constexpr int WAVES = 4, LANES = WAVES * 64, QUERIES = WAVES * 32, KEYS = 64;
 
 /* Prompts: a workgroup takes 128 queries of a head, 32 per wavefront, and walks over its keys in tiles of 64, the next tile on its
  * way while one is worked on. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES) __attribute__((amdgpu_waves_per_eu(2, 2))) attend_forward(const Args a) {
+template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_forward(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
     const int blocks = (a.queries + QUERIES - 1) / QUERIES, count = a.batch * a.heads * blocks;
@@ -501,7 +514,7 @@ constexpr int FEW_TILES = 3;
 
 /* dQ: queries in registers, keys in tiles as in attend_forward; per block of 32 keys S^T = K Q^T, dP^T = V dO^T,
  * dQ^T += K^T dS^T.  It also leaves delta = sum dO O of every query for attend_dkv. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES) __attribute__((amdgpu_waves_per_eu(2, 2))) attend_dq(const Args a) {
+template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_dq(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
     const int blocks = (a.queries + QUERIES - 1) / QUERIES, count = a.batch * a.heads * blocks;
@@ -678,15 +691,15 @@ template <class T, int DP> struct KeyGrads {
 
 /* Tiles of queries: rows of q and of the answer's gradient, then log-sums and deltas, by LANES lanes. */
 template <class T, int PITCH, int ROWS, int LANES> struct QueryTiles {
-    static constexpr int BYTES = ROWS * PITCH * 2, STAGE = 2 * BYTES + 2 * 256, LOADS = 2 * Tile<T, PITCH, ROWS, LANES>::LOADS + (LANES == 64 ? 2 : 1);
-    Tile<T, PITCH, ROWS, LANES> q, g;
+    static constexpr int BYTES = ROWS * PITCH * 2, STAGE = 2 * BYTES + 2 * 256, LOADS = 2 * Tile<T, PITCH, ROWS, LANES, LANES != 64>::LOADS + (LANES == 64 ? 2 : 1);
+    Tile<T, PITCH, ROWS, LANES, LANES != 64> q, g;
     const float *lse, *delta;
     __device__ inline QueryTiles(const Args &a, int b, int lane)
         : q((const T *)a.q + b * a.q_stride[0], a.q_stride[1], a.dim, lane), g((const T *)a.g + b * a.g_stride[0], a.g_stride[1], a.dim, lane),
           lse(a.lse + (int64_t)b * a.heads * a.queries), delta(a.delta + (int64_t)b * a.heads * a.queries) {}
     /* (a workgroup's four wavefronts: each asks for as many loads, the last two for those of the first two again) */
     __device__ inline void ask(const Args &a, uint32_t lds, int head, int row, int wave, int lane) const {
-        Tile<T, PITCH, ROWS, LANES> qh = q, gh = g;
+        Tile<T, PITCH, ROWS, LANES, LANES != 64> qh = q, gh = g;
         qh.base += head * a.q_stride[2], gh.base += head * a.g_stride[2];
         qh.ask(lds, row, a.queries), gh.ask(lds + BYTES, row, a.queries);
         const int64_t at = (int64_t)head * a.queries + row;
@@ -697,24 +710,25 @@ template <class T, int PITCH, int ROWS, int LANES> struct QueryTiles {
 };
 
 /* The pairs of a window: a workgroup takes 128 keys and walks over the queries whose window they are in, of every head that shares the
- * key head, in tiles of 64. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES) __attribute__((amdgpu_waves_per_eu(2, 2))) attend_dkv(const Args a) {
+ * key head, in tiles of 64.  With SHARE 2 it takes 64 keys, and two wavefronts share 32 keys and halve each tile's queries: twice the
+ * workgroups, for calls that would leave CUs without one. */
+template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_dkv(const Args a) {
     extern __shared__ char lds[];
-    constexpr int PITCH = Shape<DP>::PITCH;
+    constexpr int PITCH = Shape<DP>::PITCH, OWN = QUERIES / SHARE;
     typedef QueryTiles<T, PITCH, KEYS, LANES> Queries;
-    const int blocks = (a.keys + QUERIES - 1) / QUERIES, count = a.batch * a.kv_heads * blocks;
+    const int blocks = (a.keys + OWN - 1) / OWN, count = a.batch * a.kv_heads * blocks;
     const int work = place(count);
     if (work >= count) return;
     const int block = work % blocks, kv = work / blocks % a.kv_heads, b = work / blocks / a.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Sequence seq = sequence(a, b);
-    const int k0 = block * QUERIES, mine = k0 + wave * 32, key = mine + (lane & 31);
+    const int k0 = block * OWN, mine = k0 + wave % (WAVES / SHARE) * 32, key = mine + (lane & 31);
     const T *krow = (const T *)a.k + b * a.k_stride[0] + (int64_t)key * a.k_stride[1] + kv * a.k_stride[2];
     const T *vrow = (const T *)a.v + b * a.v_stride[0] + (int64_t)key * a.v_stride[1] + kv * a.v_stride[2];
     /* queries from the first key's position on, up to the last key's window */
     int from = k0 - seq.start, to = a.queries;
     if (a.window > 0) {
-        const int64_t most = (int64_t)k0 + QUERIES - 1 + a.window - seq.start;
+        const int64_t most = (int64_t)k0 + OWN - 1 + a.window - seq.start;
         to = most < to ? (int)most : to;
     }
     from = from < 0 ? 0 : from;
@@ -739,18 +753,40 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) __attribute_
         meet();
         if (t + 1 < steps) ask(t + 1);
         const uint32_t buffer_at = lds0 + (t & 1) * Queries::STAGE;
-        if (mine < seq.length)
+        auto half_tile = [&](int n) {
+            const int lo = seq.start + q + n * 32, hi = lo + 31;
+            if (mine >= seq.length || q + n * 32 >= a.queries || hi < mine || (a.window > 0 && lo - (mine + 31) >= a.window)) return;
+            const bool masked = q + n * 32 + 32 > a.queries || mine + 32 > seq.length || lo < mine + 31 || (a.window > 0 && hi - mine >= a.window);
+            const uint32_t qtile = buffer_at + n * 32 * PITCH * 2, lse = buffer_at + 2 * Queries::BYTES + n * 32 * 4;
+            grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + 256, a.scale2, lo - key, sight, masked, half);
+        };
+        if (SHARE == 2) half_tile(wave >> 1);
+        else
 #pragma unroll 1
-            for (int n = 0; n < KEYS / 32; ++n) {
-                const int lo = seq.start + q + n * 32, hi = lo + 31;
-                if (q + n * 32 >= a.queries || hi < mine || (a.window > 0 && lo - (mine + 31) >= a.window)) continue;
-                const bool masked = q + n * 32 + 32 > a.queries || mine + 32 > seq.length || lo < mine + 31 || (a.window > 0 && hi - mine >= a.window);
-                const uint32_t qtile = buffer_at + n * 32 * PITCH * 2, lse = buffer_at + 2 * Queries::BYTES + n * 32 * 4;
-                grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + 256, a.scale2, lo - key, sight, masked, half);
-            }
+            for (int n = 0; n < KEYS / 32; ++n) half_tile(n);
         q = q + KEYS < (first + per_head) * KEYS ? q + KEYS : first * KEYS;
     }
     grads.stop();
+    if (SHARE == 2) {
+        /* the second two wavefronts' sums go to the first two's, dK and then dV */
+        float *sums = (float *)lds + (wave & 1) * DP * 32 + (lane & 31);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            meet();
+            if (wave >= 2)
+#pragma unroll
+                for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sums[(t * 32 + result_row(i, half)) * 32] = which ? grads.dv[t][i] : grads.dk[t][i];
+            meet();
+            if (wave < 2)
+#pragma unroll
+                for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) (which ? grads.dv : grads.dk)[t][i] += sums[(t * 32 + result_row(i, half)) * 32];
+        }
+        if (wave >= 2) return;
+    }
     if (key >= a.keys) return;
     /* what queries beyond the window have left for a first key */
     if (a.far_parts > 0 && mine < a.sinks) {
@@ -908,13 +944,14 @@ void far_of(const ace_attend_t *a, Args &k) {
     parts = parts < most ? parts : most;
     k.far_parts = parts < 1 ? 1 : parts > 32 ? 32 : (int)parts;
 }
+constexpr int SHARED_BELOW = 384;
 int width_of(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 int64_t delta_floats(const ace_attend_t *a) { return ((int64_t)a->batch * a->heads * a->queries + 3) / 4 * 4; }
 
 template <class T, int DP> int backward(const Args &k, hipStream_t stream) {
     constexpr int PITCH = Shape<DP>::PITCH, DQ = 4 * KEYS * PITCH * 2, DKV = 2 * QueryTiles<T, PITCH, KEYS, LANES>::STAGE;
     constexpr int FAR_TILES = WAVES * 2 * QueryTiles<T, PITCH, 32, 64>::STAGE, FAR_JOIN = WAVES * DP * 32 * 4, FAR = FAR_TILES > FAR_JOIN ? FAR_TILES : FAR_JOIN;
-    static const int ready = with_lds(attend_dq<T, DP>, DQ), ready2 = with_lds(attend_dkv<T, DP>, DKV), ready3 = with_lds(attend_far<T, DP>, FAR);
+    static const int ready = with_lds(attend_dq<T, DP>, DQ), ready2 = with_lds(attend_dkv<T, DP, 1>, DKV) | with_lds(attend_dkv<T, DP, 2>, DKV), ready3 = with_lds(attend_far<T, DP>, FAR);
     if (ready != ACE_OK || ready2 != ACE_OK || ready3 != ACE_OK) return ACE_EHIP;
     int rc = ACE_OK;
     if (k.queries > 0) {
@@ -927,7 +964,9 @@ template <class T, int DP> int backward(const Args &k, hipStream_t stream) {
         attend_far<T, DP><<<dim3(k.far_parts, k.kv_heads * k.far_blocks, k.batch), LANES, FAR, stream>>>(k);
         if ((rc = layer_launched()) != ACE_OK) return rc;
     }
-    attend_dkv<T, DP><<<places((int64_t)k.batch * k.kv_heads * ((k.keys + QUERIES - 1) / QUERIES)), LANES, DKV, stream>>>(k);
+    const int64_t heads = (int64_t)k.batch * k.kv_heads, groups = heads * ((k.keys + QUERIES - 1) / QUERIES);
+    if (groups < SHARED_BELOW) attend_dkv<T, DP, 2><<<places(heads * ((k.keys + QUERIES / 2 - 1) / (QUERIES / 2))), LANES, DKV, stream>>>(k);
+    else attend_dkv<T, DP, 1><<<places(groups), LANES, DKV, stream>>>(k);
     return layer_launched();
 }
 
