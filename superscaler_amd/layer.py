@@ -14,6 +14,7 @@ sizes raise ValueError, other types TypeError, a missing library or a HIP failur
 import ctypes
 import math
 import os
+import struct
 from typing import NamedTuple, Optional
 
 import numpy as np
@@ -37,9 +38,9 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
 
-class _BlockNorm(ctypes.Structure):
-    _fields_ = [("rows", _i64), ("rows_per_gate", _i64), ("width", _i32), ("dtype", _i32), ("layer", _i32), ("residual_scale", _f32), ("eps", _f32),
-                ("d_x", _vp), ("d_block", _vp), ("d_gate", _vp), ("d_exit_weight", _vp), ("d_exit_bias", _vp), ("d_entry_weight", _vp), ("d_entry_bias", _vp)]
+# ace_block_norm_t: rows, rows_per_gate; width, dtype, layer; residual_scale, eps; seven pointers (packed: a third of the time that a
+# ctypes structure takes, on a call that a single token waits for)
+_BLOCK_NORM = struct.Struct("=2q3i2f4x7Q")
 
 
 class _Attend(ctypes.Structure):
@@ -83,14 +84,17 @@ def load_library():
     return lib
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(device, name, *args):
     """A call of the library on `device` and its current stream."""
-    lib = load_library()
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+    lib, index = _lib or load_library(), device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            rc = getattr(lib, name)(*args, _raw_stream(index))
     else:
-        rc = getattr(lib, name)(*args, torch.cuda.current_stream(device).cuda_stream)
+        rc = getattr(lib, name)(*args, _raw_stream(index))
     if rc != 0:
         hip = lib.ace_layer_last_hip_error().decode() if rc == -3 else ""
         raise AceError(f"{name}: {lib.ace_layer_strerror(rc).decode()}" + (f" ({hip})" if hip else ""))
@@ -135,7 +139,12 @@ def _rows_per_gate(gate_shape, shape):
     return None
 
 
-def _block_norm_args(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind, eps):
+def _fits(t, dtype, device, shape):
+    return t is None or (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and (shape is None or t.shape == shape))
+
+
+def _refuse_block_norm(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind):
+    """Says what is wrong with arguments that do not fit together."""
     _on_gpu(x, "x")
     if x.dtype not in _TYPES:
         raise TypeError(f"x: float32, bfloat16 or float16 expected, not {x.dtype}")
@@ -143,9 +152,9 @@ def _block_norm_args(x, block, residual_scale, gate, exit_weight, exit_bias, ent
         raise ValueError(f"kind: 'layer' or 'rms' expected, not {kind!r}")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
         raise ValueError(f"x: rows of 1 to {MAX_WIDTH} elements expected, got shape {tuple(x.shape)}")
-    shape, width = tuple(x.shape), x.shape[-1]
-    for name, t, size in (("block", block, shape), ("gate", gate, None), ("exit_weight", exit_weight, (width,)), ("exit_bias", exit_bias, (width,)),
-                          ("entry_weight", entry_weight, (width,)), ("entry_bias", entry_bias, (width,))):
+    width = tuple(x.shape[-1:])
+    for name, t, size in (("block", block, tuple(x.shape)), ("gate", gate, None), ("exit_weight", exit_weight, width), ("exit_bias", exit_bias, width),
+                          ("entry_weight", entry_weight, width), ("entry_bias", entry_bias, width)):
         if t is None:
             continue
         _on_gpu(t, name)
@@ -159,16 +168,28 @@ def _block_norm_args(x, block, residual_scale, gate, exit_weight, exit_bias, ent
         raise ValueError("a gate, an exit norm and a residual scale go with a block")
     if (exit_bias is not None and exit_weight is None) or (entry_bias is not None and entry_weight is None):
         raise ValueError("a bias goes with its norm's weight")
-    if block is None and entry_weight is None:
-        raise ValueError("neither a block nor an entry norm: nothing to compute")
+    raise ValueError("neither a block nor an entry norm: nothing to compute")
+
+
+def _block_norm_args(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind, eps):
+    """(packed arguments, the tensors whose addresses they hold, rows)"""
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _TYPES and x.dim() > 0 and 1 <= x.shape[-1] <= MAX_WIDTH and kind in ("layer", "rms")):
+        _refuse_block_norm(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind)
+    dtype, device, shape = x.dtype, x.device, x.shape
+    width = shape[-1:]
+    if not (_fits(block, dtype, device, shape) and _fits(gate, dtype, device, None) and _fits(exit_weight, dtype, device, width) and
+            _fits(exit_bias, dtype, device, width) and _fits(entry_weight, dtype, device, width) and _fits(entry_bias, dtype, device, width)) or \
+            (exit_bias is not None and exit_weight is None) or (entry_bias is not None and entry_weight is None) or \
+            (block is None and (entry_weight is None or gate is not None or exit_weight is not None or residual_scale != 1.0)):
+        _refuse_block_norm(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind)
     per_gate = 1
     if gate is not None:
-        per_gate = _rows_per_gate(tuple(gate.shape), shape)
+        per_gate = _rows_per_gate(tuple(gate.shape), tuple(shape))
         if per_gate is None:
-            raise ValueError(f"gate: one row for all of x, or for each of its leading indices, expected; got {tuple(gate.shape)} for x {shape}")
+            raise ValueError(f"gate: one row for all of x, or for each of its leading indices, expected; got {tuple(gate.shape)} for x {tuple(shape)}")
     keep = [t if t is None else t.contiguous() for t in (x, block, gate, exit_weight, exit_bias, entry_weight, entry_bias)]
-    rows = x.numel() // width
-    a = _BlockNorm(rows, per_gate, width, _TYPES[x.dtype], kind == "layer", residual_scale, eps, *map(_pointer, keep))
+    rows = x.numel() // width[0]
+    a = _BLOCK_NORM.pack(rows, per_gate, width[0], _TYPES[dtype], kind == "layer", residual_scale, eps, *[0 if t is None else t.data_ptr() for t in keep])
     return a, keep, rows
 
 
@@ -184,10 +205,11 @@ def block_norm(x, block=None, *, residual_scale=1.0, gate=None, exit_weight=None
     [width], or one for each of x's leading indices ([batch, width] for x [batch, length, width], or x's own shape).  All tensors are
     of one type; `normed` is computed from the residual before that is rounded to it."""
     a, keep, rows = _block_norm_args(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind, eps)
-    residual = x if block is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    normed = None if entry_weight is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device)
-    _call(x.device, "ace_block_norm_forward", ctypes.byref(a), None if block is None else residual.data_ptr(), _pointer(normed), stats.data_ptr())
+    x0 = keep[0]   # (contiguous: so is what is made like it)
+    residual = x if block is None else torch.empty_like(x0)
+    normed = None if entry_weight is None else torch.empty_like(x0)
+    stats = x0.new_empty((rows, 4), dtype=torch.float32)
+    _call(x0.device, "ace_block_norm_forward", a, None if block is None else residual.data_ptr(), _pointer(normed), stats.data_ptr())
     return BlockNorm(residual, normed, stats)
 
 
@@ -214,8 +236,8 @@ def block_norm_backward(d_residual, d_normed, x, block, stats, *, residual_scale
     lib = load_library()
     out = [None if t is None else (torch.zeros if rows == 0 else torch.empty)(t.shape, dtype=t.dtype, device=t.device)
            for t in (x, block, gate, exit_weight, exit_bias, entry_weight, entry_bias)]
-    workspace = torch.empty(lib.ace_block_norm_workspace_bytes(ctypes.byref(a)), dtype=torch.uint8, device=x.device)
-    _call(x.device, "ace_block_norm_backward", ctypes.byref(a), *map(_pointer, grads), stats.data_ptr(), *map(_pointer, out), workspace.data_ptr(),
+    workspace = torch.empty(lib.ace_block_norm_workspace_bytes(a), dtype=torch.uint8, device=x.device)
+    _call(x.device, "ace_block_norm_backward", a, *map(_pointer, grads), stats.data_ptr(), *map(_pointer, out), workspace.data_ptr(),
           workspace.numel())
     return BlockNormGrads(*out)
 

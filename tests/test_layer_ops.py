@@ -51,18 +51,16 @@ def test_refusals_of_the_c_entries():
     """Everything here is refused before a kernel would be launched."""
     lib = layer.load_library()
     assert lib.ace_layer_strerror(-1) == b"invalid argument" and lib.ace_layer_strerror(-99) == b"unknown error"
-    n = layer._BlockNorm(4, 1, 8, 1, 1, 1.0, 1e-5, 64, 64)
+
+    def norm(rows=4, width=8, dtype=1):
+        return layer._BLOCK_NORM.pack(rows, 1, width, dtype, 1, 1.0, 1e-5, 64, 64, 0, 0, 0, 0, 0)      # x and a block
     assert lib.ace_block_norm_forward(None, 64, 64, 64, None) == -1
-    assert lib.ace_block_norm_forward(ctypes.byref(n), None, None, 64, None) == -1          # a block, and nowhere to write its residual
-    n.width = layer.MAX_WIDTH + 1
-    assert lib.ace_block_norm_forward(ctypes.byref(n), 64, None, 64, None) == -2
-    n.width, n.dtype = 8, 3
-    assert lib.ace_block_norm_forward(ctypes.byref(n), 64, None, 64, None) == -1
-    n.dtype, n.rows = 1, 0
-    assert lib.ace_block_norm_forward(ctypes.byref(n), 64, None, 64, None) == 0             # no rows
-    n.rows = 4
-    assert lib.ace_block_norm_backward(ctypes.byref(n), 64, None, 64, 64, 64, None, None, None, None, None, None, 0, None) == -1   # no workspace
-    assert lib.ace_block_norm_workspace_bytes(ctypes.byref(n)) == 2 * 4 * 8 * 4
+    assert lib.ace_block_norm_forward(norm(), None, None, 64, None) == -1          # nowhere to write the residual
+    assert lib.ace_block_norm_forward(norm(width=layer.MAX_WIDTH + 1), 64, None, 64, None) == -2
+    assert lib.ace_block_norm_forward(norm(dtype=3), 64, None, 64, None) == -1
+    assert lib.ace_block_norm_forward(norm(rows=0), 64, None, 64, None) == 0       # no rows
+    assert lib.ace_block_norm_backward(norm(), 64, None, 64, 64, 64, None, None, None, None, None, None, 0, None) == -1   # no workspace
+    assert lib.ace_block_norm_workspace_bytes(norm()) == 2 * 4 * 8 * 4
 
     def attend(**change):
         a = layer._Attend(2, 32, 32, 4, 2, 64, 1, 0, 0, 0.125)
