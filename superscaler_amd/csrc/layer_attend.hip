@@ -229,11 +229,14 @@ __device__ inline void hide(float *s, const Sight &sight, int key0, int half, bo
 }
 
 /* Work in an order that keeps a head's blocks, which read the same keys, on one of the eight dies and its cache: workgroups go to
- * the dies in turn, so die d gets the d-th eighth of the work.  Returns count where a workgroup has nothing to do. */
+ * the dies in turn, so die d gets the d-th eighth of the work.  On a die they go to its 32 CUs in turn: every other 32 are
+ * taken in reverse, so that a CU's second workgroup is short where its first is long (blocks at the beginning of a sequence see few
+ * keys).  Returns count where a workgroup has nothing to do. */
 __device__ inline int place(int count) {
-    const int per = (count + 7) / 8;
-    const int at = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-    return blockIdx.x / 8 < (unsigned)per && at < count ? at : count;
+    const int per = (count + 7) / 8, turn = (int)(blockIdx.x / 8), group = turn / 32 * 32;
+    const int left = per - group < 32 ? per - group : 32;
+    const int at = (int)(blockIdx.x % 8) * per + (group & 32 ? group + left - 1 - turn % 32 : turn);
+    return turn < per && at < count ? at : count;
 }
 inline int places(int64_t count) { return (int)((count + 7) / 8 * 8); }
 
