@@ -57,7 +57,7 @@ template <int BITS, class G, class C> __global__ void __launch_bounds__(LANES) a
     C *copy = (C *)t.d_copy;
     const float gs = a.grad_scale ? *a.grad_scale : 1.0f;
     const int64_t base = (chunk - t.first_chunk) * ACE_ADAMW_CHUNK;
-#pragma unroll 2
+#pragma unroll 1
     for (int pass = 0; pass < ACE_ADAMW_CHUNK / PASS; ++pass) {
         const int64_t at = base + pass * PASS + threadIdx.x * 8;
         const int64_t left = t.n - at;

@@ -159,11 +159,14 @@ template <class T> __device__ inline typename Mma<T>::frag global_frag(const T *
 
 __device__ inline int result_row(int i, int half) { return 8 * (i / 4) + 4 * half + i % 4; }
 
+/* Queries and keys number up to MOST.  A sequence that begins further before the first key than that has no query that sees one; past
+ * LATEST positions are taken as beginning there, and a window as the first that holds every key from there on: no sum or difference of
+ * positions, lengths and a window leaves 32 bits. */
+constexpr int MOST = 1 << 28, LATEST = 1 << 30, WIDEST = LATEST + MOST;
 struct Sequence { int start, length; };
 __device__ inline Sequence sequence(const Args &a, int b) {
-    const int length = a.length ? a.length[b] : a.keys;
-    const int start = a.start ? a.start[b] : a.keys - a.queries, far = 1 << 30;   /* (positions as far off as that keep their order) */
-    return {start < -far ? -far : start > far ? far : start, length < 0 ? 0 : length > a.keys ? a.keys : length};
+    const int length = a.length ? a.length[b] : a.keys, start = a.start ? a.start[b] : a.keys - a.queries;
+    return {start < -MOST ? -MOST : start > LATEST ? LATEST : start, length < 0 ? 0 : length > a.keys ? a.keys : length};
 }
 
 /* The order of a run of PRODUCTS matrix products whose operands come from LDS in READS reads each: operands of LEAD products are on
@@ -209,7 +212,7 @@ struct Sight {
     uint32_t count;
     __device__ inline Sight(const Args &a, int length, int p) {
         const int end = p + 1 < length ? p + 1 : length;
-        from = a.window > 0 ? p - a.window + 1 : 0;
+        from = a.window > 0 && p >= a.window ? p - a.window + 1 : 0;
         count = end > from ? end - from : 0;
         first = a.window > 0 ? (a.sinks < end ? a.sinks : end) : 0;
     }
@@ -873,7 +876,7 @@ int check(const ace_attend_t *a) {
     if (!a || a->batch < 0 || a->queries < 0 || a->keys < 0 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads) return ACE_EINVAL;
     if (a->dim < 8 || a->dim % 8 || a->window < 0 || a->sinks < 0 || (a->dtype != ACE_T_BF16 && a->dtype != ACE_T_F16)) return ACE_EINVAL;
     if (!(a->scale > 0.0f) || a->scale > 1e30f) return ACE_EINVAL;
-    if (a->dim > 128 || a->queries > (1 << 30) || a->keys > (1 << 30)) return ACE_ETOOBIG;
+    if (a->dim > 128 || a->queries > MOST || a->keys > MOST) return ACE_ETOOBIG;
     /* (a tile of 64 rows is named by 32-bit places) */
     const int64_t widest = (int64_t)1 << 23;
     if (a->q_stride[1] >= widest || a->k_stride[1] >= widest || a->v_stride[1] >= widest || a->q_stride[1] < 0 || a->k_stride[1] < 0 || a->v_stride[1] < 0) return ACE_ETOOBIG;
@@ -890,26 +893,43 @@ int check(const ace_attend_t *a) {
 Args args_of(const ace_attend_t *a) {
     Args k = {};
     k.batch = a->batch, k.queries = a->queries, k.keys = a->keys, k.heads = a->heads, k.kv_heads = a->kv_heads, k.dim = a->dim;
-    k.shared = a->heads / a->kv_heads, k.window = a->window, k.sinks = a->sinks, k.scale = a->scale, k.scale2 = a->scale * LOG2E;
+    k.shared = a->heads / a->kv_heads, k.window = a->window < WIDEST ? a->window : WIDEST, k.sinks = a->sinks, k.scale = a->scale, k.scale2 = a->scale * LOG2E;
     k.start = a->d_start, k.length = a->d_length;
     for (int i = 0; i < 3; ++i) k.q_stride[i] = a->q_stride[i], k.k_stride[i] = a->k_stride[i], k.v_stride[i] = a->v_stride[i], k.out_stride[i] = a->out_stride[i];
     k.q = a->d_q, k.k = a->d_k, k.v = a->d_v, k.out = a->d_out, k.lse = a->d_lse;
     return k;
 }
 
-/* Few queries go to attend_split. */
-constexpr int SPLIT_QUERIES = 16;
-bool few(const ace_attend_t *a) { return a->queries <= SPLIT_QUERIES; }
+int row_blocks(const ace_attend_t *a) { return (int)(((int64_t)a->queries * (a->heads / a->kv_heads) + 31) / 32); }
 
-int row_blocks(const ace_attend_t *a) { return (a->queries * (a->heads / a->kv_heads) + 31) / 32; }
+/* the most keys that a query's block can see */
+int64_t most_seen(const ace_attend_t *a) {
+    const int64_t seen = (int64_t)a->window + a->queries + a->sinks;
+    return a->window > 0 && seen < a->keys ? seen : a->keys;
+}
 
+/* How many workgroups attend_split takes for a key head's block of rows: no more than there are CUs for (LDS holds one of these
+ * workgroups), and two tiles or more for a wavefront.  32 x 8 heads of 8,192 keys (256 blocks) in one part each: 180 us, in two:
+ * 187; 24 x 4 heads of 4,096 (96 blocks) in two: 38, in three, some CUs with a second one: 47; 4 x 40 heads of 2,048 (160 blocks)
+ * in one: 29, in two: 39, in four: 40. */
 int splits_of(const ace_attend_t *a) {
-    int64_t seen = a->window > 0 ? (int64_t)a->window + a->queries + a->sinks : a->keys;
-    seen = seen < a->keys ? seen : a->keys;
-    const int64_t groups = (int64_t)a->batch * a->kv_heads * row_blocks(a), most = (seen + SPLIT_KEYS * WAVES * 2 - 1) / (SPLIT_KEYS * WAVES * 2);
-    int64_t splits = (512 + groups - 1) / groups;
+    const int64_t groups = (int64_t)a->batch * a->kv_heads * row_blocks(a), most = (most_seen(a) + SPLIT_KEYS * WAVES * 2 - 1) / (SPLIT_KEYS * WAVES * 2);
+    int64_t splits = 256 / groups;
     splits = splits < most ? splits : most;
     return splits < 1 ? 1 : splits > 64 ? 64 : (int)splits;
+}
+
+/* Whether few queries go to attend_split, which reads a key once for all the heads that share it and splits the keys, or to
+ * attend_forward, which reads them once per head: by what each would take.  While a CU waits for memory more than it computes, a step of
+ * a workgroup of attend_split, 128 keys, takes about 2.4 us and its join 6, one of attend_forward, 64 keys, 1.3 us.  Measured, split
+ * and forward: 32 x 32 heads on 8 of 8,192 keys, 1 query: 187 and 342 us, 16: 301 and 339, 24: 481 and 342, 64: 1,227 and 489; 40 heads of
+ * 2,048 keys, 1: 26 and 42, 128: 38 and 45; 32 heads on 4 of 32,768, 128: 166 and 625; 16 x 16 heads, a window of 512, 64: 32 and 21. */
+bool few(const ace_attend_t *a) {
+    if (a->queries > QUERIES || a->batch > 65535 || (int64_t)a->kv_heads * row_blocks(a) > 65535) return false;
+    const int64_t groups = (int64_t)a->batch * a->kv_heads * row_blocks(a), heads = (int64_t)a->batch * a->heads, splits = splits_of(a), seen = most_seen(a);
+    const int64_t split = (groups * splits + 255) / 256 * ((seen + SPLIT_KEYS * WAVES * splits - 1) / (SPLIT_KEYS * WAVES * splits)) * 24 + (splits > 1 ? 60 : 0);
+    const int64_t whole = (heads + 511) / 512 * ((seen + KEYS - 1) / KEYS) * 13;
+    return split < whole;
 }
 
 template <class K> int with_lds(K kernel, int bytes) { return layer_hip_status(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)); }
@@ -926,7 +946,6 @@ template <class T, int DP> int forward(Args &k, const ace_attend_t *a, hipStream
     constexpr int TILES = WAVES * 4 * SPLIT_KEYS * PITCH * 2, JOIN = (WAVES * DP * 32 + WAVES * 2 * 32) * 4, LDS = TILES > JOIN ? TILES : JOIN;
     static const int ready = with_lds(attend_split<T, DP>, LDS);
     if (ready != ACE_OK) return ready;
-    if (k.batch > 65535 || (int64_t)k.kv_heads * k.row_blocks > 65535) return ACE_ETOOBIG;
     attend_split<T, DP><<<dim3(k.splits, k.kv_heads * k.row_blocks, k.batch), LANES, LDS, stream>>>(k);
     int rc = layer_launched();
     if (rc != ACE_OK || k.splits == 1) return rc;
@@ -935,18 +954,21 @@ template <class T, int DP> int forward(Args &k, const ace_attend_t *a, hipStream
     return layer_launched();
 }
 
-/* Blocks of 32 first keys, and over how many workgroups the queries beyond their window go: about two for every CU, at least four
- * tiles of queries for a wavefront. */
+/* Blocks of 32 first keys, and over how many workgroups the queries beyond their window go: as many as there are CUs, at least four
+ * tiles of queries for a wavefront.  (4 x 40 heads of 2,048 queries, all of the backward pass: 495 us; with two workgroups for every CU
+ * 513.  4 heads of 4 x 16,384: 369 us in up to 32 parts, 391 in up to 16.) */
 void far_of(const ace_attend_t *a, Args &k) {
     const int64_t sinks = a->window > 0 ? (a->sinks < a->keys ? a->sinks : a->keys) : 0;
     k.far_blocks = (int)((sinks + 31) / 32), k.far_parts = 0;
     if (sinks == 0 || a->batch == 0 || a->queries == 0) return;
     const int64_t groups = (int64_t)a->batch * a->kv_heads * k.far_blocks, tiles = (int64_t)(a->heads / a->kv_heads) * ((a->queries + 31) / 32);
-    int64_t parts = (512 + groups - 1) / groups;
+    int64_t parts = 256 / groups;
     const int64_t most = (tiles + WAVES * 4 - 1) / (WAVES * 4);
     parts = parts < most ? parts : most;
     k.far_parts = parts < 1 ? 1 : parts > 32 ? 32 : (int)parts;
 }
+/* Fewer workgroups of 128 keys than this: half as many keys for each.  Measured, all of the backward pass, 128 keys and 64, at
+ * 512 workgroups (2 x 16 heads of 2,048 keys, a window of 512): 110 and 120 us; at 256: 83 and 77; at 64 (4 key heads): 175 and 131. */
 constexpr int SHARED_BELOW = 384;
 int width_of(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 int64_t delta_floats(const ace_attend_t *a) { return ((int64_t)a->batch * a->heads * a->queries + 3) / 4 * 4; }

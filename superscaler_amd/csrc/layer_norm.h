@@ -22,21 +22,24 @@ int norm_backward_launch(const NormArgs &a, int dtype, hipStream_t stream);
 /* A row's lanes hold NV vectors of eight elements each, at distances of the workgroup: as few vectors and lanes as hold the row.
  * Up to 12,288 elements of 16 bits (7,680 of 32) the parameters lie in LDS beside the row and its sums in a lane's registers: one
  * vector per lane of up to 1,024, two of up to 768 lanes, whose 168 registers the backward pass needs.  Longer rows read the
- * parameters where they are and ask for no row ahead.  CAP: the most lanes of a variant. */
-struct NormShape { int cap, nv, lanes; };
-inline NormShape norm_shape(int width, int bytes) {
-    const int v = (width + 7) / 8;
-    const int nv = bytes == 2 ? (v <= 1024 ? 1 : v <= 1536 ? 2 : v <= 3072 ? 3 : 4) : (v <= 960 ? 1 : v <= 3072 ? 3 : 4);
-    return {nv == 1 && v <= 256 ? 256 : nv == 2 ? 768 : 1024, nv, ((v + nv - 1) / nv + 63) / 64 * 64};
+ * parameters where they are and ask for no row ahead: at 12,288 that takes 161 us instead of 155 forward and 737 instead of 285 backward
+ * (8,192 rows of bfloat16; at 7,680 of float32 223 and 195, 830 and 314).  Forward, two vectors per lane begin where one would need
+ * more than 768 lanes, of which a CU holds one workgroup: 16,384 rows of 8,192 in 201 us instead of 231, of 6,656 in 177 instead of 216, of
+ * 6,144 in 171 against 156.  Backward the sums of a second vector cost more than that: 379 us against 320 at 8,192. */
+struct NormShape { int nv, lanes; };
+inline NormShape norm_shape(int width, int bytes, bool forward) {
+    const int v = (width + 7) / 8, one = forward ? 768 : 1024;
+    const int nv = bytes == 2 ? (v <= one ? 1 : v <= 1536 ? 2 : v <= 3072 ? 3 : 4) : (v <= 960 ? 1 : v <= 3072 ? 3 : 4);
+    return {nv, ((v + nv - 1) / nv + 63) / 64 * 64};
 }
 template <int NV> constexpr bool norm_params_in_lds() { return NV <= 2; }
 /* a parameter's elements in LDS: a vector for every lane, whether the row reaches it or not */
 inline int norm_pitch(const NormShape &s) { return s.lanes * s.nv * 8; }
 
-#define NORM_FOR_SHAPE(CALL)                                              \
-    const NormShape shape = norm_shape(a.width, sizeof(T));               \
-    if (shape.cap == 256) NORM_EVEN(CALL, 256, 1)                         \
-    else if (shape.nv == 1) NORM_EVEN(CALL, 1024, 1)                      \
+/* CALL(CAP, NV, EVEN), CAP: the most lanes that a variant is launched with */
+#define NORM_FOR_SHAPE(CALL, FORWARD)                                     \
+    const NormShape shape = norm_shape(a.width, sizeof(T), FORWARD);      \
+    if (shape.nv == 1) NORM_EVEN(CALL, 1024, 1)                           \
     else if (shape.nv == 2) NORM_TWO(CALL)                                \
     else if (shape.nv == 3) NORM_EVEN(CALL, 1024, 3)                      \
     else NORM_EVEN(CALL, 1024, 4)

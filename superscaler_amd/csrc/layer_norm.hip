@@ -108,12 +108,20 @@ template <class T, int CAP, int NV, bool EVEN, bool HAS_F, bool ENTRY> __global_
 
 int64_t least(int64_t a, int64_t b) { return a < b ? a : b; }
 
+/* Workgroups that walk over the rows, each with its parameters in LDS: as many as a CU holds at once by their LDS, with 1,536 lanes or
+ * fewer.  16,384 rows of bfloat16, up to 1,024, 1,536 and 2,048 lanes and one workgroup per row: 2,048 elements in 51.6, 50.0, 55.7 and
+ * 57.2 us; 5,120 in 165, 138, 141 and 177 us.  12,288 elements, of which LDS holds the parameters once: 292 us, with two workgroups 297. */
+int64_t grid_of(const NormShape &shape, int64_t rows, int lds) {
+    const int64_t by_lanes = shape.lanes > 768 ? 1 : 1536 / shape.lanes;
+    return least(rows, 256 * (lds > 0 ? least(by_lanes, 160 * 1024 / lds) : by_lanes));
+}
+
 template <class T, int CAP, int NV, bool EVEN, bool HAS_F, bool ENTRY> int launch(const NormArgs &a, const NormShape &shape, hipStream_t stream) {
     const auto kernel = norm_forward<T, CAP, NV, EVEN, HAS_F, ENTRY>;
     static const int ready = norm_params_in_lds<NV>() ? layer_hip_status(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 155 * 1024)) : ACE_OK;
     if (ready != ACE_OK) return ready;
-    const dim3 grid((uint32_t)least(a.rows, 256 * (2048 / shape.lanes)));
-    kernel<<<grid, shape.lanes, norm_params_in_lds<NV>() ? PARAMS * norm_pitch(shape) * (int)sizeof(T) : 0, stream>>>(a);
+    const int room = norm_params_in_lds<NV>() ? PARAMS * norm_pitch(shape) * (int)sizeof(T) : 0;
+    kernel<<<(uint32_t)grid_of(shape, a.rows, room), shape.lanes, room, stream>>>(a);
     return layer_launched();
 }
 
@@ -125,14 +133,17 @@ template <class T> int forward(const NormArgs &a, hipStream_t stream) {
         else if (!a.w1) rc = launch<T, CAP, NV, EVEN, true, false>(a, shape, stream);                       \
         else rc = launch<T, CAP, NV, EVEN, true, true>(a, shape, stream);                                   \
     }
-    NORM_FOR_SHAPE(CALL)
+    NORM_FOR_SHAPE(CALL, true)
 #undef CALL
     return rc;
 }
 
-/* Runs of consecutive rows of the backward pass, one per workgroup. */
+/* Runs of consecutive rows of the backward pass, one per workgroup: as many as the CUs hold at once, as far as lanes with 168
+ * registers go.  16,384 rows of bfloat16 in 256, 512 and 1,024 runs: 1,024 elements (128 lanes) in 104, 70 and 61 us; 2,048 in 120, 96 and
+ * 100; 4,096 in 178, 178 and 196; 5,120 (640 lanes) in 214, 225 and 225; 12,288 in 528, 553 and 553. */
 int64_t runs_of(const ace_block_norm_t *a) {
-    const int64_t most = norm_shape(a->width, a->dtype == ACE_T_F32 ? 4 : 2).lanes > 512 ? 256 : 512;
+    const int lanes = norm_shape(a->width, a->dtype == ACE_T_F32 ? 4 : 2, false).lanes;
+    const int64_t most = lanes > 512 ? 256 : lanes > 128 ? 512 : 1024;
     const int64_t run = (a->rows + most - 1) / most;
     return (a->rows + run - 1) / run;
 }

@@ -246,7 +246,7 @@ template <class T> int backward(const NormArgs &a, hipStream_t stream) {
         else if (!a.w1) rc = launch<T, CAP, NV, EVEN, true, false>(a, shape, stream);                       \
         else rc = launch<T, CAP, NV, EVEN, true, true>(a, shape, stream);                                   \
     }
-    NORM_FOR_SHAPE(CALL)
+    NORM_FOR_SHAPE(CALL, false)
 #undef CALL
     if (rc != ACE_OK) return rc;
     const int gates = a.dgate && !a.token_gate ? (int)a.gates : 0;
