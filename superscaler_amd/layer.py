@@ -34,6 +34,8 @@ MAX_HEAD = 128
 ADAMW_BLOCK, ADAMW_CHUNK = 256, 8192
 
 _NONE = 3
+_LONGEST = (1 << 31) - 1
+_HALVES = (torch.bfloat16, torch.float16)
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
 
@@ -41,12 +43,9 @@ _vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.
 # ace_block_norm_t: rows, rows_per_gate; width, dtype, layer; residual_scale, eps; seven pointers (packed: a third of the time that a
 # ctypes structure takes, on a call that a single token waits for)
 _BLOCK_NORM = struct.Struct("=2q3i2f4x7Q")
-
-
-class _Attend(ctypes.Structure):
-    _fields_ = [(n, _i32) for n in ("batch", "queries", "keys", "heads", "kv_heads", "dim", "dtype", "window", "sinks")] + [("scale", _f32)] + \
-        [("d_start", _vp), ("d_length", _vp)] + [(n, _i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + \
-        [(n, _vp) for n in ("d_q", "d_k", "d_v", "d_out", "d_lse")]
+# ace_attend_t: batch, queries, keys, heads, kv_heads, dim, dtype, window, sinks; scale; start and length; four times three strides;
+# q, k, v, out and lse
+_ATTEND = struct.Struct("=9if2Q12q5Q")
 
 
 class _AdamW(ctypes.Structure):
@@ -244,29 +243,27 @@ def block_norm_backward(d_residual, d_normed, x, block, stats, *, residual_scale
 
 # ---- attention over a window and a few first keys ----------------------------------------------------------------------------
 def _heads(t, what, like=None):
-    """A [batch, tokens, heads, dim] tensor as the kernels read it: a head's elements adjacent, everything else at multiples of
-    16 bytes; a copy where it is not so."""
-    _on_gpu(t, what)
-    if t.dim() != 4:
-        raise ValueError(f"{what}: [batch, tokens, heads, size] expected, got shape {tuple(t.shape)}")
-    if t.dtype not in (torch.bfloat16, torch.float16) or (like is not None and t.dtype != like.dtype):
-        raise TypeError(f"{what}: {'bfloat16 or float16' if like is None else like.dtype} expected, not {t.dtype}")
-    if like is not None and t.device != like.device:
+    """A [batch, tokens, heads, size] tensor as the kernels read it, a head's elements adjacent and everything else at multiples of
+    16 bytes, or a copy where it is not so; and its three strides."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 and (t.dtype in _HALVES if like is None else t.dtype is like.dtype and t.device == like.device)):
+        _on_gpu(t, what)
+        if t.dim() != 4:
+            raise ValueError(f"{what}: [batch, tokens, heads, size] expected, got shape {tuple(t.shape)}")
+        if t.dtype not in _HALVES or (like is not None and t.dtype != like.dtype):
+            raise TypeError(f"{what}: {'bfloat16 or float16' if like is None else like.dtype} expected, not {t.dtype}")
         raise ValueError(f"{what} is on {t.device}, q on {like.device}")
-    stride = t.stride()
-    if (t.shape[3] > 1 and stride[3] != 1) or any(n > 1 and s % 8 for n, s in zip(t.shape[:3], stride)) or t.data_ptr() % 16 or \
-            (t.shape[1] > 1 and stride[1] >= 1 << 23):
+    (batch, tokens, heads, size), (b, n, h, e) = t.shape, t.stride()
+    b, n, h = b if batch > 1 else 0, n if tokens > 1 else 0, h if heads > 1 else 0
+    if (size > 1 and e != 1) or (b | n | h) & 7 or n >= 1 << 23 or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _strides(t):
-    return (_i64 * 3)(*(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride())))
+        b, n, h, _ = t.stride()
+    return t, (b, n, h)
 
 
 def _attend_args(q, k, v, window, sinks, scale, start, lengths):
-    q = _heads(q, "q")
-    k, v = _heads(k, "k", q), _heads(v, "v", q)
+    """(q, k and v as the kernels read them, the arguments' part before the strides, q's, k's and v's strides, (batch, heads, queries))"""
+    q, q_strides = _heads(q, "q")
+    (k, k_strides), (v, v_strides) = _heads(k, "k", q), _heads(v, "v", q)
     (batch, queries, heads, dim), (_, keys, kv_heads, _) = q.shape, k.shape
     if not 8 <= dim <= MAX_HEAD or dim % 8:
         raise ValueError(f"q: heads of a multiple of 8 elements up to {MAX_HEAD} expected, got {dim}")
@@ -287,11 +284,10 @@ def _attend_args(q, k, v, window, sinks, scale, start, lengths):
             raise TypeError(f"{name}: int32 expected, not {t.dtype}")
         if tuple(t.shape) != (batch,) or t.device != q.device or not t.is_contiguous():
             raise ValueError(f"{name}: [{batch}] on {q.device} expected, got {tuple(t.shape)} on {t.device}")
-    # (a window that no key is outside of is none)
-    a = _Attend(batch, queries, keys, heads, kv_heads, dim, _TYPES[q.dtype], 0 if window is None else min(int(window), 1 << 30), min(int(sinks), 1 << 30), scale,
-                _pointer(start), _pointer(lengths), _strides(q), _strides(k), _strides(v))
-    a.d_q, a.d_k, a.d_v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    return a, q, k, v
+    # (no key is outside of a window of 2^31 - 1)
+    head = (batch, queries, keys, heads, kv_heads, dim, _TYPES[q.dtype], 0 if window is None else min(int(window), _LONGEST), min(int(sinks), _LONGEST), scale,
+            0 if start is None else start.data_ptr(), 0 if lengths is None else lengths.data_ptr())
+    return q, k, v, head, q_strides + k_strides + v_strides, (batch, heads, queries)
 
 
 def window_attention(q, k, v, *, window=None, sinks=0, scale=None, start=None, lengths=None):
@@ -303,32 +299,33 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, start=None, l
     j < lengths[b], j <= p and (p - j < window or j < sinks); `start` and `lengths` are int32 [batch], by default
     keys - queries and keys: new queries at the end of a full cache.  `window` None: all earlier keys.  `scale`: 1 / sqrt(size)
     by default.  A query that sees no key has out 0 and lse -inf.  What stands at or past lengths[b] is not read; a value
-    of v below it that is not finite can reach queries of the same 64 that do not see it."""
-    a, q, k, v = _attend_args(q, k, v, window, sinks, scale, start, lengths)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((a.batch, a.heads, a.queries), dtype=torch.float32, device=q.device)
-    a.out_stride, a.d_out, a.d_lse = _strides(out), out.data_ptr(), lse.data_ptr()
-    size = load_library().ace_attend_workspace_bytes(ctypes.byref(a))
-    workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    _call(q.device, "ace_attend_forward", ctypes.byref(a), _pointer(workspace), size)
+    of v below it that is not finite can reach queries that do not see it, where their blocks of 128 see a key of the same 64 (so can,
+    in the gradients, one of k, q or d_out)."""
+    q, k, v, head, strides, rows = _attend_args(q, k, v, window, sinks, scale, start, lengths)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(rows, dtype=torch.float32)
+    a = _ATTEND.pack(*head, *strides, *out.stride()[:3], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
+    size = load_library().ace_attend_workspace_bytes(a)
+    workspace = q.new_empty(size, dtype=torch.uint8) if size else None
+    _call(q.device, "ace_attend_forward", a, _pointer(workspace), size)
     return out, lse
 
 
 def window_attention_backward(d_out, q, k, v, out, lse, *, window=None, sinks=0, scale=None, start=None, lengths=None):
     """Gradients (dq, dk, dv) of window_attention's q, k and v from that of its `out`; `out` and `lse` are what it returned.  The
     same call gives the same bits."""
-    a, q, k, v = _attend_args(q, k, v, window, sinks, scale, start, lengths)
-    d_out, out = _heads(d_out, "d_out", q), _heads(out, "out", q)
+    q, k, v, head, strides, rows = _attend_args(q, k, v, window, sinks, scale, start, lengths)
+    (d_out, d_strides), (out, out_strides) = _heads(d_out, "d_out", q), _heads(out, "out", q)
     if d_out.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"d_out and out: {tuple(q.shape)} expected, got {tuple(d_out.shape)} and {tuple(out.shape)}")
     _on_gpu(lse, "lse")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (a.batch, a.heads, a.queries) or not lse.is_contiguous() or lse.device != q.device:
+    if lse.dtype != torch.float32 or tuple(lse.shape) != rows or not lse.is_contiguous() or lse.device != q.device:
         raise ValueError("lse: what window_attention returned expected")
-    a.out_stride, a.d_out, a.d_lse = _strides(out), out.data_ptr(), lse.data_ptr()
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    size = load_library().ace_attend_backward_workspace_bytes(ctypes.byref(a))
-    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-    _call(q.device, "ace_attend_backward", ctypes.byref(a), d_out.data_ptr(), _strides(d_out), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), size)
+    a = _ATTEND.pack(*head, *strides, *out_strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    size = load_library().ace_attend_backward_workspace_bytes(a)
+    workspace = q.new_empty(size, dtype=torch.uint8)
+    _call(q.device, "ace_attend_backward", a, d_out.data_ptr(), (_i64 * 3)(*d_strides), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), size)
     return dq, dk, dv
 
 

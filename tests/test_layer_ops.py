@@ -63,18 +63,14 @@ def test_refusals_of_the_c_entries():
     assert lib.ace_block_norm_workspace_bytes(norm()) == 2 * 4 * 8 * 4
 
     def attend(**change):
-        a = layer._Attend(2, 32, 32, 4, 2, 64, 1, 0, 0, 0.125)
-        for s in (a.q_stride, a.k_stride, a.v_stride, a.out_stride):
-            s[0], s[1], s[2] = 8192, 256, 64
-        a.d_q = a.d_k = a.d_v = a.d_out = a.d_lse = 64
-        for name, value in change.items():
-            setattr(a, name, value)
-        return lib.ace_attend_forward(ctypes.byref(a), None, 0, None)
+        a = dict(batch=2, queries=32, keys=32, heads=4, kv_heads=2, dim=64, dtype=1, window=0, sinks=0, scale=0.125, d_start=0, d_length=0)
+        a.update({f"{t}_stride{i}": s for t in ("q", "k", "v", "out") for i, s in enumerate((8192, 256, 64))}, d_q=64, d_k=64, d_v=64, d_out=64, d_lse=64)
+        return lib.ace_attend_forward(layer._ATTEND.pack(*{**a, **change}.values()), None, 0, None)
     assert attend(batch=0) == 0 and attend(queries=0) == 0
-    for bad in ({"heads": 3}, {"dim": 12}, {"dim": 0}, {"dtype": 0}, {"scale": 0.0}, {"scale": float("nan")}, {"window": -1}, {"d_q": None}, {"d_k": 72}, {"keys": -1},
-                {"kv_heads": 0}):
+    for bad in ({"heads": 3}, {"dim": 12}, {"dim": 0}, {"dtype": 0}, {"scale": 0.0}, {"scale": float("nan")}, {"window": -1}, {"d_q": 0}, {"d_k": 72}, {"keys": -1},
+                {"kv_heads": 0}, {"k_stride1": 252}):
         assert attend(**bad) == -1, bad
-    assert attend(dim=136) == -2 and attend(batch=1 << 21) == -2
+    assert attend(dim=136) == -2 and attend(batch=1 << 21) == -2 and attend(keys=(1 << 28) + 1) == -2 and attend(v_stride1=1 << 23) == -2
     a = layer._AdamW(64, 64, 1, 1, 16, 1, 1, 64, 64)
     first = (ctypes.c_int64 * 2)(0, 1)
     grads = (ctypes.c_void_p * 1)(64)
@@ -364,6 +360,19 @@ def test_attention_of_new_tokens(queries, keys, window, sinks):
 
 
 @gpu
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 3), (1, 0)])
+@pytest.mark.parametrize("batch,queries,keys,heads,kv_heads", [(1, 1, 700, 2, 2), (3, 7, 1200, 6, 2), (1, 16, 1000, 40, 4), (2, 100, 1500, 2, 1), (20, 1, 256, 20, 20), (3, 128, 600, 2, 2),
+                                                               (40, 9, 200, 8, 1)])
+def test_attention_of_few_queries_over_long_caches(batch, queries, keys, heads, kv_heads, window, sinks):
+    """Keys split over wavefronts and workgroups, whose answers are joined, and caches too short for that."""
+    device = cuda_or_skip()
+    q, k, v, do = attention_case(31, batch, queries, keys, heads, kv_heads, 64, BF16)
+    check_attention(q, k, v, do, device, backward=False, window=window, sinks=sinks)
+    lengths = torch.arange(batch, dtype=torch.int32) * 37 % (keys + 1)
+    check_attention(q, k, v, do, device, backward=False, window=window, sinks=sinks, start=lengths - queries, lengths=lengths)
+
+
+@gpu
 @pytest.mark.parametrize("queries,heads,kv_heads", [(1, 8, 2), (5, 16, 1), (130, 4, 2)])
 def test_attention_of_ragged_sequences(queries, heads, kv_heads):
     """Lengths from none to all, queries before the first key and behind the last, and what is past a length is not read."""
@@ -439,6 +448,32 @@ def test_attention_at_offsets_past_32_bits():
         want = ref.attention(q, k1, v1, window=300, unit=ref.UNIT[BF16])
         ref.close(out, *want["out"])
         ref.close(lse, *want["lse"])
+
+
+@gpu
+@pytest.mark.parametrize("queries", [3, 40])
+def test_attention_at_positions_and_windows_at_the_ends_of_32_bits(queries):
+    """A window that holds every key is none, a sequence before the first key sees none, one far behind the last sees the first keys:
+    the same kernels on the same keys, so the same bits."""
+    device, least, most = cuda_or_skip(), -(1 << 31), (1 << 31) - 1
+    q, k, v, do = (t.to(device) for t in attention_case(23, 1, queries, 90, 2, 1, 64, BF16))
+
+    def both(start, **how):
+        at = torch.tensor([start], dtype=torch.int32, device=device)
+        out, lse = layer.window_attention(q, k, v, start=at, **how)
+        return (out, lse) + layer.window_attention_backward(do, q, k, v, out, lse, start=at, **how)
+    for start, window in ((50, most), (0, 1 << 30), (1 << 30, most), (most, most), (1000, (1 << 30) + 5)):
+        for got, want in zip(both(start, window=window), both(start)):
+            assert torch.equal(got, want), (start, window)
+    for start in (least, -(1 << 30), -(1 << 28) - 7, -queries):
+        for window in (None, 5, most):
+            out, lse, dq, dk, dv = both(start, window=window, sinks=3)
+            assert (out == 0).all() and (lse == -float("inf")).all() and not any(g.any() for g in (dq, dk, dv)), (start, window)
+    for start in (most, 1 << 30, 100_000):
+        out, lse, dq, dk, dv = both(start, window=5, sinks=3)
+        few, few_lse = layer.window_attention(q, k[:, :3], v[:, :3], start=torch.tensor([9], dtype=torch.int32, device=device))
+        assert torch.equal(out, few) and torch.equal(lse, few_lse), start
+        assert not dk[:, 3:].any() and not dv[:, 3:].any() and dv[:, :3].any()
 
 
 @gpu
