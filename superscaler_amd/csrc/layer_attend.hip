@@ -697,38 +697,43 @@ template <class T, int DP> struct KeyGrads {
 
 /* Tiles of queries: rows of q and of the answer's gradient, then log-sums and deltas, by LANES lanes. */
 template <class T, int PITCH, int ROWS, int LANES> struct QueryTiles {
-    static constexpr int BYTES = ROWS * PITCH * 2, STAGE = 2 * BYTES + 2 * 256, LOADS = 2 * Tile<T, PITCH, ROWS, LANES, LANES != 64>::LOADS + (LANES == 64 ? 2 : 1);
+    static constexpr int BYTES = ROWS * PITCH * 2, ROW_VALUES = ROWS > 64 ? ROWS * 4 : 256, STAGE = 2 * BYTES + 2 * ROW_VALUES;
+    static constexpr int LOADS = 2 * Tile<T, PITCH, ROWS, LANES, LANES != 64>::LOADS + (LANES == 64 ? 2 : 1);
+    static_assert(ROWS <= 64 || (ROWS == 128 && LANES == 256), "a row's values by one or two wavefronts");
     Tile<T, PITCH, ROWS, LANES, LANES != 64> q, g;
     const float *lse, *delta;
     __device__ inline QueryTiles(const Args &a, int b, int lane)
         : q((const T *)a.q + b * a.q_stride[0], a.q_stride[1], a.dim, lane), g((const T *)a.g + b * a.g_stride[0], a.g_stride[1], a.dim, lane),
           lse(a.lse + (int64_t)b * a.heads * a.queries), delta(a.delta + (int64_t)b * a.heads * a.queries) {}
-    /* (a workgroup's four wavefronts: each asks for as many loads, the last two for those of the first two again) */
+    /* (a workgroup's four wavefronts: each asks for as many loads, the last two for the second 64 rows' or, of 64, for those of the first two
+     * again) */
     __device__ inline void ask(const Args &a, uint32_t lds, int head, int row, int wave, int lane) const {
         Tile<T, PITCH, ROWS, LANES, LANES != 64> qh = q, gh = g;
         qh.base += head * a.q_stride[2], gh.base += head * a.g_stride[2];
         qh.ask(lds, row, a.queries), gh.ask(lds + BYTES, row, a.queries);
-        const int64_t at = (int64_t)head * a.queries + row;
-        const int64_t bytes = (int64_t)(a.queries - row < ROWS ? a.queries - row : ROWS) * 4;
-        if (LANES == 64 || (wave & 1) == 0) to_lds4(buffer(lse + at, bytes), lane * 4, __builtin_amdgcn_readfirstlane(lds + 2 * BYTES));
-        if (LANES == 64 || (wave & 1) == 1) to_lds4(buffer(delta + at, bytes), lane * 4, __builtin_amdgcn_readfirstlane(lds + 2 * BYTES + 256));
+        const int second = ROWS > 64 ? wave >> 1 : 0, left = a.queries - row - 64 * second;
+        const int64_t at = (int64_t)head * a.queries + row + 64 * second, bytes = left < 0 ? 0 : (int64_t)(left < 64 && left < ROWS ? left : ROWS < 64 ? ROWS : 64) * 4;
+        const uint32_t to = lds + 2 * BYTES + 256 * second;
+        if (LANES == 64 || (wave & 1) == 0) to_lds4(buffer(lse + at, bytes), lane * 4, __builtin_amdgcn_readfirstlane(to));
+        if (LANES == 64 || (wave & 1) == 1) to_lds4(buffer(delta + at, bytes), lane * 4, __builtin_amdgcn_readfirstlane(to + ROW_VALUES));
     }
 };
 
 /* The pairs of a window: a workgroup takes 128 keys and walks over the queries whose window they are in, of every head that shares the
- * key head, in tiles of 64.  With SHARE 2 it takes 64 keys, and two wavefronts share 32 keys and halve each tile's queries: twice the
- * workgroups, for calls that would leave CUs without one. */
+ * key head, in tiles of 64.  With SHARE 2 or 4 it takes 64 or 32 keys, and so many wavefronts share 32 keys and a tile's queries (128 of
+ * them with SHARE 4): more workgroups, for calls that would leave CUs without one. */
+constexpr int query_rows(int share) { return share == 4 ? 128 : 64; }
 template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_dkv(const Args a) {
     extern __shared__ char lds[];
-    constexpr int PITCH = Shape<DP>::PITCH, OWN = QUERIES / SHARE;
-    typedef QueryTiles<T, PITCH, KEYS, LANES> Queries;
+    constexpr int PITCH = Shape<DP>::PITCH, OWN = QUERIES / SHARE, OWNERS = WAVES / SHARE, ROWS = query_rows(SHARE);
+    typedef QueryTiles<T, PITCH, ROWS, LANES> Queries;
     const int blocks = (a.keys + OWN - 1) / OWN, count = a.batch * a.kv_heads * blocks;
     const int work = place(count);
     if (work >= count) return;
     const int block = work % blocks, kv = work / blocks % a.kv_heads, b = work / blocks / a.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Sequence seq = sequence(a, b);
-    const int k0 = block * OWN, mine = k0 + wave % (WAVES / SHARE) * 32, key = mine + (lane & 31);
+    const int k0 = block * OWN, mine = k0 + wave % OWNERS * 32, key = mine + (lane & 31);
     const T *krow = (const T *)a.k + b * a.k_stride[0] + (int64_t)key * a.k_stride[1] + kv * a.k_stride[2];
     const T *vrow = (const T *)a.v + b * a.v_stride[0] + (int64_t)key * a.v_stride[1] + kv * a.v_stride[2];
     /* queries from the first key's position on, up to the last key's window */
@@ -738,13 +743,13 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
         to = most < to ? (int)most : to;
     }
     from = from < 0 ? 0 : from;
-    const int first = from / KEYS, per_head = k0 < seq.length && to > from ? (to + KEYS - 1) / KEYS - first : 0, steps = per_head * a.shared;
+    const int first = from / ROWS, per_head = k0 < seq.length && to > from ? (to + ROWS - 1) / ROWS - first : 0, steps = per_head * a.shared;
     const uint32_t lds0 = lds_offset(lds);
     const Operands<T, PITCH> ops(lane);
     const Queries queries(a, b, threadIdx.x);
     int head = kv * a.shared, tile = first;      /* of the next step to be asked for */
     auto ask = [&](int t) {
-        queries.ask(a, lds0 + (t & 1) * Queries::STAGE, head, tile * KEYS, wave, lane);
+        queries.ask(a, lds0 + (t & 1) * Queries::STAGE, head, tile * ROWS, wave, lane);
         if (++tile == first + per_head) tile = first, ++head;
     };
     KeyGrads<T, DP> grads;
@@ -753,7 +758,7 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
     const int64_t left = (int64_t)seq.start + a.queries - key;
     const uint32_t sight = key >= seq.length || left <= 0 ? 0 : a.window > 0 && a.window < left ? a.window : (uint32_t)left;
     if (steps > 0) ask(0);
-    int q = first * KEYS;
+    int q = first * ROWS;
     for (int t = 0; t < steps; ++t) {
         wait_tiles<0>();
         meet();
@@ -764,34 +769,35 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
             if (mine >= seq.length || q + n * 32 >= a.queries || hi < mine || (a.window > 0 && lo - (mine + 31) >= a.window)) return;
             const bool masked = q + n * 32 + 32 > a.queries || mine + 32 > seq.length || lo < mine + 31 || (a.window > 0 && hi - mine >= a.window);
             const uint32_t qtile = buffer_at + n * 32 * PITCH * 2, lse = buffer_at + 2 * Queries::BYTES + n * 32 * 4;
-            grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + 256, a.scale2, lo - key, sight, masked, half);
+            grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + Queries::ROW_VALUES, a.scale2, lo - key, sight, masked, half);
         };
-        if (SHARE == 2) half_tile(wave >> 1);
+        if (SHARE > 1) half_tile(wave / OWNERS);
         else
 #pragma unroll 1
-            for (int n = 0; n < KEYS / 32; ++n) half_tile(n);
-        q = q + KEYS < (first + per_head) * KEYS ? q + KEYS : first * KEYS;
+            for (int n = 0; n < ROWS / 32; ++n) half_tile(n);
+        q = q + ROWS < (first + per_head) * ROWS ? q + ROWS : first * ROWS;
     }
     grads.stop();
-    if (SHARE == 2) {
-        /* the second two wavefronts' sums go to the first two's, dK and then dV */
-        float *sums = (float *)lds + (wave & 1) * DP * 32 + (lane & 31);
+    if (SHARE > 1) {
+        /* the other wavefronts' sums go to those of the first one or two, in order, dK and then dV */
+        float *sums = (float *)lds + (lane & 31);
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             meet();
-            if (wave >= 2)
+            if (wave >= OWNERS)
 #pragma unroll
                 for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sums[(t * 32 + result_row(i, half)) * 32] = which ? grads.dv[t][i] : grads.dk[t][i];
+                    for (int i = 0; i < 16; ++i) sums[((wave - OWNERS) * DP + t * 32 + result_row(i, half)) * 32] = which ? grads.dv[t][i] : grads.dk[t][i];
             meet();
-            if (wave < 2)
+            if (wave < OWNERS)
+                for (int from = wave; from < WAVES - OWNERS; from += OWNERS)
 #pragma unroll
-                for (int t = 0; t < DP / 32; ++t)
+                    for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) (which ? grads.dv : grads.dk)[t][i] += sums[(t * 32 + result_row(i, half)) * 32];
+                        for (int i = 0; i < 16; ++i) (which ? grads.dv : grads.dk)[t][i] += sums[(from * DP + t * 32 + result_row(i, half)) * 32];
         }
-        if (wave >= 2) return;
+        if (wave >= OWNERS) return;
     }
     if (key >= a.keys) return;
     /* what queries beyond the window have left for a first key */
@@ -854,7 +860,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_far(c
         } else
             wait_tiles<0>();
         const uint32_t qtile = lds0 + buffer * Queries::STAGE, lse = qtile + 2 * Queries::BYTES;
-        grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + 256, a.scale2, seq.start + (first + i % per_head) * 32 - key - a.window, sight, true, half);
+        grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + Queries::ROW_VALUES, a.scale2, seq.start + (first + i % per_head) * 32 - key - a.window, sight, true, half);
     }
     grads.stop();
     float *sums = (float *)lds;
@@ -967,17 +973,28 @@ void far_of(const ace_attend_t *a, Args &k) {
     parts = parts < most ? parts : most;
     k.far_parts = parts < 1 ? 1 : parts > 32 ? 32 : (int)parts;
 }
-/* Fewer workgroups of 128 keys than this: half as many keys for each.  Measured, all of the backward pass, 128 keys and 64, at
- * 512 workgroups (2 x 16 heads of 2,048 keys, a window of 512): 110 and 120 us; at 256: 83 and 77; at 64 (4 key heads): 175 and 131. */
-constexpr int SHARED_BELOW = 384;
+/* Fewer workgroups of 128 keys than this: half as many keys for each, or a quarter.  Measured, all of the backward pass, with 128, 64
+ * and 32 keys, at 512 workgroups of 128 (2 x 16 heads of 2,048 tokens, a window of 512): 116, 124 and 210 us; at 384 (8 x 4 heads
+ * of 1,531 tokens and size 64, 256): 125, 112 and 142; at 256: 84, 77 and 124; at 128 (8 heads): 80, 72 and 88; at 64 (4 key heads of 16):
+ * 173, 131 and 117; at 8 (512 tokens, size 64): 81, 58 and 45. */
+constexpr int SHARED_BELOW = 448, SHARED_BY_4_BELOW = 96;
 int width_of(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 int64_t delta_floats(const ace_attend_t *a) { return ((int64_t)a->batch * a->heads * a->queries + 3) / 4 * 4; }
 
+template <class T, int DP, int SHARE> int key_grads(const Args &k, hipStream_t stream) {
+    constexpr int LDS = 2 * QueryTiles<T, Shape<DP>::PITCH, query_rows(SHARE), LANES>::STAGE, OWN = QUERIES / SHARE;
+    static_assert(LDS >= (WAVES - WAVES / SHARE) * DP * 32 * 4, "the wavefronts' sums");
+    static const int ready = with_lds(attend_dkv<T, DP, SHARE>, LDS);
+    if (ready != ACE_OK) return ready;
+    attend_dkv<T, DP, SHARE><<<places((int64_t)k.batch * k.kv_heads * ((k.keys + OWN - 1) / OWN)), LANES, LDS, stream>>>(k);
+    return layer_launched();
+}
+
 template <class T, int DP> int backward(const Args &k, hipStream_t stream) {
-    constexpr int PITCH = Shape<DP>::PITCH, DQ = 4 * KEYS * PITCH * 2, DKV = 2 * QueryTiles<T, PITCH, KEYS, LANES>::STAGE;
+    constexpr int PITCH = Shape<DP>::PITCH, DQ = 4 * KEYS * PITCH * 2;
     constexpr int FAR_TILES = WAVES * 2 * QueryTiles<T, PITCH, 32, 64>::STAGE, FAR_JOIN = WAVES * DP * 32 * 4, FAR = FAR_TILES > FAR_JOIN ? FAR_TILES : FAR_JOIN;
-    static const int ready = with_lds(attend_dq<T, DP>, DQ), ready2 = with_lds(attend_dkv<T, DP, 1>, DKV) | with_lds(attend_dkv<T, DP, 2>, DKV), ready3 = with_lds(attend_far<T, DP>, FAR);
-    if (ready != ACE_OK || ready2 != ACE_OK || ready3 != ACE_OK) return ACE_EHIP;
+    static const int ready = with_lds(attend_dq<T, DP>, DQ), ready2 = with_lds(attend_far<T, DP>, FAR);
+    if (ready != ACE_OK || ready2 != ACE_OK) return ACE_EHIP;
     int rc = ACE_OK;
     if (k.queries > 0) {
         attend_dq<T, DP><<<places((int64_t)k.batch * k.heads * ((k.queries + QUERIES - 1) / QUERIES)), LANES, DQ, stream>>>(k);
@@ -989,10 +1006,8 @@ template <class T, int DP> int backward(const Args &k, hipStream_t stream) {
         attend_far<T, DP><<<dim3(k.far_parts, k.kv_heads * k.far_blocks, k.batch), LANES, FAR, stream>>>(k);
         if ((rc = layer_launched()) != ACE_OK) return rc;
     }
-    const int64_t heads = (int64_t)k.batch * k.kv_heads, groups = heads * ((k.keys + QUERIES - 1) / QUERIES);
-    if (groups < SHARED_BELOW) attend_dkv<T, DP, 2><<<places(heads * ((k.keys + QUERIES / 2 - 1) / (QUERIES / 2))), LANES, DKV, stream>>>(k);
-    else attend_dkv<T, DP, 1><<<places(groups), LANES, DKV, stream>>>(k);
-    return layer_launched();
+    const int64_t groups = (int64_t)k.batch * k.kv_heads * ((k.keys + QUERIES - 1) / QUERIES);
+    return groups < SHARED_BY_4_BELOW ? key_grads<T, DP, 4>(k, stream) : groups < SHARED_BELOW ? key_grads<T, DP, 2>(k, stream) : key_grads<T, DP, 1>(k, stream);
 }
 
 }  // namespace

@@ -360,6 +360,16 @@ def test_attention_of_new_tokens(queries, keys, window, sinks):
 
 
 @gpu
+@pytest.mark.parametrize("batch,heads,kv_heads", [(1, 4, 2), (6, 8, 8), (19, 8, 8)])
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (56, F16)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (100, 40)])
+def test_attention_gradients_of_few_and_many_heads(batch, heads, kv_heads, dim, dtype, window, sinks):
+    """Key blocks of 32, 64 and 128 keys per workgroup."""
+    device = cuda_or_skip()
+    check_attention(*attention_case(47, batch, 270, 270, heads, kv_heads, dim, dtype), device, window=window, sinks=sinks)
+
+
+@gpu
 @pytest.mark.parametrize("window,sinks", [(None, 0), (150, 3), (1, 0)])
 @pytest.mark.parametrize("batch,queries,keys,heads,kv_heads", [(1, 1, 700, 2, 2), (3, 7, 1200, 6, 2), (1, 16, 1000, 40, 4), (2, 100, 1500, 2, 1), (20, 1, 256, 20, 20), (3, 128, 600, 2, 2),
                                                                (40, 9, 200, 8, 1)])
