@@ -234,7 +234,9 @@ __device__ inline void hide(float *s, const Sight &sight, int key0, int half, bo
 /* Work in an order that keeps a head's blocks, which read the same keys, on one of the eight dies and its cache: workgroups go to
  * the dies in turn, so die d gets the d-th eighth of the work.  On a die they go to its 32 CUs in turn: every other 32 are
  * taken in reverse, so that a CU's second workgroup is short where its first is long (blocks at the beginning of a sequence see few
- * keys).  Returns count where a workgroup has nothing to do. */
+ * keys).  Returns count where a workgroup has nothing to do.  In launch order, by dies, and with every other 32 in reverse: forward, 4 x 40
+ * heads of 2,048 tokens, a window of 512: 164, 140 and 140 us, backward 586, 525 and 517; 8 x 16 heads of 512, backward: 55, 51 and 46;
+ * 16 heads on 4 of 8,192, no window, backward: 1,733, 1,339 and 1,380. */
 __device__ inline int place(int count) {
     const int per = (count + 7) / 8, turn = (int)(blockIdx.x / 8), group = turn / 32 * 32;
     const int left = per - group < 32 ? per - group : 32;
@@ -338,13 +340,20 @@ template <class T> __device__ inline void store4(T *to, float a, float b, float 
 template <int DP> struct Shape { static constexpr int PITCH = DP <= 64 ? 64 : 128; };
 
 /* How many wavefronts of a SIMD a kernel is scheduled for: exactly as many as its registers allow, so that what is left of them goes to
- * operands on their way. */
+ * operands on their way.  Without it: 4 x 40 heads of 2,048 tokens, a window of 512, 228 us instead of 160; 8 heads of 16,384, 2,048:
+ * 230 instead of 157; 2 x 16 heads of 2,048, 1,024, forward and backward: 307 instead of 197. */
 #define RESIDENT(DP) __attribute__((amdgpu_waves_per_eu((DP) <= 64 ? 3 : 2, (DP) <= 64 ? 3 : 2)))
 
 constexpr int WAVES = 4, LANES = WAVES * 64, QUERIES = WAVES * 32, KEYS = 64;
 
 /* Prompts: a workgroup takes 128 queries of a head, 32 per wavefront, and walks over its keys in tiles of 64, the next tile on its
- * way while one is worked on. */
+ * way while one is worked on.  Tiles of 32 keys, which leave registers for a third wavefront per SIMD, took 3% off where a window is
+ * 512 and added 6% where it is 2,048; single blocks of 32 at a window's edges took nothing off and added 7%.
+ *
+ * 4 x 40 heads of 2,048 tokens and size 128, a window of 512: 146 us, 518 TFLOP/s of the pairs that are seen; 8 heads of 16,384, 2,048:
+ * 150 us, 868 (a large product of the matrix library: 1,250).  The two wavefronts of a SIMD share it: its matrix unit is at work 32%
+ * and 48% of the time, softmax's 210 vector instructions to a tile's 32 matrix instructions about as much, and a short walk
+ * pays for its first loads and last stores, some 5 us of 28.  LDS has no conflicts and is at work for less than a quarter. */
 template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_forward(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
@@ -403,7 +412,9 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
 }
 
 /* Few queries: the queries of a key head's heads are the columns of one block of 32; every wavefront walks over tiles of 32 keys
- * of its own, with its own two buffers and no barrier, and the wavefronts' and then the workgroups' results are joined. */
+ * of its own, with its own two buffers and no barrier, and the wavefronts' and then the workgroups' results are joined.  Bound by
+ * memory: 32 x 8 heads of 8,192 keys of size 128, one query of 4 heads each: 180 us, 6.0 TB/s (a large copy reaches 5.2, half of it
+ * writes). */
 constexpr int SPLIT_KEYS = 32;
 template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split(const Args a) {
     extern __shared__ char lds[];
@@ -516,10 +527,14 @@ template <class T> __global__ void __launch_bounds__(LANES) attend_join(const Ar
     if (lane == 0) a.lse[row] = total == 0.0f ? -__builtin_inff() : top * a.scale + __logf(total);
 }
 
+/* Of how many tiles a walk counts as short (attend_dq takes delta differently there): with up to three 64s of keys the error of dQ and
+ * dK in half precision is 3.0e-4 of their norm, 3.1e-4 without; at most 0.7% of the backward pass's time (4 x 40 heads of 2,048,
+ * a window of 512: 518 us and 515). */
 constexpr int FEW_TILES = 3;
 
 /* dQ: queries in registers, keys in tiles as in attend_forward; per block of 32 keys S^T = K Q^T, dP^T = V dO^T,
- * dQ^T += K^T dS^T.  It also leaves delta = sum dO O of every query for attend_dkv. */
+ * dQ^T += K^T dS^T.  It also leaves delta = sum dO O of every query for attend_dkv.  2 x 16 heads of 2,048 tokens and size 128, a window of
+ * 1,024: 70 us, 555 TFLOP/s of the pairs that are seen, the matrix units at work 30% of the time. */
 template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_dq(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
@@ -721,7 +736,9 @@ template <class T, int PITCH, int ROWS, int LANES> struct QueryTiles {
 
 /* The pairs of a window: a workgroup takes 128 keys and walks over the queries whose window they are in, of every head that shares the
  * key head, in tiles of 64.  With SHARE 2 or 4 it takes 64 or 32 keys, and so many wavefronts share 32 keys and a tile's queries (128 of
- * them with SHARE 4): more workgroups, for calls that would leave CUs without one. */
+ * them with SHARE 4): more workgroups, for calls that would leave CUs without one.  2 x 16 heads of 2,048 tokens and size 128, a window of
+ * 1,024: 88 us, 588 TFLOP/s of the pairs that are seen, the matrix units at work 33% of the time: all 256 registers of a wavefront are
+ * in use, and the four products of a block of 32 x 32 wait for each other. */
 constexpr int query_rows(int share) { return share == 4 ? 128 : 64; }
 template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_dkv(const Args a) {
     extern __shared__ char lds[];
@@ -826,7 +843,8 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
 
 /* The first keys and the queries beyond their window: every later query of every head sees those few keys, so the work is split
  * over the queries.  A wavefront walks over tiles of 32 queries with buffers of its own; a workgroup's sums, element d of key j at
- * [dk, dv][d][j], are one part, and attend_dkv adds the parts in order. */
+ * [dk, dv][d][j], are one part, and attend_dkv adds the parts in order.  4 first keys of 2 x 16 heads, 1,024 queries beyond their window: 12 us,
+ * two or three tiles for each wavefront, from launch to end a chain of loads, one tile and the sums. */
 template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_far(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH;

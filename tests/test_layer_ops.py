@@ -672,6 +672,53 @@ def test_adamw_state_is_saved_and_restored():
 
 
 @gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_calls_replayed_in_a_graph(bits):
+    """A layer's calls, captured, give on every replay the bits that they give by themselves on the same inputs."""
+    device = cuda_or_skip()
+    x, f, w = normal(1, 64, 256, dtype=BF16).to(device), normal(2, 64, 256, dtype=BF16).to(device), normal(3, 256, dtype=BF16).to(device)
+    q, k, v, do = (t.to(device) for t in attention_case(5, 2, 200, 200, 4, 2, 64, BF16))
+    cache = normal(9, 2, 600, 2, 64, dtype=BF16).to(device)
+    params, grads = [normal(11, n).to(device) for n in (300, 5000)], [normal(12, n).to(device) for n in (300, 5000)]
+    start = [p.clone() for p in params]
+    opt = layer.AdamW(params, state_bits=bits)
+
+    def calls():
+        r = layer.block_norm(x, f, entry_weight=w, exit_weight=w)
+        g = layer.block_norm_backward(r.residual, r.normed, x, f, r.stats, entry_weight=w, exit_weight=w)
+        out, lse = layer.window_attention(q, k, v, window=50, sinks=3)
+        back = layer.window_attention_backward(do, q, k, v, out, lse, window=50, sinks=3)
+        one = layer.window_attention(q[:, :1], cache, cache)
+        opt.step(grads, lr=1e-2)
+        return [t for t in (*r, *g, out, lse, *back, *one, *params, *opt.state.values()) if t is not None]
+
+    def reset(seed):
+        for t, s in ((x, 0), (f, 1), (q, 2), (cache, 3)):
+            t.copy_(normal(seed + s, *t.shape, dtype=BF16))
+        for p, s in zip(params, start):
+            p.copy_(s)
+        for t in opt.state.values():
+            t.copy_(torch.zeros_like(t))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = calls()
+    for seed in (100, 200, 300, 400):
+        reset(seed)
+        want = [t.clone() for t in calls()]
+        torch.cuda.synchronize()
+        reset(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, (got, w0) in enumerate(zip(held, want)):
+            assert torch.equal(got, w0), (seed, i)
+
+
+@gpu
 def test_adamw_refusals():
     device = cuda_or_skip()
     p = torch.ones(8, 4, device=device)
