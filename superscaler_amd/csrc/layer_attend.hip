@@ -79,10 +79,10 @@ __device__ inline void meet() {
 template <class V> __device__ inline void arrived(V &v) { asm volatile("" : "+v"(v)); }
 
 /* A buffer descriptor of `bytes` bytes from `p` on, both the same for the wavefront. */
-__device__ inline u32x4 buffer(const void *p, int64_t bytes) {
+__device__ inline u32x4 buffer(const void *p, uint32_t bytes) {
     const uint64_t at = (uint64_t)(uintptr_t)p;
     return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xffff),
-                 (uint32_t)__builtin_amdgcn_readfirstlane(bytes < 0 ? 0 : (int)bytes), 0x00027000u};
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00027000u};
 }
 
 /* A tile's rows in memory and where the lanes find their pieces of them: ROWS rows of PITCH elements by LANES lanes.  A lane keeps a
@@ -93,23 +93,22 @@ template <class T, int PITCH, int ROWS, int LANES, bool ONE = false> struct Tile
     static constexpr int PER = PITCH / 8, LOADS = ROWS * PER / LANES, STEP = LANES / PER, PLACES = ONE ? 1 : LOADS;
     static_assert(ROWS * PER % LANES == 0 && (!ONE || STEP % 16 == 0), "whole loads");
     const T *base;
-    int64_t stride;
-    int dim;
+    uint32_t stride, dim;   /* (tokens are up to 2^23 elements apart) */
     uint32_t at[PLACES], to;
-    __device__ inline Tile(const T *b, int64_t s, int d, int lane) : base(b), stride(s), dim(d) {
+    __device__ inline Tile(const T *b, int64_t s, int d, int lane) : base(b), stride((uint32_t)s), dim(d) {
 #pragma unroll
         for (int i = 0; i < PLACES; ++i) {
             const int p = i * LANES + lane, row = p / PER, piece = (p % PER) ^ (swizzle<PITCH>(row) & (PER - 1));
             at[i] = piece * 8 < d ? (uint32_t)(row * (int)s + piece * 8) * 2u : 0x80000000u;   /* (past every descriptor's end) */
         }
-        to = (lane & ~63) * 16;
+        to = __builtin_amdgcn_readfirstlane((lane & ~63) * 16);
     }
     __device__ inline u32x4 rows(int row0, int end, int most) const {
         const int n = end - row0 < most ? end - row0 : most;
-        return buffer(base + (int64_t)row0 * stride, n > 0 ? ((int64_t)(n - 1) * stride + dim) * 2 : 0);
+        return buffer(base + (uint64_t)(uint32_t)row0 * stride, n > 0 ? ((uint32_t)(n - 1) * stride + dim) * 2 : 0);
     }
     __device__ inline void ask(uint32_t lds, int row0, int end) const {
-        const uint32_t at_lds = __builtin_amdgcn_readfirstlane(lds + to);
+        const uint32_t at_lds = __builtin_amdgcn_readfirstlane(lds) + to;
         u32x4 b;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
@@ -198,13 +197,22 @@ template <int SIZE> __device__ inline Tiles tiles_of(const Args &a, const Sequen
     return {first, at, first + to - at};
 }
 
-/* whether positions lo..hi all see (or all do not see) keys from..to - 1 */
-__device__ inline bool all_see(const Args &a, int length, int lo, int hi, int from, int to) {
-    return to <= length && to - 1 <= lo && (a.window == 0 || hi - from < a.window || to <= a.sinks);
-}
+/* whether positions lo..hi all do not see keys from..to - 1 */
 __device__ inline bool none_see(const Args &a, int length, int lo, int hi, int from, int to) {
     return from >= length || from > hi || (a.window > 0 && lo - (to - 1) >= a.window && from >= a.sinks);
 }
+
+/* The keys that positions lo..hi all see by their window: `count` blocks of 32 begin at `from` or behind it. */
+struct Clear {
+    int from;
+    uint32_t count;
+    __device__ inline Clear(const Args &a, int length, int lo, int hi) {
+        from = a.window > 0 && hi >= a.window ? hi - a.window + 1 : 0;
+        const int end = length < lo + 1 ? length : lo + 1;
+        count = end - from >= 32 ? end - from - 31 : 0;
+    }
+    __device__ inline bool block(int key0) const { return (uint32_t)(key0 - from) < count; }
+};
 
 /* What a query sees: `count` keys from `from` on, and those below `first`. */
 struct Sight {
@@ -218,7 +226,7 @@ struct Sight {
     }
 };
 /* Values of keys key0 + result_row(i) that are not seen become `otherwise`.  `sinks`: some of the keys are first ones. */
-__device__ inline void hide(float *s, const Sight &sight, int key0, int half, bool sinks, float otherwise) {
+template <class V> __device__ inline void hide(V &s, const Sight &sight, int key0, int half, bool sinks, float otherwise) {
     const int t = key0 + 4 * half - sight.from, u = key0 + 4 * half;
     if (sinks) {
 #pragma unroll
@@ -346,6 +354,123 @@ template <int DP> struct Shape { static constexpr int PITCH = DP <= 64 ? 64 : 12
 
 constexpr int WAVES = 4, LANES = WAVES * 64, QUERIES = WAVES * 32, KEYS = 64;
 
+/* f(0) to f(END - 1), each with its number as a constant */
+template <int I> struct Number { static constexpr int value = I; };
+template <int I, int END, class F> __device__ __attribute__((always_inline)) inline void each(F f) {
+    if constexpr (I < END) f(Number<I>()), each<I + 1, END>(f);
+}
+
+/* A wavefront's walk over blocks of 32 keys, three of them in work at a time: scores of one are taken and the weights of another meet
+ * its values, matrix instructions that do not depend on each other, and between them softmax turns the scores of the block in the
+ * middle into weights, a few vector instructions to each matrix instruction.  The maximum that exponentials are taken around moves only
+ * when a score passes it by 8 powers of two: the sums stay far from their range's end, and most blocks need no rescaling. */
+template <class T, int DP, int PITCH> struct Walk {
+    typedef typename Mma<T>::frag frag;
+    typedef T pair __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    static constexpr int N = DP / 16, DT = DP / 32, TILE = KEYS * PITCH * 2, BLOCK = 32 * PITCH * 2;
+    uint32_t row[N], column[2 * DT];   /* where a lane finds operands in a tile at 0 */
+    frag qf[N];
+    f32x16 o[DT], s;                   /* weighted values; scores of the last block */
+    union { uint32_t two[8]; frag whole[2]; } p;   /* weights of the one before it */
+    float top, total, around, limit, scale2;   /* around: top as an exponent; past `limit` a score moves it */
+    __device__ inline void start(const Operands<T, PITCH> &ops, uint32_t lds, float scale) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) row[i] = (lds + ops.row) ^ (i << 5);
+#pragma unroll
+        for (int i = 0; i < 2 * DT; ++i) column[i] = (lds + ops.column) ^ (i << 5);
+        top = limit = -__builtin_inff(), total = around = 0.0f, scale2 = scale;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+    }
+    __device__ inline frag keys(uint32_t at, int i) const { return lds_load<frag>(row[i] + at); }
+    __device__ inline frag values(uint32_t at, int i) const {
+        union { s16x4 half[2]; frag whole; } u;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            u.half[k] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(lds_ptr)(column[2 * (i % DT) + k] + at + (i / DT * 16 + 8 * k) * PITCH * 2));
+        return u.whole;
+    }
+    struct Soft { float by, last; bool moved; uint32_t two[8]; };
+    /* the maximum of s, and whether it moves the one that exponentials are taken around (also from no key at all, -inf, to any) */
+    __device__ inline void look(Soft &f) {
+        float most = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, s[i]);
+        f.moved = __any(most > limit), f.by = 1.0f;
+        if (f.moved) {
+            most = max_halves(most);
+            if (most > limit) {
+                f.by = __builtin_amdgcn_exp2f((top - most) * scale2);
+                total *= f.by, top = most, around = most * scale2, limit = most + 8.0f / scale2;
+            }
+        }
+    }
+    /* the weight of key i */
+    __device__ inline void weight(Soft &f, int i) {
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale2, -around));
+        total += w;
+        if (i % 2) f.two[i / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{f.last, w}, pair)), arrived(f.two[i / 2]);
+        else f.last = w, arrived(f.last);
+        arrived(total);   /* here, not where they are used */
+    }
+    __device__ inline void finish(const Soft &f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p.two[i] = f.two[i];
+        if (f.moved)
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= f.by;
+    }
+    __device__ inline f32x16 scores(uint32_t at) const {
+        f32x16 acc = {};
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc = Mma<T>::go(keys(at, i), qf[i], acc);
+        in_step<N, 1, 4>();
+        return acc;
+    }
+    __device__ inline void weigh(uint32_t at) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i % DT] = Mma<T>::go(values(at, i), p.whole[i / DT], o[i % DT]);
+        in_step<N, 2, 3>();
+    }
+    __device__ inline void softmax() {
+        Soft f;
+        look(f);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) weight(f, i);
+        finish(f);
+    }
+    /* the scores of the block at k_at, the weights of the last one, and p times the values at v_at */
+    __device__ inline void step(uint32_t k_at, uint32_t v_at) {
+        constexpr int AHEAD = 3, PRODUCTS = 2 * N;
+        f32x16 acc = {};
+        frag kf[N], vf[N];
+        Soft f;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) kf[i] = keys(k_at, i), vf[i] = values(v_at, i);
+        each<0, PRODUCTS>([&](auto at) __attribute__((always_inline)) {
+            constexpr int m = decltype(at)::value, i = m / 2;
+            __builtin_amdgcn_sched_barrier(0);
+            if (m % 2 == 0) {
+                if (i + AHEAD < N) kf[i + AHEAD] = keys(k_at, i + AHEAD), vf[i + AHEAD] = values(v_at, i + AHEAD);
+                acc = Mma<T>::go(kf[i], qf[i], acc);
+            } else
+                o[i % DT] = Mma<T>::go(vf[i], p.whole[i / DT], o[i % DT]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (m == 1) look(f);
+            if (m >= 2)
+#pragma unroll
+                for (int j = (m - 2) * 16 / (PRODUCTS - 2); j < (m - 1) * 16 / (PRODUCTS - 2); ++j) weight(f, j);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        finish(f);
+        s = acc;
+    }
+};
+
 /* Prompts: a workgroup takes 128 queries of a head, 32 per wavefront, and walks over its keys in tiles of 64, the next tile on its
  * way while one is worked on.  Tiles of 32 keys, which leave registers for a third wavefront per SIMD, took 3% off where a window is
  * 512 and added 6% where it is 2,048; single blocks of 32 at a window's edges took nothing off and added 7%.
@@ -368,36 +493,60 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
     const T *k = (const T *)a.k + b * a.k_stride[0] + head / a.shared * a.k_stride[2], *v = (const T *)a.v + b * a.v_stride[0] + head / a.shared * a.v_stride[2];
     const Tiles tiles = tiles_of<KEYS>(a, seq, seq.start + q0, seq.start + last);
     const uint32_t lds0 = lds_offset(lds);
-    const Operands<T, PITCH> ops(lane);
     const Tile<T, PITCH, KEYS, LANES> ktiles(k, a.k_stride[1], a.dim, threadIdx.x), vtiles(v, a.v_stride[1], a.dim, threadIdx.x);
+    /* a buffer holds a tile's keys and the values of the tile before it: those of two blocks behind */
     auto ask = [&](int t) {
         const uint32_t to = lds0 + (t & 1) * 2 * TILE;
-        const int at = tiles.tile(t) * KEYS;
-        ktiles.ask(to, at, seq.length), vtiles.ask(to + TILE, at, seq.length);
+        if (t < tiles.count) ktiles.ask(to, tiles.tile(t) * KEYS, seq.length);
+        if (t > 0) vtiles.ask(to + TILE, tiles.tile(t - 1) * KEYS, seq.length);
     };
     if (tiles.count > 0) ask(0);
     const T *qrow = (const T *)a.q + b * a.q_stride[0] + (int64_t)query * a.q_stride[1] + head * a.q_stride[2];
-    typename Mma<T>::frag qf[DP / 16];
+    Walk<T, DP, PITCH> walk;
+    walk.start(Operands<T, PITCH>(lane), lds0, a.scale2);
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) qf[s] = global_frag<T>(qrow, s * 16 + half * 8, a.dim, query < a.queries);
+    for (int s = 0; s < DP / 16; ++s) walk.qf[s] = global_frag<T>(qrow, s * 16 + half * 8, a.dim, query < a.queries);
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) arrived(qf[s]);
-    Running<DP / 32> run;
-    run.clear();
+    for (int s = 0; s < DP / 16; ++s) arrived(walk.qf[s]);
     const Sight sight(a, seq.length, seq.start + query);
     const int lo = seq.start + mine, hi = seq.start + (mine + 31 < a.queries ? mine + 31 : a.queries - 1);
-    for (int t = 0; t < tiles.count; ++t) {
+    const Clear clear(a, seq.length, lo, hi);
+    auto mask = [&](int key0) {
+        if (!clear.block(key0)) hide(walk.s, sight, key0, half, key0 < a.sinks, -__builtin_inff());
+    };
+    auto arrive = [&](int t) {
         wait_tiles<0>();
         meet();
-        if (t + 1 < tiles.count) ask(t + 1);
-        const int at = tiles.tile(t) * KEYS;
-        if (mine >= a.queries || none_see(a, seq.length, lo, hi, at, at + KEYS)) continue;
-        const uint32_t ktile = lds0 + (t & 1) * 2 * TILE;
-        block_step<T, DP, PITCH, KEYS / 32>(run, qf, ops, ktile, ktile + TILE, a, sight, at, !all_see(a, seq.length, lo, hi, at, at + KEYS), lane);
+        if (t < tiles.count) ask(t + 1);
+    };
+    constexpr int BLOCK = 32 * PITCH * 2;
+    if (tiles.count > 0) {
+        arrive(0);
+        walk.s = walk.scores(0);
+        mask(tiles.tile(0) * KEYS);
+        walk.softmax();
+        walk.s = walk.scores(BLOCK);
+        mask(tiles.tile(0) * KEYS + 32);
+        auto middle = [&](int t, uint32_t at) {
+            arrive(t);
+            const int key0 = tiles.tile(t) * KEYS;
+            walk.step(at, at + TILE);
+            mask(key0);
+            walk.step(at + BLOCK, at + TILE + BLOCK);
+            mask(key0 + 32);
+        };
+        int t = 1;
+        for (; t + 1 < tiles.count; t += 2) middle(t, 2 * TILE), middle(t + 1, 0);
+        if (t < tiles.count) middle(t, 2 * TILE), ++t;
+        arrive(t);
+        const uint32_t at = (t & 1) * 2 * TILE + TILE;
+        walk.weigh(at);
+        walk.softmax();
+        walk.weigh(at + BLOCK);
     }
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t) arrived(run.o[t]);
-    const float total = sum_halves(run.total);
+    for (int t = 0; t < DP / 32; ++t) arrived(walk.o[t]);
+    const float total = sum_halves(walk.total);
     if (query >= a.queries) return;
     const float by = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total;   /* (nothing visible: zero; not a number: that) */
     T *to = (T *)a.out + b * a.out_stride[0] + (int64_t)query * a.out_stride[1] + head * a.out_stride[2];
@@ -406,9 +555,9 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             const int d = t * 32 + result_row(i, half);
-            if (d < a.dim) store4(to + d, run.o[t][i] * by, run.o[t][i + 1] * by, run.o[t][i + 2] * by, run.o[t][i + 3] * by);
+            if (d < a.dim) store4(to + d, walk.o[t][i] * by, walk.o[t][i + 1] * by, walk.o[t][i + 2] * by, walk.o[t][i + 3] * by);
         }
-    if (half == 0) a.lse[((int64_t)b * a.heads + head) * a.queries + query] = total == 0.0f ? -__builtin_inff() : run.top * a.scale + __logf(total);
+    if (half == 0) a.lse[((int64_t)b * a.heads + head) * a.queries + query] = total == 0.0f ? -__builtin_inff() : walk.top * a.scale + __logf(total);
 }
 
 /* Few queries: the queries of a key head's heads are the columns of one block of 32; every wavefront walks over tiles of 32 keys
@@ -445,6 +594,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split
     Running<DP / 32> run;
     run.clear();
     const Sight sight(a, seq.length, seq.start + query);
+    const Clear clear(a, seq.length, lo, hi);
     int buffer = 0;
     if (worker < tiles.count) ask(worker, 0);
     for (int t = worker; t < tiles.count; t += workers, buffer ^= 1) {
@@ -457,7 +607,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split
             wait_tiles<0>();
         const int at = tiles.tile(t) * SPLIT_KEYS;
         const uint32_t ktile = lds0 + buffer * 2 * TILE;
-        block_step<T, DP, PITCH, 1>(run, qf, ops, ktile, ktile + TILE, a, sight, at, !all_see(a, seq.length, lo, hi, at, at + SPLIT_KEYS), lane);
+        block_step<T, DP, PITCH, 1>(run, qf, ops, ktile, ktile + TILE, a, sight, at, !clear.block(at), lane);
     }
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(run.o[t]);
@@ -582,6 +732,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
     arrived(lse2);
     const int lo = seq.start + mine, hi = seq.start + (mine + 31 < a.queries ? mine + 31 : a.queries - 1);
     const Sight sight(a, seq.length, seq.start + query);
+    const Clear clear(a, seq.length, lo, hi);
     /* With few keys the rounding of the forward pass's answer, which delta goes by, is no small part of dS: there delta is the sum of
      * P dP itself, in a walk before the walk. */
     const bool few = tiles.count <= FEW_TILES;
@@ -620,7 +771,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
                 const float less = walk == 0 ? 0.0f : delta;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse2)) * (dp[i] - less);
-                if (!all_see(a, seq.length, lo, hi, key0, key0 + 32)) hide(ds, sight, key0, half, key0 < a.sinks, 0.0f);
+                if (!clear.block(key0)) hide(ds, sight, key0, half, key0 < a.sinks, 0.0f);
                 if (walk == 0) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sum += ds[i];
@@ -727,10 +878,10 @@ template <class T, int PITCH, int ROWS, int LANES> struct QueryTiles {
         qh.base += head * a.q_stride[2], gh.base += head * a.g_stride[2];
         qh.ask(lds, row, a.queries), gh.ask(lds + BYTES, row, a.queries);
         const int second = ROWS > 64 ? wave >> 1 : 0, left = a.queries - row - 64 * second;
-        const int64_t at = (int64_t)head * a.queries + row + 64 * second, bytes = left < 0 ? 0 : (int64_t)(left < 64 && left < ROWS ? left : ROWS < 64 ? ROWS : 64) * 4;
+        const int64_t at = (int64_t)head * a.queries + row + 64 * second, last = left < 0 ? 0 : left < 64 && left < ROWS ? left : ROWS < 64 ? ROWS : 64;
         const uint32_t to = lds + 2 * BYTES + 256 * second;
-        if (LANES == 64 || (wave & 1) == 0) to_lds4(buffer(lse + at, bytes), lane * 4, __builtin_amdgcn_readfirstlane(to));
-        if (LANES == 64 || (wave & 1) == 1) to_lds4(buffer(delta + at, bytes), lane * 4, __builtin_amdgcn_readfirstlane(to + ROW_VALUES));
+        if (LANES == 64 || (wave & 1) == 0) to_lds4(buffer(lse + at, (uint32_t)last * 4), lane * 4, __builtin_amdgcn_readfirstlane(to));
+        if (LANES == 64 || (wave & 1) == 1) to_lds4(buffer(delta + at, (uint32_t)last * 4), lane * 4, __builtin_amdgcn_readfirstlane(to + ROW_VALUES));
     }
 };
 
