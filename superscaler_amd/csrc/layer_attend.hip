@@ -197,22 +197,21 @@ template <int SIZE> __device__ inline Tiles tiles_of(const Args &a, const Sequen
     return {first, at, first + to - at};
 }
 
-/* whether positions lo..hi all do not see keys from..to - 1 */
-__device__ inline bool none_see(const Args &a, int length, int lo, int hi, int from, int to) {
-    return from >= length || from > hi || (a.window > 0 && lo - (to - 1) >= a.window && from >= a.sinks);
-}
-
-/* The keys that positions lo..hi all see by their window: `count` blocks of 32 begin at `from` or behind it. */
-struct Clear {
+/* Numbers from `from` to `end` - 1, asked for by one comparison. */
+struct Range {
     int from;
     uint32_t count;
-    __device__ inline Clear(const Args &a, int length, int lo, int hi) {
-        from = a.window > 0 && hi >= a.window ? hi - a.window + 1 : 0;
-        const int end = length < lo + 1 ? length : lo + 1;
-        count = end - from >= 32 ? end - from - 31 : 0;
-    }
-    __device__ inline bool block(int key0) const { return (uint32_t)(key0 - from) < count; }
+    __device__ inline Range(int f, int end) : from(f), count(end > f ? end - f : 0) {}
+    __device__ inline bool has(int i) const { return (uint32_t)(i - from) < count; }
 };
+__device__ inline int lesser(int a, int b) { return a < b ? a : b; }
+/* Where a block of 32 keys begins that positions lo..hi all see by their window, and one that any of them sees. */
+__device__ inline Range all_see(const Args &a, int length, int lo, int hi) {
+    return Range(a.window > 0 && hi >= a.window ? hi - a.window + 1 : 0, lesser(length, lo + 1) - 31);
+}
+__device__ inline Range any_see(const Args &a, int length, int lo, int hi) {
+    return Range((a.window > 0 && lo >= a.window ? lo - a.window + 1 : 0) - 31, lesser(length, hi + 1));
+}
 
 /* What a query sees: `count` keys from `from` on, and those below `first`. */
 struct Sight {
@@ -276,32 +275,24 @@ __device__ inline float max_halves(float x) {
     return fmaxf(__uint_as_float(a), __uint_as_float(b));
 }
 
-/* One block of 32 keys times NB more for 32 queries: scores, softmax, weighted values.  The maximum that exponentials are taken
- * around moves only when a score passes it by 8 powers of two: the sums stay far from their range's end, and most blocks
- * need no rescaling. */
-template <class T, int DP, int PITCH, int NB> __device__ inline void block_step(Running<DP / 32> &run, const typename Mma<T>::frag *qf, const Operands<T, PITCH> &ops, uint32_t ktile, uint32_t vtile,
-                                                                                const Args &a, const Sight &sight, int key0, bool masked, int lane) {
+/* One block of 32 keys for 32 queries: scores, softmax, weighted values.  The maximum that exponentials are taken around moves only when a
+ * score passes it by 8 powers of two: the sums stay far from their range's end, and most blocks need no rescaling. */
+template <class T, int DP, int PITCH> __device__ inline void block_step(Running<DP / 32> &run, const typename Mma<T>::frag *qf, const Operands<T, PITCH> &ops, uint32_t ktile, uint32_t vtile,
+                                                                        const Args &a, const Sight &sight, int key0, bool masked, int lane) {
     const int half = lane >> 5;
-    float s[NB][16];
+    float s[16];
     float top = -__builtin_inff();
+    __builtin_amdgcn_s_setprio(1), __builtin_amdgcn_sched_barrier(0);
+    f32x16 acc = {};
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        if (n == 0) __builtin_amdgcn_s_setprio(1), __builtin_amdgcn_sched_barrier(0);
-        f32x16 acc = {};
+    for (int k = 0; k < DP / 16; ++k) acc = Mma<T>::go(ops.rows(ktile, 0, k), qf[k], acc);
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) acc = Mma<T>::go(ops.rows(ktile, n * 32, k), qf[k], acc);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = acc[i];
-    }
-    in_step<NB * DP / 16, 1, 4>();
+    for (int i = 0; i < 16; ++i) s[i] = acc[i];
+    in_step<DP / 16, 1, 4>();
     __builtin_amdgcn_s_setprio(0);
-    if (masked)
+    if (masked) hide(s, sight, key0, half, key0 < a.sinks, -__builtin_inff());
 #pragma unroll
-        for (int n = 0; n < NB; ++n) hide(s[n], sight, key0 + n * 32, half, key0 < a.sinks, -__builtin_inff());
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
     top = max_halves(top);
     const bool more = (top - run.top) * a.scale2 > 8.0f;   /* (also from no key at all, -inf, to any) */
     if (__any(more)) {
@@ -315,27 +306,21 @@ template <class T, int DP, int PITCH, int NB> __device__ inline void block_step(
             for (int i = 0; i < 16; ++i) run.o[t][i] *= by;
     }
     const float around = run.top == -__builtin_inff() ? 0.0f : run.top * a.scale2;
-    typename Mma<T>::frag pf[NB][2];
+    float sum = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], a.scale2, -around));
-            sum += s[n][i];
-        }
-        run.total += sum;
-        pf[n][0] = pack8<T>(s[n]), pf[n][1] = pack8<T>(s[n] + 8);
+    for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -around));
+        sum += s[i];
     }
+    run.total += sum;
+    const typename Mma<T>::frag pf[2] = {pack8<T>(s), pack8<T>(s + 8)};
     __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int t = 0; t < DP / 32; ++t) run.o[t] = Mma<T>::go(ops.columns(vtile, n * 32 + k * 16, t), pf[n][k], run.o[t]);
-    in_step<NB * 2 * DP / 32, 2, 3>();
+        for (int t = 0; t < DP / 32; ++t) run.o[t] = Mma<T>::go(ops.columns(vtile, k * 16, t), pf[k], run.o[t]);
+    in_step<2 * DP / 32, 2, 3>();
     __builtin_amdgcn_s_setprio(0);
 }
 
@@ -510,9 +495,9 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
     for (int s = 0; s < DP / 16; ++s) arrived(walk.qf[s]);
     const Sight sight(a, seq.length, seq.start + query);
     const int lo = seq.start + mine, hi = seq.start + (mine + 31 < a.queries ? mine + 31 : a.queries - 1);
-    const Clear clear(a, seq.length, lo, hi);
+    const Range clear = all_see(a, seq.length, lo, hi);
     auto mask = [&](int key0) {
-        if (!clear.block(key0)) hide(walk.s, sight, key0, half, key0 < a.sinks, -__builtin_inff());
+        if (!clear.has(key0)) hide(walk.s, sight, key0, half, key0 < a.sinks, -__builtin_inff());
     };
     auto arrive = [&](int t) {
         wait_tiles<0>();
@@ -594,7 +579,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split
     Running<DP / 32> run;
     run.clear();
     const Sight sight(a, seq.length, seq.start + query);
-    const Clear clear(a, seq.length, lo, hi);
+    const Range clear = all_see(a, seq.length, lo, hi);
     int buffer = 0;
     if (worker < tiles.count) ask(worker, 0);
     for (int t = worker; t < tiles.count; t += workers, buffer ^= 1) {
@@ -607,7 +592,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split
             wait_tiles<0>();
         const int at = tiles.tile(t) * SPLIT_KEYS;
         const uint32_t ktile = lds0 + buffer * 2 * TILE;
-        block_step<T, DP, PITCH, 1>(run, qf, ops, ktile, ktile + TILE, a, sight, at, !clear.block(at), lane);
+        block_step<T, DP, PITCH>(run, qf, ops, ktile, ktile + TILE, a, sight, at, !clear.has(at), lane);
     }
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(run.o[t]);
@@ -732,7 +717,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
     arrived(lse2);
     const int lo = seq.start + mine, hi = seq.start + (mine + 31 < a.queries ? mine + 31 : a.queries - 1);
     const Sight sight(a, seq.length, seq.start + query);
-    const Clear clear(a, seq.length, lo, hi);
+    const Range clear = all_see(a, seq.length, lo, hi), seen = any_see(a, seq.length, lo, hi);
+    const int first = a.window > 0 ? a.sinks : 0;
     /* With few keys the rounding of the forward pass's answer, which delta goes by, is no small part of dS: there delta is the sum of
      * P dP itself, in a walk before the walk. */
     const bool few = tiles.count <= FEW_TILES;
@@ -757,7 +743,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
             for (int n = 0; n < KEYS / 32; ++n) {
                 const int key0 = at + n * 32;
                 const uint32_t ktile = buffer_at + n * 32 * PITCH * 2, vtile = ktile + TILE;
-                if (none_see(a, seq.length, lo, hi, key0, key0 + 32)) continue;
+                if (!seen.has(key0) && key0 >= first) continue;
                 __builtin_amdgcn_s_setprio(1);
                 __builtin_amdgcn_sched_barrier(0);
                 f32x16 s = {}, dp = {};
@@ -771,7 +757,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
                 const float less = walk == 0 ? 0.0f : delta;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse2)) * (dp[i] - less);
-                if (!clear.block(key0)) hide(ds, sight, key0, half, key0 < a.sinks, 0.0f);
+                if (!clear.has(key0)) hide(ds, sight, key0, half, key0 < a.sinks, 0.0f);
                 if (walk == 0) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sum += ds[i];
@@ -925,6 +911,10 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
     /* this lane's key is seen from its own position on, for a window's length, by queries that there are */
     const int64_t left = (int64_t)seq.start + a.queries - key;
     const uint32_t sight = key >= seq.length || left <= 0 ? 0 : a.window > 0 && a.window < left ? a.window : (uint32_t)left;
+    /* where a block of 32 queries begins of which any sees one of the wavefront's keys, and one of which all see all */
+    const int begin = mine - seq.start;
+    const Range seen(begin - 31, mine < seq.length ? a.window > 0 ? lesser(begin + 31 + a.window, a.queries) : a.queries : begin - 31);
+    const Range clear(begin + 31, mine + 32 <= seq.length ? a.window > 0 ? lesser(begin - 31 + a.window, a.queries - 31) : a.queries - 31 : begin);
     if (steps > 0) ask(0);
     int q = first * ROWS;
     for (int t = 0; t < steps; ++t) {
@@ -933,11 +923,10 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
         if (t + 1 < steps) ask(t + 1);
         const uint32_t buffer_at = lds0 + (t & 1) * Queries::STAGE;
         auto half_tile = [&](int n) {
-            const int lo = seq.start + q + n * 32, hi = lo + 31;
-            if (mine >= seq.length || q + n * 32 >= a.queries || hi < mine || (a.window > 0 && lo - (mine + 31) >= a.window)) return;
-            const bool masked = q + n * 32 + 32 > a.queries || mine + 32 > seq.length || lo < mine + 31 || (a.window > 0 && hi - mine >= a.window);
+            const int q0 = q + n * 32;
+            if (!seen.has(q0)) return;
             const uint32_t qtile = buffer_at + n * 32 * PITCH * 2, lse = buffer_at + 2 * Queries::BYTES + n * 32 * 4;
-            grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + Queries::ROW_VALUES, a.scale2, lo - key, sight, masked, half);
+            grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + Queries::ROW_VALUES, a.scale2, seq.start + q0 - key, sight, !clear.has(q0), half);
         };
         if (SHARE > 1) half_tile(wave / OWNERS);
         else
