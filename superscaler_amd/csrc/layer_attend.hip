@@ -334,7 +334,7 @@ template <int DP> struct Shape { static constexpr int PITCH = DP <= 64 ? 64 : 12
 
 /* How many wavefronts of a SIMD a kernel is scheduled for: exactly as many as its registers allow, so that what is left of them goes to
  * operands on their way.  Without it: 4 x 40 heads of 2,048 tokens, a window of 512, 228 us instead of 160; 8 heads of 16,384, 2,048:
- * 230 instead of 157; 2 x 16 heads of 2,048, 1,024, forward and backward: 307 instead of 197. */
+ * 230 instead of 157; 2 x 16 heads of 2,048, 1,024, forward and backward: 307 instead of 197 (before blocks overlapped in the forward kernel). */
 #define RESIDENT(DP) __attribute__((amdgpu_waves_per_eu((DP) <= 64 ? 3 : 2, (DP) <= 64 ? 3 : 2)))
 
 constexpr int WAVES = 4, LANES = WAVES * 64, QUERIES = WAVES * 32, KEYS = 64;
@@ -457,13 +457,14 @@ template <class T, int DP, int PITCH> struct Walk {
 };
 
 /* Prompts: a workgroup takes 128 queries of a head, 32 per wavefront, and walks over its keys in tiles of 64, the next tile on its
- * way while one is worked on.  Tiles of 32 keys, which leave registers for a third wavefront per SIMD, took 3% off where a window is
- * 512 and added 6% where it is 2,048; single blocks of 32 at a window's edges took nothing off and added 7%.
+ * way while one is worked on; blocks that a wavefront does not see are masked like others (passing over them took 1% off where a
+ * window is 512 and added 3% where it is 2,048).  Tiles of 32 keys, which leave registers for a third wavefront per SIMD, took 3% off with
+ * a window of 512 and added 6% with 2,048.
  *
- * 4 x 40 heads of 2,048 tokens and size 128, a window of 512: 146 us, 518 TFLOP/s of the pairs that are seen; 8 heads of 16,384, 2,048:
- * 150 us, 868 (a large product of the matrix library: 1,250).  The two wavefronts of a SIMD share it: its matrix unit is at work 32%
- * and 48% of the time, softmax's 210 vector instructions to a tile's 32 matrix instructions about as much, and a short walk
- * pays for its first loads and last stores, some 5 us of 28.  LDS has no conflicts and is at work for less than a quarter. */
+ * 4 x 40 heads of 2,048 tokens and size 128, a window of 512: 139 us, 545 TFLOP/s of the pairs that are seen; 8 heads of 16,384, 2,048:
+ * 140 us, 926 (a large product of the matrix library: 1,250).  The card lowers its clock under this load: on zeros the same calls take
+ * 12% and 20% less, the library's product 25%; how operands and softmax are ordered further makes no difference.  A short walk pays for
+ * its first loads and last stores as well, some 5 us of 27.  LDS has no conflicts and is at work for less than a quarter of the time. */
 template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_forward(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
@@ -669,7 +670,7 @@ constexpr int FEW_TILES = 3;
 
 /* dQ: queries in registers, keys in tiles as in attend_forward; per block of 32 keys S^T = K Q^T, dP^T = V dO^T,
  * dQ^T += K^T dS^T.  It also leaves delta = sum dO O of every query for attend_dkv.  2 x 16 heads of 2,048 tokens and size 128, a window of
- * 1,024: 70 us, 555 TFLOP/s of the pairs that are seen, the matrix units at work 30% of the time. */
+ * 1,024: 67 us, 579 TFLOP/s of the pairs that are seen, the matrix units at work a third of the time. */
 template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_dq(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
@@ -874,7 +875,7 @@ template <class T, int PITCH, int ROWS, int LANES> struct QueryTiles {
 /* The pairs of a window: a workgroup takes 128 keys and walks over the queries whose window they are in, of every head that shares the
  * key head, in tiles of 64.  With SHARE 2 or 4 it takes 64 or 32 keys, and so many wavefronts share 32 keys and a tile's queries (128 of
  * them with SHARE 4): more workgroups, for calls that would leave CUs without one.  2 x 16 heads of 2,048 tokens and size 128, a window of
- * 1,024: 88 us, 588 TFLOP/s of the pairs that are seen, the matrix units at work 33% of the time: all 256 registers of a wavefront are
+ * 1,024: 79 us, 654 TFLOP/s of the pairs that are seen, the matrix units at work a third of the time: all 256 registers of a wavefront are
  * in use, and the four products of a block of 32 x 32 wait for each other. */
 constexpr int query_rows(int share) { return share == 4 ? 128 : 64; }
 template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_dkv(const Args a) {
