@@ -152,7 +152,7 @@ int64_t runs_of(const ace_block_norm_t *a) {
     return (a->rows + run - 1) / run;
 }
 
-int64_t gates_of(const ace_block_norm_t *a) { return a->d_gate ? (a->rows + a->rows_per_gate - 1) / a->rows_per_gate : 1; }
+int64_t gates_of(const ace_block_norm_t *a) { return a->d_gate && a->rows_per_gate < a->rows ? (a->rows + a->rows_per_gate - 1) / a->rows_per_gate : 1; }
 
 bool token_gate(const ace_block_norm_t *a) { return a->d_gate && a->rows_per_gate == 1 && a->rows > 1; }
 
@@ -170,7 +170,7 @@ int check(const ace_block_norm_t *a) {
 
 NormArgs args_of(const ace_block_norm_t *a) {
     NormArgs k = {};
-    k.rows = a->rows, k.rows_per_gate = a->d_gate ? a->rows_per_gate : a->rows + 1, k.gates = gates_of(a);
+    k.rows = a->rows, k.rows_per_gate = a->d_gate && a->rows_per_gate <= a->rows ? a->rows_per_gate : a->rows + 1, k.gates = gates_of(a);
     k.width = a->width, k.layer = a->layer, k.alpha = a->d_block ? a->residual_scale : 1.0f, k.eps = a->eps;
     k.x = a->d_x, k.f = a->d_block, k.gate = a->d_gate, k.w2 = a->d_exit_weight, k.b2 = a->d_exit_bias, k.w1 = a->d_entry_weight, k.b1 = a->d_entry_bias;
     return k;

@@ -139,7 +139,7 @@ def _rows_per_gate(gate_shape, shape):
 
 
 def _fits(t, dtype, device, shape):
-    return t is None or (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and (shape is None or t.shape == shape))
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and (shape is None or t.shape == shape)
 
 
 def _refuse_block_norm(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind):
@@ -176,8 +176,9 @@ def _block_norm_args(x, block, residual_scale, gate, exit_weight, exit_bias, ent
         _refuse_block_norm(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind)
     dtype, device, shape = x.dtype, x.device, x.shape
     width = shape[-1:]
-    if not (_fits(block, dtype, device, shape) and _fits(gate, dtype, device, None) and _fits(exit_weight, dtype, device, width) and
-            _fits(exit_bias, dtype, device, width) and _fits(entry_weight, dtype, device, width) and _fits(entry_bias, dtype, device, width)) or \
+    if not ((block is None or _fits(block, dtype, device, shape)) and (gate is None or _fits(gate, dtype, device, None)) and
+            (exit_weight is None or _fits(exit_weight, dtype, device, width)) and (exit_bias is None or _fits(exit_bias, dtype, device, width)) and
+            (entry_weight is None or _fits(entry_weight, dtype, device, width)) and (entry_bias is None or _fits(entry_bias, dtype, device, width))) or \
             (exit_bias is not None and exit_weight is None) or (entry_bias is not None and entry_weight is None) or \
             (block is None and (entry_weight is None or gate is not None or exit_weight is not None or residual_scale != 1.0)):
         _refuse_block_norm(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind)

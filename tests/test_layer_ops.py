@@ -61,6 +61,8 @@ def test_refusals_of_the_c_entries():
     assert lib.ace_block_norm_forward(norm(rows=0), 64, None, 64, None) == 0       # no rows
     assert lib.ace_block_norm_backward(norm(), 64, None, 64, 64, 64, None, None, None, None, None, None, 0, None) == -1   # no workspace
     assert lib.ace_block_norm_workspace_bytes(norm()) == 2 * 4 * 8 * 4
+    one_gate = layer._BLOCK_NORM.pack(4, (1 << 63) - 1, 8, 1, 1, 1.0, 1e-5, 64, 64, 64, 0, 0, 0, 0)
+    assert lib.ace_block_norm_workspace_bytes(one_gate) == 2 * 4 * 8 * 4      # (as many rows per gate as there can be)
 
     def attend(**change):
         a = dict(batch=2, queries=32, keys=32, heads=4, kv_heads=2, dim=64, dtype=1, window=0, sinks=0, scale=0.125, d_start=0, d_length=0)
