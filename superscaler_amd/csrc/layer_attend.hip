@@ -457,8 +457,8 @@ template <class T, int DP, int PITCH> struct Walk {
 };
 
 /* Prompts: a workgroup takes 128 queries of a head, 32 per wavefront, and walks over its keys in tiles of 64, the next tile on its
- * way while one is worked on; blocks that a wavefront does not see are masked like others (passing over them took 1% off where a
- * window is 512 and added 3% where it is 2,048).  Tiles of 32 keys, which leave registers for a third wavefront per SIMD, took 3% off with
+ * way while one is worked on; blocks that a wavefront does not see are masked like others, but for the second and the last two
+ * (passing over the rest took 1% off where a window is 512 and added 3% where it is 2,048).  Tiles of 32 keys, which leave registers for a third wavefront per SIMD, took 3% off with
  * a window of 512 and added 6% with 2,048.
  *
  * 4 x 40 heads of 2,048 tokens and size 128, a window of 512: 139 us, 545 TFLOP/s of the pairs that are seen; 8 heads of 16,384, 2,048:
@@ -496,7 +496,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
     for (int s = 0; s < DP / 16; ++s) arrived(walk.qf[s]);
     const Sight sight(a, seq.length, seq.start + query);
     const int lo = seq.start + mine, hi = seq.start + (mine + 31 < a.queries ? mine + 31 : a.queries - 1);
-    const Range clear = all_see(a, seq.length, lo, hi);
+    const Range clear = all_see(a, seq.length, lo, hi), seen = any_see(a, seq.length, lo, hi);
+    const int sinks = a.window > 0 ? a.sinks : 0;
     auto mask = [&](int key0) {
         if (!clear.has(key0)) hide(walk.s, sight, key0, half, key0 < a.sinks, -__builtin_inff());
     };
@@ -511,7 +512,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
         walk.s = walk.scores(0);
         mask(tiles.tile(0) * KEYS);
         walk.softmax();
-        walk.s = walk.scores(BLOCK);
+        /* (a tile of first keys is often one block only, and the last tile's blocks are not seen by the first wavefronts) */
+        if (seen.has(tiles.tile(0) * KEYS + 32) || tiles.tile(0) * KEYS + 32 < sinks) walk.s = walk.scores(BLOCK);
         mask(tiles.tile(0) * KEYS + 32);
         auto middle = [&](int t, uint32_t at) {
             arrive(t);
@@ -526,9 +528,12 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
         if (t < tiles.count) middle(t, 2 * TILE), ++t;
         arrive(t);
         const uint32_t at = (t & 1) * 2 * TILE + TILE;
-        walk.weigh(at);
-        walk.softmax();
-        walk.weigh(at + BLOCK);
+        const int key0 = tiles.tile(t - 1) * KEYS;
+        if (seen.has(key0) || key0 < sinks) walk.weigh(at);
+        if (seen.has(key0 + 32) || key0 + 32 < sinks) {
+            walk.softmax();
+            walk.weigh(at + BLOCK);
+        }
     }
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(walk.o[t]);
