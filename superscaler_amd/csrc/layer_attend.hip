@@ -353,7 +353,7 @@ template <class T, int DP, int PITCH> struct Walk {
     typedef typename Mma<T>::frag frag;
     typedef T pair __attribute__((ext_vector_type(2)));
     typedef float f32x2 __attribute__((ext_vector_type(2)));
-    static constexpr int N = DP / 16, DT = DP / 32, TILE = KEYS * PITCH * 2, BLOCK = 32 * PITCH * 2;
+    static constexpr int N = DP / 16, DT = DP / 32;
     uint32_t row[N], column[2 * DT];   /* where a lane finds operands in a tile at 0 */
     frag qf[N];
     f32x16 o[DT], s;                   /* weighted values; scores of the last block */

@@ -29,7 +29,7 @@ int norm_backward_launch(const NormArgs &a, int dtype, hipStream_t stream);
 struct NormShape { int nv, lanes; };
 inline NormShape norm_shape(int width, int bytes, bool forward) {
     const int v = (width + 7) / 8, one = forward ? 768 : 1024;
-    const int nv = bytes == 2 ? (v <= one ? 1 : v <= 1536 ? 2 : v <= 3072 ? 3 : 4) : (v <= 960 ? 1 : v <= 3072 ? 3 : 4);
+    const int nv = bytes == 2 ? (v <= one ? 1 : v <= 1536 ? 2 : v <= 3 * 1024 ? 3 : 4) : (v <= 960 ? 1 : v <= 3 * 1024 ? 3 : 4);
     return {nv, ((v + nv - 1) / nv + 63) / 64 * 64};
 }
 template <int NV> constexpr bool norm_params_in_lds() { return NV <= 2; }

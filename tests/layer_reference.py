@@ -1,5 +1,5 @@
 """The training-layer operators in 64 bits, from their definitions, with bounds on what a computation in 32 bits (and its
-roundings to the tensors' type) may differ by.  Checker only."""
+roundings to the tensors' type) may differ by.  For the tests only."""
 import math
 
 import torch

@@ -372,6 +372,17 @@ def test_attention_gradients_of_few_and_many_heads(batch, heads, kv_heads, dim, 
 
 
 @gpu
+@pytest.mark.parametrize("batch", [1, 6, 19])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (90, 5), (33, 70)])
+def test_attention_gradients_of_ragged_sequences(batch, window, sinks):
+    """Key blocks of 32, 64 and 128 keys per workgroup, sequences of any length that begin anywhere."""
+    device = cuda_or_skip()
+    lengths = (torch.arange(batch, dtype=torch.int32) * 53 + 201) % 271
+    start = (torch.arange(batch, dtype=torch.int32) * 61 + 17) % 300 - 120
+    check_attention(*attention_case(53, batch, 265, 270, 8, 8, 64, BF16), device, window=window, sinks=sinks, start=start, lengths=lengths)
+
+
+@gpu
 @pytest.mark.parametrize("window,sinks", [(None, 0), (150, 3), (1, 0)])
 @pytest.mark.parametrize("batch,queries,keys,heads,kv_heads", [(1, 1, 700, 2, 2), (3, 7, 1200, 6, 2), (1, 16, 1000, 40, 4), (2, 100, 1500, 2, 1), (20, 1, 256, 20, 20), (3, 128, 600, 2, 2),
                                                                (40, 9, 200, 8, 1)])
