@@ -324,6 +324,50 @@ template <class T, int DP, int PITCH> __device__ inline void block_step(Running<
     __builtin_amdgcn_s_setprio(0);
 }
 
+/* Half precision has five bits of exponent, and gradients of scores go with those of the answer, of any size, and with weights that a
+ * long sequence makes small.  So they meet their products with a power of two of the lane's query or key, which moves only when a
+ * gradient would pass 2^15 (the largest is 2^8 to 2^9 then: what is 2^22 times smaller still has all its bits) and takes the sums along.
+ * It begins where no gradient above 2^-49 leaves it.  Normalized weights, 1 at most, meet theirs with 2^12.  The backward pass of 2 x 16
+ * heads of 2,048 tokens and size 128, a window of 1,024, takes 164 us with this and 152 without. */
+template <class T> struct Fit {
+    static constexpr bool FITS = __is_same(T, f16);
+    static constexpr int FIRST = FITS ? 64 : 0, WEIGHTS = FITS ? 12 : 0;
+    int power;
+    __device__ inline void start() { power = FIRST; }
+    /* of gradients that have been multiplied: the change of the power, 0 or less */
+    template <int DT> __device__ inline int check(float (&ds)[16], f32x16 (&sums)[DT]) {
+        if (!FITS) return 0;
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, __builtin_fabsf(ds[i]));
+        if (!__any(most > 32768.0f)) return 0;
+        most = max_halves(most);
+        const int change = most > 32768.0f && most < __builtin_inff() ? 127 + 8 - (int)(__float_as_uint(most) >> 23) : 0;
+        power += change;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_ldexpf(ds[i], change);
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[t][i] = __builtin_amdgcn_ldexpf(sums[t][i], change);
+        return change;
+    }
+    template <int DT> __device__ inline void apply(float (&ds)[16], f32x16 (&sums)[DT]) {
+        if (!FITS) return;
+        const float by = __uint_as_float((uint32_t)(127 + power) << 23);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ds[i] *= by;
+        check(ds, sums);
+    }
+    template <int DT> static __device__ inline void undo(f32x16 (&sums)[DT], int by) {
+        if (!FITS) return;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[t][i] = __builtin_amdgcn_ldexpf(sums[t][i], -by);
+    }
+};
+
 /* Four neighbouring elements of a result, rounded. */
 template <class T> __device__ inline void store4(T *to, float a, float b, float c, float d) {
     typedef T vec __attribute__((ext_vector_type(4)));
@@ -729,9 +773,12 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
      * P dP itself, in a walk before the walk. */
     const bool few = tiles.count <= FEW_TILES;
     float sum = 0.0f;
+    Fit<T> fit;
+    fit.start();
     for (int walk = few ? 0 : 1; walk < 2; ++walk) {
         if (walk == 1) {
             if (few) delta = sum_halves(sum);
+            lse2 -= (float)fit.power;   /* (weights of the first walk are as they are; here their exponent is rounded to 2^-18) */
             if (there && half == 0) a.delta[flat] = delta;
         }
         if (few && walk == 1) {
@@ -769,6 +816,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
                     for (int i = 0; i < 16; ++i) sum += ds[i];
                     continue;
                 }
+                lse2 -= (float)fit.check(ds, dq);
                 const typename Mma<T>::frag df[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
                 __builtin_amdgcn_s_setprio(1);
                 __builtin_amdgcn_sched_barrier(0);
@@ -783,6 +831,7 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
     }
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(dq[t]);
+    fit.undo(dq, fit.power);
     if (!there) return;
     T *to = (T *)a.dq + (((int64_t)b * a.queries + query) * a.heads + head) * a.dim;
 #pragma unroll
@@ -800,6 +849,7 @@ template <class T, int DP> struct KeyGrads {
     static constexpr int PITCH = Shape<DP>::PITCH;
     typename Mma<T>::frag kf[DP / 16], vf[DP / 16];
     f32x16 dk[DP / 32], dv[DP / 32];
+    Fit<T> fit;
     __device__ inline void start(const T *krow, const T *vrow, int dim, bool there, int half) {
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) kf[s] = global_frag<T>(krow, s * 16 + half * 8, dim, there), vf[s] = global_frag<T>(vrow, s * 16 + half * 8, dim, there);
@@ -807,10 +857,12 @@ template <class T, int DP> struct KeyGrads {
         for (int s = 0; s < DP / 16; ++s) arrived(kf[s]), arrived(vf[s]);
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
+        fit.start();
     }
     __device__ inline void stop() {
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t) arrived(dk[t]), arrived(dv[t]);
+        fit.undo(dk, fit.power + Fit<T>::WEIGHTS), fit.undo(dv, Fit<T>::WEIGHTS);
     }
     /* `t`: the first query's position from the first one that sees this lane's key; the `count` from there on see it */
     __device__ inline void step(const Operands<T, PITCH> &ops, uint32_t qtile, uint32_t gtile, uint32_t lse, uint32_t delta, float scale2, int t, uint32_t count, bool masked,
@@ -830,7 +882,8 @@ template <class T, int DP> struct KeyGrads {
             const f32x4 l = lds_load<f32x4>(lse + 16 * half + 8 * i), d = lds_load<f32x4>(delta + 16 * half + 8 * i);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                prob[i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + e], scale2, -l[e] * LOG2E));
+                const float lse2 = Fit<T>::FITS ? __builtin_fmaf(l[e], -LOG2E, (float)Fit<T>::WEIGHTS) : -l[e] * LOG2E;
+                prob[i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + e], scale2, lse2));
                 ds[i + e] = prob[i + e] * (dp[i + e] - d[e]);
             }
         }
@@ -838,6 +891,7 @@ template <class T, int DP> struct KeyGrads {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if ((uint32_t)(t + result_row(i, half)) >= count) prob[i] = ds[i] = 0.0f;
+        fit.apply(ds, dk);
         const typename Mma<T>::frag pf[2] = {pack8<T>(prob), pack8<T>(prob + 8)}, df[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
         __builtin_amdgcn_s_setprio(1);
         __builtin_amdgcn_sched_barrier(0);
