@@ -10,7 +10,8 @@ timed works together.  Collectives and bandwidths between GPUs cannot be taken o
 Prints one JSON line; `--out` writes the database as files.
 
 A row's times are those of calls that follow each other on the card without waiting for the host, as in a training step whose host is
-ahead.
+ahead.  Its reserved memory is what a call has in use at its peak beyond what it leaves: forward its results, backward the gradients
+of weights.
 
 Attention is one operator here: its time stands in the row of the scores, which keeps the answer and a log-sum per query, and the rows of
 softmax, dropout and context keep and take nothing.  A block's residual addition is part of the norm behind it, whose row has both.
@@ -141,16 +142,29 @@ def _time_us(call, reps, device="cuda:0"):
     return statistics.median(times)
 
 
+def _reserved_mb(call, device="cuda:0", left=None):
+    """MB that `call` has in use at its peak beyond its results, or beyond `left` MB of them."""
+    torch.cuda.synchronize(device)
+    before = torch.cuda.memory_allocated(device)
+    torch.cuda.reset_peak_memory_stats(device)
+    results = call()
+    peak, after = torch.cuda.max_memory_allocated(device), torch.cuda.memory_allocated(device)
+    del results
+    return max(0.0, (peak - after) * MB if left is None else (peak - before) * MB - left)
+
+
 def measure(w, micro_batch, tp, window=None, sinks=0, vocab=51200, reps=10, device="cuda:0"):
-    """{operator name: (forward us, backward us)} of a layer's shard of workload `w`, for the rows of opgraph.GPT_TYPES."""
+    """{operator name: (forward us, backward us, reserved forward MB, backward MB)} of a layer's shard of workload `w`, for the rows of
+    opgraph.GPT_TYPES."""
     net, h, s = GptLayer(w.hidden, tp, window, sinks, device), w.hidden, w.seq
     x = torch.randn(micro_batch, s, h, device=device).bfloat16()
     block, d = torch.randn_like(x), torch.randn_like(x)
     r2, m, saved = net.forward(x, block)
-    out = {name: (0.0, 0.0) for name in CONTAINED}
+    out = {name: (0.0,) * 4 for name in CONTAINED}
 
     def both(name, forward, backward):
-        out[name] = (_time_us(forward, reps, device), _time_us(backward, reps, device))
+        out[name] = (_time_us(forward, reps, device), _time_us(backward, reps, device), _reserved_mb(forward, device),
+                     _reserved_mb(backward, device, sizes(w, name, micro_batch, tp)[2]))
 
     def product(name, a, weight):
         a = a.flatten(0, -2)
@@ -189,15 +203,16 @@ def sizes(w, name, micro_batch, tp):
 
 
 def database(w, graph, measured, base):
-    """The database `base` of workload `w` with the rows of `measured` ({(micro-batch, tp): measure's result}) in their places."""
+    """The database `base` of workload `w` with the rows of `measured` ({(micro-batch, tp): measure's result}) in their places; of
+    rows that are two times only, the reserved memory stays that of `base`."""
     db = ProfileDB.empty(w.model_name, base.op_names, base.mbs_list, base.tp_list, base.n_algo)
     db.collectives, db.intra_band, db.inter_band = base.collectives, base.intra_band, base.inter_band
     for f in FIELDS:
         db.tables[f][...] = base.tables[f]
     for (b, tp), rows in measured.items():
         at = db.mbs_list.index(b), db.tp_list.index(tp)
-        for name, (fwd, bwd) in rows.items():
-            values = dict(zip(FIELDS[2:6], sizes(w, name, b, tp)), fwd=fwd, bwd=bwd, reserved_fwd=0.0, reserved_bwd=0.0)
+        for name, row in rows.items():
+            values = dict(zip(FIELDS[2:6], sizes(w, name, b, tp)), **dict(zip(FIELDS[:2] + FIELDS[6:], row)))
             for f, v in values.items():
                 db.tables[f][(db.op_names.index(name),) + at] = round(v, 3)
     return db
@@ -248,7 +263,7 @@ def main(argv=None):
     db = database(w, graph, measured, base)
     result = {"workload": w.name, "ops": graph.num_ops, "window": args.window, "sinks": args.sinks, "measured": len(measured)}
     (b, tp), rows = next(iter(measured.items()))
-    result["forward_backward_us"] = {f"micro-batch {b}, tp {tp}": {n: [round(f, 1), round(g, 1)] for n, (f, g) in rows.items()}}
+    result["forward_backward_us"] = {f"micro-batch {b}, tp {tp}": {n: [round(t, 1) for t in row[:2]] for n, row in rows.items()}}
     if args.out:
         write(db, f"{w.model_name}_{w.name}", args.out)
     for bits, kind in ((32, CostModelSettings), (8, EightBitSettings)):

@@ -1,12 +1,28 @@
-"""What a measured profile database says of itself: times of the card and not of the host."""
+"""What a measured profile database says of itself: times of the card and not of the host, and reserved memory."""
 import time
 
+import numpy as np
 import pytest
 import torch
 
-from superscaler_amd import profile_layer
+from superscaler_amd import opgraph, profile_layer, synth
 
 gpu = pytest.mark.gpu
+
+
+def database(row):
+    w = synth.WORKLOADS["gpt3_1_3b"]
+    base = synth.make_db(w, synth.make_graph(w))
+    return base, profile_layer.database(w, synth.make_graph(w), {(2, 4): {name: row for name in opgraph.GPT_TYPES}}, base)
+
+
+def test_reserved_memory_is_what_was_measured():
+    base, db = database((1.0, 2.0, 3.5, 4.25))
+    assert (db.tables["reserved_fwd"][:, 1, 2] == 3.5).all() and (db.tables["reserved_bwd"][:, 1, 2] == 4.25).all()
+    assert (db.tables["fwd"][:, 1, 2] == 1.0).all() and (db.tables["bwd"][:, 1, 2] == 2.0).all()
+    base, db = database((1.0, 2.0))      # times only: nothing is known of the rest
+    for f in ("reserved_fwd", "reserved_bwd"):
+        assert base.tables[f].any() and np.array_equal(db.tables[f], base.tables[f])
 
 
 @gpu
@@ -24,3 +40,20 @@ def test_times_are_the_card_s():
     assert 0.5 < profile_layer._time_us(call, 10) < 100
     big = torch.zeros(1 << 28, device="cuda")      # 1 GiB read and written: 0.27 ms at the card's peak, some 0.41 at a copy's rate
     assert 250 < profile_layer._time_us(lambda: big.add_(1.0), 10) < 1000
+
+
+@gpu
+def test_reserved_memory_is_what_a_call_gives_back():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+
+    def mb(n):
+        return torch.empty(n << 20, dtype=torch.uint8, device="cuda")
+
+    def call():
+        kept, scratch = mb(64), mb(96)
+        del scratch
+        return kept
+    assert profile_layer._reserved_mb(call) == 96.0
+    assert profile_layer._reserved_mb(call, left=40.0) == 120.0
+    assert profile_layer._reserved_mb(lambda: mb(32)) == 0.0
