@@ -7,14 +7,16 @@ tensor-parallel degree of the workload: products by the matrix library, norms wi
 The times go into a database of the form that ProfileDB.from_directory loads; seeded plans are scored with it twice, with the
 optimizer's moments in 32 bits and in 8.  `--steps` trains the layer for that many steps with both, as a check that what was
 timed works together.  Collectives and bandwidths between GPUs cannot be taken on one card: they are those of the synthetic database.
-Prints one JSON line; `--out` writes the database as files.
+Where only some sizes and degrees are measured, the others are the synthetic database's, too: the line names them and no best plan.
+Prints one JSON line; `--out` writes the database as files, and beside them which of them were measured.
 
 A row's times are those of calls that follow each other on the card without waiting for the host, as in a training step whose host is
 ahead.  Its reserved memory is what a call has in use at its peak beyond what it leaves: forward its results, backward the gradients
 of weights.
 
 Attention is one operator here: its time stands in the row of the scores, which keeps the answer and a log-sum per query, and the rows of
-softmax, dropout and context keep and take nothing.  A block's residual addition is part of the norm behind it, whose row has both.
+softmax, dropout and context keep and take nothing.  A block's residual addition is part of the norm behind it, whose row has both.  The
+layer has no dropout: a database of one that has needs its times from elsewhere.
 """
 import argparse
 import csv
@@ -218,9 +220,13 @@ def database(w, graph, measured, base):
     return db
 
 
-def write(db, stem, directory):
-    """The database's operator tables as files that ProfileDB.from_directory reads (profiler/op_profiler.py:461-482)."""
+def write(db, stem, directory, measured=None):
+    """The database's operator tables as files that ProfileDB.from_directory reads (profiler/op_profiler.py:461-482).  `measured`: the
+    (micro-batch, tp) that were, to be listed with the others in a file of their own, <stem>_origin.csv."""
     os.makedirs(directory, exist_ok=True)
+    if measured is not None:
+        with open(os.path.join(directory, f"{stem}_origin.csv"), "w", newline="") as f:
+            csv.writer(f).writerows([["mbs", "tp", "origin"]] + [[b, tp, "measured" if (b, tp) in measured else "synthetic"] for b in db.mbs_list for tp in db.tp_list])
     for mi, mbs in enumerate(db.mbs_list):
         for ti, tp in enumerate(db.tp_list):
             for algo in range(db.n_algo):
@@ -264,12 +270,13 @@ def main(argv=None):
     result = {"workload": w.name, "ops": graph.num_ops, "window": args.window, "sinks": args.sinks, "measured": len(measured)}
     (b, tp), rows = next(iter(measured.items()))
     result["forward_backward_us"] = {f"micro-batch {b}, tp {tp}": {n: [round(t, 1) for t in row[:2]] for n, row in rows.items()}}
+    result["synthetic"] = [[b, tp] for b in base.mbs_list for tp in base.tp_list if (b, tp) not in measured]
     if args.out:
-        write(db, f"{w.model_name}_{w.name}", args.out)
+        write(db, f"{w.model_name}_{w.name}", args.out, measured)
     for bits, kind in ((32, CostModelSettings), (8, EightBitSettings)):
         cm = CostModel(kind(**dataclasses.asdict(synth.make_settings(w))), db, graph)
         ms, mb, feasible = cm.score_batch(synth.make_plans(w, cm.tables, n_plans=args.plans))
-        best = np.where(feasible > 0, ms, np.inf)
+        best = np.where((feasible > 0) & (not result["synthetic"]), ms, np.inf)
         result[f"plans_with_{bits}_bit_moments"] = {"scored": len(ms), "feasible": int((feasible > 0).sum()),
                                                     "best_ms": float(best.min()) if np.isfinite(best.min()) else None, "median_peak_mb": float(np.nanmedian(mb))}
         cm.close()

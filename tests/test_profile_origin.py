@@ -1,4 +1,6 @@
-"""What a measured profile database says of itself: times of the card and not of the host, and reserved memory."""
+"""What a measured profile database says of itself: times of the card and not of the host, reserved memory, and which rows were measured."""
+import csv
+import json
 import time
 
 import numpy as np
@@ -23,6 +25,15 @@ def test_reserved_memory_is_what_was_measured():
     base, db = database((1.0, 2.0))      # times only: nothing is known of the rest
     for f in ("reserved_fwd", "reserved_bwd"):
         assert base.tables[f].any() and np.array_equal(db.tables[f], base.tables[f])
+
+
+def test_files_say_which_of_them_were_measured(tmp_path):
+    _, db = database((1.0, 2.0, 0.0, 0.0))
+    profile_layer.write(db, "gpt_x", str(tmp_path), {(2, 4): None})
+    with open(tmp_path / "gpt_x_origin.csv") as f:
+        rows = list(csv.reader(f))
+    assert rows[0] == ["mbs", "tp", "origin"] and len(rows) == 1 + len(db.mbs_list) * len(db.tp_list)
+    assert [r[:2] for r in rows if r[2] == "measured"] == [["2", "4"]]
 
 
 @gpu
@@ -57,3 +68,14 @@ def test_reserved_memory_is_what_a_call_gives_back():
     assert profile_layer._reserved_mb(call) == 96.0
     assert profile_layer._reserved_mb(call, left=40.0) == 120.0
     assert profile_layer._reserved_mb(lambda: mb(32)) == 0.0
+
+
+@gpu
+def test_a_partly_measured_database_has_no_best_plan(capsys, tmp_path):
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    profile_layer.main(["--workload", "gpt3_1_3b", "--micro-batches", "2", "--tp", "4", "--reps", "2", "--plans", "256", "--out", str(tmp_path)])
+    r = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert len(r["synthetic"]) == 14 and [2, 4] not in r["synthetic"]
+    assert all(r[f"plans_with_{bits}_bit_moments"]["best_ms"] is None for bits in (8, 32))
+    assert sum("measured" in line for line in open(tmp_path / "gpt_gpt3_1_3b_origin.csv")) == 1
