@@ -1156,19 +1156,22 @@ bool few(const ace_attend_t *a) {
     return split < whole;
 }
 
-template <class K> int with_lds(K kernel, int bytes) { return layer_hip_status(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)); }
+template <auto KERNEL> int with_lds(int bytes) {
+    static std::atomic<uint64_t> done;
+    return layer_allow_lds((const void *)KERNEL, bytes, done);
+}
 
 template <class T, int DP> int forward(Args &k, const ace_attend_t *a, hipStream_t stream) {
     constexpr int PITCH = Shape<DP>::PITCH;
     if (!few(a)) {
         constexpr int LDS = 4 * KEYS * PITCH * 2;
-        static const int ready = with_lds(attend_forward<T, DP>, LDS);
+        const int ready = with_lds<attend_forward<T, DP>>(LDS);
         if (ready != ACE_OK) return ready;
         attend_forward<T, DP><<<places((int64_t)k.batch * k.heads * ((k.queries + QUERIES - 1) / QUERIES)), LANES, LDS, stream>>>(k);
         return layer_launched();
     }
     constexpr int TILES = WAVES * 4 * SPLIT_KEYS * PITCH * 2, JOIN = (WAVES * DP * 32 + WAVES * 2 * 32) * 4, LDS = TILES > JOIN ? TILES : JOIN;
-    static const int ready = with_lds(attend_split<T, DP>, LDS);
+    const int ready = with_lds<attend_split<T, DP>>(LDS);
     if (ready != ACE_OK) return ready;
     attend_split<T, DP><<<dim3(k.splits, k.kv_heads * k.row_blocks, k.batch), LANES, LDS, stream>>>(k);
     int rc = layer_launched();
@@ -1202,7 +1205,7 @@ int64_t delta_floats(const ace_attend_t *a) { return ((int64_t)a->batch * a->hea
 template <class T, int DP, int SHARE> int key_grads(const Args &k, hipStream_t stream) {
     constexpr int LDS = 2 * QueryTiles<T, Shape<DP>::PITCH, query_rows(SHARE), LANES>::STAGE, OWN = QUERIES / SHARE;
     static_assert(LDS >= (WAVES - WAVES / SHARE) * DP * 32 * 4, "the wavefronts' sums");
-    static const int ready = with_lds(attend_dkv<T, DP, SHARE>, LDS);
+    const int ready = with_lds<attend_dkv<T, DP, SHARE>>(LDS);
     if (ready != ACE_OK) return ready;
     attend_dkv<T, DP, SHARE><<<places((int64_t)k.batch * k.kv_heads * ((k.keys + OWN - 1) / OWN)), LANES, LDS, stream>>>(k);
     return layer_launched();
@@ -1211,7 +1214,7 @@ template <class T, int DP, int SHARE> int key_grads(const Args &k, hipStream_t s
 template <class T, int DP> int backward(const Args &k, hipStream_t stream) {
     constexpr int PITCH = Shape<DP>::PITCH, DQ = 4 * KEYS * PITCH * 2;
     constexpr int FAR_TILES = WAVES * 2 * QueryTiles<T, PITCH, 32, 64>::STAGE, FAR_JOIN = WAVES * DP * 32 * 4, FAR = FAR_TILES > FAR_JOIN ? FAR_TILES : FAR_JOIN;
-    static const int ready = with_lds(attend_dq<T, DP>, DQ), ready2 = with_lds(attend_far<T, DP>, FAR);
+    const int ready = with_lds<attend_dq<T, DP>>(DQ), ready2 = with_lds<attend_far<T, DP>>(FAR);
     if (ready != ACE_OK || ready2 != ACE_OK) return ACE_EHIP;
     int rc = ACE_OK;
     if (k.queries > 0) {

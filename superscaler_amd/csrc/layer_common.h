@@ -6,10 +6,15 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
+#include <atomic>
 #include "ace_layer.h"
 
 /* (in layer_norm.hip) remembers a HIP error for ace_layer_last_hip_error; ACE_OK or ACE_EHIP */
 int layer_hip_status(hipError_t e);
+
+/* (in layer_norm.hip) lets a kernel have `bytes` of LDS on the current device: asked for once per device, whose bits `done` keeps, and
+ * again after a failure */
+int layer_allow_lds(const void *kernel, int bytes, std::atomic<uint64_t> &done);
 
 static inline int layer_launched() { return layer_hip_status(hipGetLastError()); }
 

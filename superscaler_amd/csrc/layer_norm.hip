@@ -121,7 +121,8 @@ int64_t grid_of(const NormShape &shape, int64_t rows, int lds) {
 
 template <class T, int CAP, int NV, bool EVEN, bool HAS_F, bool ENTRY> int launch(const NormArgs &a, const NormShape &shape, hipStream_t stream) {
     const auto kernel = norm_forward<T, CAP, NV, EVEN, HAS_F, ENTRY>;
-    static const int ready = norm_params_in_lds<NV>() ? layer_hip_status(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 155 * 1024)) : ACE_OK;
+    static std::atomic<uint64_t> done;
+    const int ready = norm_params_in_lds<NV>() ? layer_allow_lds((const void *)kernel, 155 * 1024, done) : ACE_OK;
     if (ready != ACE_OK) return ready;
     const int room = norm_params_in_lds<NV>() ? PARAMS * norm_pitch(shape) * (int)sizeof(T) : 0;
     kernel<<<(uint32_t)grid_of(shape, a.rows, room), shape.lanes, room, stream>>>(a);
@@ -182,6 +183,17 @@ int layer_hip_status(hipError_t e) {
     if (e == hipSuccess) return ACE_OK;
     last_error = e;
     return ACE_EHIP;
+}
+
+int layer_allow_lds(const void *kernel, int bytes, std::atomic<uint64_t> &done) {
+    int device = 0;
+    const int rc = layer_hip_status(hipGetDevice(&device));
+    if (rc != ACE_OK) return rc;
+    const uint64_t bit = device >= 0 && device < 64 ? (uint64_t)1 << device : 0;
+    if (done.load(std::memory_order_acquire) & bit) return ACE_OK;
+    if (layer_hip_status(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) != ACE_OK) return ACE_EHIP;
+    done.fetch_or(bit, std::memory_order_release);
+    return ACE_OK;
 }
 
 extern "C" int ace_layer_abi_version(void) { return ACE_LAYER_ABI_VERSION; }

@@ -237,7 +237,8 @@ template <class T> __global__ void __launch_bounds__(COLS * SHARES) norm_join(co
 
 template <class T, int CAP, int NV, bool EVEN, bool HAS_F, bool ENTRY> int launch(const NormArgs &a, const NormShape &shape, hipStream_t stream) {
     const auto kernel = norm_backward<T, CAP, NV, EVEN, HAS_F, ENTRY>;
-    static const int ready = norm_params_in_lds<NV>() ? layer_hip_status(hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 155 * 1024)) : ACE_OK;
+    static std::atomic<uint64_t> done;
+    const int ready = norm_params_in_lds<NV>() ? layer_allow_lds((const void *)kernel, 155 * 1024, done) : ACE_OK;
     if (ready != ACE_OK) return ready;
     kernel<<<(uint32_t)a.runs, shape.lanes, norm_params_in_lds<NV>() ? norm_pitch(shape) * (PARAMS * (int)sizeof(T) + (NV == 2 ? 4 : 0)) : 0, stream>>>(a);
     return layer_launched();
