@@ -344,8 +344,8 @@ class AdamW:
     where it is zero.  A block with a value that is not finite comes back as NaN.
 
     `state`: the moments, as flat tensors ("m", "v", and with 8 bits "m_scale", "v_scale"), to be saved and restored with copy_;
-    tensor i's elements begin at `offsets[i]`, a multiple of 256.  The tensors' memory is taken down here: a parameter or copy that
-    is to move needs a new AdamW."""
+    tensor i's elements begin at `offsets[i]`, a multiple of 256.  The tensors' memory is taken down here: a step with a parameter or copy that
+    has moved since raises ValueError, and needs a new AdamW."""
 
     def __init__(self, params, *, copies=None, state_bits=32):
         params = list(params)
@@ -390,6 +390,7 @@ class AdamW:
             for name in ("m_scale", "v_scale"):
                 self.state[name] = torch.zeros(self.size // ADAMW_BLOCK, dtype=torch.float32, device=self.device)
         self._shapes = [p.shape for p in params]
+        self._places = table[:, 0].tolist(), table[:, 1].tolist()
         self._args = _AdamW(self._tensors.data_ptr(), self._chunk_tensor.data_ptr(), len(params), int(self._first_chunks[-1]), state_bits, 0,
                             _NONE if self.copy_type is None else _TYPES[self.copy_type])
 
@@ -421,6 +422,10 @@ class AdamW:
             if g.shape != shape or g.device != device or not g.is_contiguous():
                 raise ValueError(f"grads[{i}]: a contiguous tensor {tuple(shape)} on {device} expected, got {tuple(g.shape)} on {g.device}")
             pointers[i] = g.data_ptr()
+        for what, held, places in (("params", self.params, self._places[0]), ("copies", self.copies if self.copy_type else (), self._places[1])):
+            for i, (t, at) in enumerate(zip(held, places)):
+                if t.data_ptr() != at:
+                    raise ValueError(f"{what}[{i}] has moved: its memory is not the one that this AdamW was made with")
         if grad_scale is not None:
             _on_gpu(grad_scale, "grad_scale")
             if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != device:
