@@ -62,8 +62,8 @@ int ace_block_norm_backward(const ace_block_norm_t *a, const void *g_residual, c
  * Query i of sequence b stands at position p = start[b] + i and sees key j where
  *     j < length[b], j <= p and (p - j < window or j < sinks).
  * out = softmax(scale q k^T) v over the keys it sees, lse = log sum exp of the scaled products; a query that sees none has
- * out = 0 and lse = -inf.  Keys at or past length[b] are not read.  Up to 2^28 queries and keys; a start past 2^30 is taken as 2^30.
- * Backward with first keys: up to 65,535 sequences, and kv_heads times the blocks of 32 first keys up to 65,535. */
+ * out = 0 and lse = -inf.  Keys at or past length[b] are not read.  Up to 2^28 queries and keys, and up to 2^22 of batch * heads *
+ * (ceil(queries / 128) + 1) and of batch * kv_heads * (ceil(keys / 128) + 1); a start past 2^30 is taken as 2^30. */
 typedef struct ace_attend {
     int32_t batch, queries, keys, heads, kv_heads, dim;   /* heads a multiple of kv_heads; dim a multiple of 8 up to 128 */
     int32_t dtype;                                        /* ACE_T_BF16 or ACE_T_F16 */

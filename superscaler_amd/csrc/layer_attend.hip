@@ -1049,7 +1049,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_far(c
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH;
     typedef QueryTiles<T, PITCH, 32, 64> Queries;
-    const int part = blockIdx.x, block = blockIdx.y % a.far_blocks, kv = blockIdx.y / a.far_blocks, b = blockIdx.z;
+    /* (in one dimension, which holds what check() lets through: fewer than 2^24 blocks, or 256 workgroups) */
+    const int part = blockIdx.x % a.far_parts, item = blockIdx.x / a.far_parts, block = item % a.far_blocks, kv = item / a.far_blocks % a.kv_heads, b = item / a.far_blocks / a.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Sequence seq = sequence(a, b);
     const int k0 = block * 32, key = k0 + (lane & 31);
@@ -1223,8 +1224,7 @@ template <class T, int DP> int backward(const Args &k, hipStream_t stream) {
     }
     if (k.keys == 0) return ACE_OK;
     if (k.far_parts > 0) {
-        if (k.batch > 65535 || (int64_t)k.kv_heads * k.far_blocks > 65535) return ACE_ETOOBIG;
-        attend_far<T, DP><<<dim3(k.far_parts, k.kv_heads * k.far_blocks, k.batch), LANES, FAR, stream>>>(k);
+        attend_far<T, DP><<<(uint32_t)((int64_t)k.far_parts * k.far_blocks * k.kv_heads * k.batch), LANES, FAR, stream>>>(k);
         if ((rc = layer_launched()) != ACE_OK) return rc;
     }
     const int64_t groups = (int64_t)k.batch * k.kv_heads * ((k.keys + QUERIES - 1) / QUERIES);

@@ -20,7 +20,7 @@ from typing import NamedTuple, Optional
 import numpy as np
 import torch
 
-from .evaluator import AceError
+from .evaluator import ACE_ETOOBIG, AceError
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libace_layer.so")
 _lib = None
@@ -95,6 +95,8 @@ def _call(device, name, *args):
     else:
         rc = getattr(lib, name)(*args, _raw_stream(index))
     if rc != 0:
+        if rc == ACE_ETOOBIG:
+            raise ValueError(f"{name}: {lib.ace_layer_strerror(rc).decode()}")
         hip = lib.ace_layer_last_hip_error().decode() if rc == -3 else ""
         raise AceError(f"{name}: {lib.ace_layer_strerror(rc).decode()}" + (f" ({hip})" if hip else ""))
 
@@ -299,7 +301,8 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, start=None, l
     heads // kv_heads heads share a head of keys.  Query i of sequence b stands at position p = start[b] + i and sees key j where
     j < lengths[b], j <= p and (p - j < window or j < sinks); `start` and `lengths` are int32 [batch], by default
     keys - queries and keys: new queries at the end of a full cache.  `window` None: all earlier keys.  `scale`: 1 / sqrt(size)
-    by default.  A query that sees no key has out 0 and lse -inf.  What stands at or past lengths[b] is not read; a value
+    by default.  A query that sees no key has out 0 and lse -inf.  Up to 2^28 queries and keys, and 2^22 of batch * heads * (blocks of 128
+    queries + 1) and of batch * kv_heads * (blocks of 128 keys + 1).  What stands at or past lengths[b] is not read; a value
     of v below it that is not finite can reach queries that do not see it, where their blocks of 128 see a key of the same 64 (so can,
     in the gradients, one of k, q or d_out)."""
     q, k, v, head, strides, rows = _attend_args(q, k, v, window, sinks, scale, start, lengths)
