@@ -236,7 +236,7 @@ extern "C" int ace_block_norm_backward(const ace_block_norm_t *a, const void *g_
         ((d_dentry_weight || d_dentry_bias) && !a->d_entry_weight))
         return ACE_EINVAL;
     if (!d_stats || !d_workspace || workspace_bytes < ace_block_norm_workspace_bytes(a)) return ACE_EINVAL;
-    if (gates_of(a) > 65533 && d_dgate && !token_gate(a)) return ACE_ETOOBIG;
+    if (gates_of(a) >= (int64_t)65535 * 65535 && d_dgate && !token_gate(a)) return ACE_ETOOBIG;
     NormArgs k = args_of(a);
     k.token_gate = token_gate(a);
     k.runs = runs_of(a), k.run = (a->rows + k.runs - 1) / k.runs;

@@ -183,25 +183,27 @@ template <class T, int CAP, int NV, bool EVEN, bool HAS_F, bool ENTRY> __global_
     }
 }
 
-/* Adds up the partial sums: workgroup y = 0 the entry norm's, y = 1 the exit norm's, y = 2 + g gate g's; 32 columns and 32 shares of
- * the rows each. */
-constexpr int COLS = 32, SHARES = 32;
+/* Adds up the partial sums: workgroup y = 0 the entry norm's, y = 1 the exit norm's, y = 2 + g gate g's (JOINS of them to a layer z of the
+ * grid); 32 columns and 32 shares of the rows each. */
+constexpr int COLS = 32, SHARES = 32, JOINS = 65535;
 
 template <class T> __global__ void __launch_bounds__(COLS * SHARES) norm_join(const NormArgs a) {
     __shared__ float lds[2][SHARES][COLS + 1];
     const int col = threadIdx.x % COLS, share = threadIdx.x / COLS, C = a.width;
+    const int64_t what = (int64_t)blockIdx.z * JOINS + blockIdx.y;
+    if (what >= 2 + (a.dgate && !a.token_gate ? a.gates : 0)) return;
     const int64_t c = (int64_t)blockIdx.x * COLS + col;
     float s[2] = {0.0f, 0.0f};
     const bool grouped = a.gate && !a.token_gate && a.gates > 1;
     if (c < C) {
-        if (blockIdx.y == 0) {
+        if (what == 0) {
 #pragma unroll 4
             for (int64_t w = share; a.sum_w1 && w < a.runs; w += SHARES) s[0] += a.sum_w1[w * C + c], s[1] += a.sum_b1[w * C + c];
-        } else if (blockIdx.y == 1 && !grouped) {
+        } else if (what == 1 && !grouped) {
             const float by = a.gate && !a.token_gate ? (float)((const T *)a.gate)[c] : 1.0f;
 #pragma unroll 4
             for (int64_t w = share; a.sum_a && w < a.runs; w += SHARES) s[0] += by * a.sum_a[w * C + c], s[1] += by * a.sum_b[w * C + c];
-        } else if (blockIdx.y == 1) {
+        } else if (what == 1) {
             for (int64_t w = share; a.sum_a && w < a.runs; w += SHARES) {
                 const int64_t last = (w + 1) * a.run < a.rows ? (w + 1) * a.run - 1 : a.rows - 1;
                 const int64_t g1 = last / a.rows_per_gate;
@@ -211,7 +213,7 @@ template <class T> __global__ void __launch_bounds__(COLS * SHARES) norm_join(co
                 }
             }
         } else {
-            const int64_t g = blockIdx.y - 2;
+            const int64_t g = what - 2;
             const int64_t end = (g + 1) * a.rows_per_gate < a.rows ? (g + 1) * a.rows_per_gate : a.rows;
             const int64_t w1 = (end - 1) / a.run;
             for (int64_t w = g * a.rows_per_gate / a.run + share; w <= w1; w += SHARES) s[0] += a.sum_a[(w + g) * C + c], s[1] += a.sum_b[(w + g) * C + c];
@@ -223,15 +225,15 @@ template <class T> __global__ void __launch_bounds__(COLS * SHARES) norm_join(co
     float total = 0.0f;
 #pragma unroll
     for (int k = 0; k < SHARES; ++k) total += lds[share][k][col];
-    if (blockIdx.y < 2) {
-        void *to = blockIdx.y == 0 ? (share == 0 ? a.dw1 : a.db1) : share == 0 ? a.dw2 : a.db2;
+    if (what < 2) {
+        void *to = what == 0 ? (share == 0 ? a.dw1 : a.db1) : share == 0 ? a.dw2 : a.db2;
         if (to) ((T *)to)[c] = (T)total;
     } else if (share == 0) {
         float b = 0.0f;
 #pragma unroll
         for (int k = 0; k < SHARES; ++k) b += lds[1][k][col];
         const float w2 = a.w2 ? (float)((const T *)a.w2)[c] : 1.0f, b2 = a.b2 ? (float)((const T *)a.b2)[c] : 0.0f;
-        ((T *)a.dgate)[(blockIdx.y - 2) * (int64_t)C + c] = (T)(total * w2 + b * b2);
+        ((T *)a.dgate)[(what - 2) * C + c] = (T)(total * w2 + b * b2);
     }
 }
 
@@ -255,8 +257,8 @@ template <class T> int backward(const NormArgs &a, hipStream_t stream) {
     NORM_FOR_SHAPE(CALL, false)
 #undef CALL
     if (rc != ACE_OK) return rc;
-    const int gates = a.dgate && !a.token_gate ? (int)a.gates : 0;
-    norm_join<T><<<dim3((a.width + COLS - 1) / COLS, 2 + gates), COLS * SHARES, 0, stream>>>(a);
+    const int64_t joins = 2 + (a.dgate && !a.token_gate ? a.gates : 0);
+    norm_join<T><<<dim3((a.width + COLS - 1) / COLS, joins < JOINS ? (uint32_t)joins : JOINS, (uint32_t)((joins + JOINS - 1) / JOINS)), COLS * SHARES, 0, stream>>>(a);
     return layer_launched();
 }
 

@@ -49,3 +49,28 @@ def test_gradients_of_very_many_sequences():
     whole, halves = both(slice(None)), [both(slice(0, batch // 2)), both(slice(batch // 2, batch))]
     for i, g in enumerate(whole):
         assert torch.equal(g, torch.cat([h[i] for h in halves])) and g.any()
+
+
+@pytest.mark.parametrize("gates", [65533, 65534, 70000, 1 << 24])
+def test_norm_with_very_many_gates(tmp_path, gates):
+    how = dict(rows=2 * gates, width=8, per_gate=2, gate=host.AT)
+    forward, backward = host.run(tmp_path, [host.call(*host.norm_forward(**how)), host.call(*host.norm_backward(**how))])
+    assert forward["rc"] == 0 and backward["rc"] == 0 and backward["launches"] == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gates", [65532, 65533, 65534, 140001])
+def test_gradients_of_very_many_gates(gates):
+    """A gate for every two rows: its gradient is the sum of their two, the same as with a gate for every row."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x, block, d = (torch.randn(gates, 2, 8, device="cuda", generator=gen) for _ in range(3))
+    gate, weight = torch.randn(gates, 8, device="cuda", generator=gen), torch.randn(8, device="cuda", generator=gen)
+    stats = layer.block_norm(x, block, gate=gate, exit_weight=weight).stats
+    got = layer.block_norm_backward(d, None, x, block, stats, gate=gate, exit_weight=weight)
+    rows = layer.block_norm_backward(d, None, x, block, stats, gate=gate[:, None].expand_as(x), exit_weight=weight)
+    assert torch.equal(got.x, rows.x) and torch.equal(got.block, rows.block)
+    # a product and a sum of two terms in another order: a few units of the larger term; the weight's sum of 2 x gates likewise, of their root
+    assert float((got.gate - rows.gate.sum(1)).abs().max()) <= 2.0 ** -21 * float(rows.gate.abs().max())
+    assert torch.allclose(got.exit_weight, rows.exit_weight, rtol=1e-4, atol=2.0 ** -20 * (2 * gates) ** 0.5 * float(gate.abs().max()))
