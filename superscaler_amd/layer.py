@@ -10,6 +10,9 @@ whose state bytes the memory model counts:
 Tensors live on a GPU; work goes to the stream that is current on their device, and nothing waits for it.  A tensor last used on
 another stream is the caller's to order.  Where a row's elements are not adjacent the call works on a contiguous copy.  Other shapes and
 sizes raise ValueError, other types TypeError, a missing library or a HIP failure AceError.  There is no other form behind these calls.
+
+Gradients come from the *_backward calls; torch's automatic differentiation records nothing of these operators.  Where it is on and an
+input requires a gradient, so do the results, and going backward through them raises AceError: no gradient is lost unnoticed.
 """
 import ctypes
 import math
@@ -112,6 +115,31 @@ def _on_gpu(t, what):
         raise ValueError(f"{what} is not on a GPU: these operators run on the HIP kernels only")
 
 
+class _Untracked(torch.autograd.Function):
+    """Results that automatic differentiation cannot go through: the first `n` of the tensors, which depend on the others."""
+    @staticmethod
+    def forward(ctx, name, n, *tensors):
+        ctx.name = name
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise AceError(f"{ctx.name} is not recorded by automatic differentiation: its gradients come from {ctx.name}_backward (call it under torch.no_grad())")
+
+
+def _lost(*inputs):
+    """Whether automatic differentiation would miss a gradient of these."""
+    for t in inputs:
+        if t is not None and t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
+
+
+def _untracked(name, results, inputs):
+    made = iter(_Untracked.apply(name, sum(t is not None for t in results), *(t for t in results + inputs if t is not None)))
+    return [None if t is None else next(made) for t in results]
+
+
 # ---- norms around a block ---------------------------------------------------------------------------------------------------
 class BlockNorm(NamedTuple):
     """`residual`: the new residual stream (`x` itself where no block was given), `normed`: what the next block reads (None
@@ -212,6 +240,9 @@ def block_norm(x, block=None, *, residual_scale=1.0, gate=None, exit_weight=None
     normed = None if entry_weight is None else torch.empty_like(x0)
     stats = x0.new_empty((rows, 4), dtype=torch.float32)
     _call(x0.device, "ace_block_norm_forward", a, None if block is None else residual.data_ptr(), _pointer(normed), stats.data_ptr())
+    if _lost(x, block, gate, exit_weight, exit_bias, entry_weight, entry_bias):
+        made = _untracked("block_norm", (None if block is None else residual, normed, stats), (x, block, gate, exit_weight, exit_bias, entry_weight, entry_bias))
+        return BlockNorm(residual if block is None else made[0], *made[1:])
     return BlockNorm(residual, normed, stats)
 
 
@@ -312,6 +343,8 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, start=None, l
     size = load_library().ace_attend_workspace_bytes(a)
     workspace = q.new_empty(size, dtype=torch.uint8) if size else None
     _call(q.device, "ace_attend_forward", a, _pointer(workspace), size)
+    if _lost(q, k, v):
+        out, lse = _untracked("window_attention", (out, lse), (q, k, v))
     return out, lse
 
 
@@ -438,6 +471,7 @@ class AdamW:
         a.d_m, a.d_v, a.d_m_scale, a.d_v_scale = map(_pointer, self._held())
         _call(device, "ace_adamw_step", ctypes.byref(a), pointers, self._first_chunks.ctypes.data, _pointer(grad_scale), b1, 1 - b1, b2, 1 - b2,
               1 - lr * weight_decay, lr / (1 - b1 ** step), 1 / math.sqrt(1 - b2 ** step), eps)
+        torch.autograd.graph.increment_version(self.params if self.copy_type is None else self.params + self.copies)
 
     def moments(self):
         """(m, v) as flat float32 tensors, elements as in `offsets`: the state itself with 32 bits, with 8 bits new tensors of
