@@ -91,7 +91,7 @@ int ace_attend_backward(const ace_attend_t *a, const void *d_gout, const int64_t
  *     g = grad_scale * grad;  m = m b1 + g (1 - b1);  v = v b2 + g^2 (1 - b2)
  *     p = p decay - m step_size / (sqrt(v) root_scale + eps);  copy = p rounded
  * with decay = 1 - lr * weight_decay, step_size = lr / (1 - b1^t), root_scale = 1 / sqrt(1 - b2^t).
- * Moments of 32 bits: d_m, d_v float.  Of 8 bits: blocks of 256 elements of a tensor, d_m int8 codes of m in steps of max|m| / 127,
+ * Moments of 32 bits: d_m, d_v float.  Of 8 bits: blocks of 256 elements of a tensor, d_m int8 codes of m in steps of max|m| / 127 (1e-30 / 127 at least),
  * d_v uint8 codes of sqrt(v) in steps of its maximum / 255; a code of d_v is 0 only where sqrt(v) is, so no divisor
  * vanishes that was not zero.  A block whose largest value is not finite comes back as NaN as a whole. */
 #define ACE_ADAMW_BLOCK 256

@@ -118,6 +118,9 @@ template <int BITS, class G, class C> __global__ void __launch_bounds__(LANES) a
             }
             const float m_top = __uint_as_float(half_wave_max(m_bits)), u_top = __uint_as_float(half_wave_max(u_bits));
             const bool m_fine = m_top < __builtin_inff(), u_fine = u_top < __builtin_inff();
+            /* (a block whose largest m is below 1e-30, whose reciprocal would pass the range's end, goes in steps of that one's; a root
+             * that is not zero is never so small) */
+            const float m_unit = m_top > 0.0f ? fmaxf(m_top, 1e-30f) : 0.0f;
             const float m_by = m_fine ? 1.0f / fmaxf(m_top, 1e-30f) * 127.0f : 0.0f, u_by = u_fine ? 1.0f / fmaxf(u_top, 1e-30f) * 255.0f : 0.0f;
             vec8<int8_t> mc;
             vec8<uint8_t> vc;
@@ -130,7 +133,7 @@ template <int BITS, class G, class C> __global__ void __launch_bounds__(LANES) a
             store8((int8_t *)a.m + t.state_at + at, mc);
             store8((uint8_t *)a.v + t.state_at + at, vc);
             if ((threadIdx.x & 31) == 0) {
-                a.m_scale[(t.state_at + at) / ACE_ADAMW_BLOCK] = m_fine ? m_top * (float)(1.0 / 127) : __builtin_nanf("");
+                a.m_scale[(t.state_at + at) / ACE_ADAMW_BLOCK] = m_fine ? m_unit * (float)(1.0 / 127) : __builtin_nanf("");
                 a.v_scale[(t.state_at + at) / ACE_ADAMW_BLOCK] = u_fine ? u_top * (float)(1.0 / 255) : __builtin_nanf("");
             }
         }
