@@ -238,6 +238,13 @@ template <class V> __device__ inline void hide(V &s, const Sight &sight, int key
     }
 }
 
+/* Ones where keys key0 + result_row(i) are seen, zeros elsewhere. */
+__device__ inline void show(float (&see)[16], const Sight &sight, int key0, int half) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) see[i] = 1.0f;
+    hide(see, sight, key0, half, true, 0.0f);
+}
+
 /* Work in an order that keeps a head's blocks, which read the same keys, on one of the eight dies and its cache: workgroups go to
  * the dies in turn, so die d gets the d-th eighth of the work.  On a die they go to its 32 CUs in turn: every other 32 are
  * taken in reverse, so that a CU's second workgroup is short where its first is long (blocks at the beginning of a sequence see few
@@ -326,7 +333,7 @@ template <class T, int DP, int PITCH> __device__ inline void block_step(Running<
 
 /* Half precision has five bits of exponent, and gradients of scores go with those of the answer, of any size, and with weights that a
  * long sequence makes small.  So they meet their products with a power of two of the lane's query or key, which moves only when a
- * gradient would pass 2^15 (the largest is 2^8 to 2^9 then: what is 2^22 times smaller still has all its bits) and takes the sums along.
+ * gradient would pass 2^15 (the largest is 2^4 to 2^5 then: what is 2^18 times smaller still has all its bits) and takes the sums along.
  * It begins where no gradient above 2^-49 leaves it.  Normalized weights, 1 at most, meet theirs with 2^12.  The backward pass of 2 x 16
  * heads of 2,048 tokens and size 128, a window of 1,024, takes 164 us with this and 152 without. */
 template <class T> struct Fit {
@@ -342,7 +349,7 @@ template <class T> struct Fit {
         for (int i = 0; i < 16; ++i) most = fmaxf(most, __builtin_fabsf(ds[i]));
         if (!__any(most > 32768.0f)) return 0;
         most = max_halves(most);
-        const int change = most > 32768.0f && most < __builtin_inff() ? 127 + 8 - (int)(__float_as_uint(most) >> 23) : 0;
+        const int change = most > 32768.0f && most < __builtin_inff() ? 127 + 4 - (int)(__float_as_uint(most) >> 23) : 0;
         power += change;
 #pragma unroll
         for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_ldexpf(ds[i], change);
@@ -372,6 +379,112 @@ template <class T> struct Fit {
 template <class T> __device__ inline void store4(T *to, float a, float b, float c, float d) {
     typedef T vec __attribute__((ext_vector_type(4)));
     *(vec *)to = vec{(T)a, (T)b, (T)c, (T)d};
+}
+
+/* A kernel's arguments and a value as if not known so far: what a rare path computes from these is computed there, and not kept in
+ * registers through the loops before it. */
+__device__ inline const Args &args_again() {
+    auto p = (const __attribute__((address_space(4))) Args *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Args *)p;
+}
+__device__ inline int again(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+/* Weights of keys that a query does not see are zero, and zero times a value that is no finite number is none: such a value in a block
+ * of which others see a part spoils sums that it is no part of.  The kernels look at their sums at the end, and a wavefront that
+ * finds one takes its walk once more, with operands from memory: what is not finite meets its products as zero, and counts for those that
+ * see it.  (Looking costs an operation per sum, once.  8 heads of 16,384 tokens, a window of 2,048, forward and backward: 159 and 519 us;
+ * with one value that is no number in the middle 304 and 3,525, with nothing else 1,280 and 7,110.) */
+template <int DT> __device__ inline bool any_odd(const f32x16 (&x)[DT]) {
+    float z[4] = {};
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i % 4] = __builtin_fmaf(x[t][i], 0.0f, z[i % 4]);
+    return !(z[0] + z[1] + z[2] + z[3] == 0.0f);
+}
+/* 32 rows from row0 on of a head's q, k, v or gradient, through a buffer descriptor: what is at or past `end`, and past a row's size, reads zero. */
+template <class T> struct Rows {
+    __amdgpu_buffer_rsrc_t rows;
+    int stride, dim;
+    __device__ inline Rows(const T *base, int64_t s, int row0, int end, int d) : stride((int)s), dim(d) {
+        const int n = end - row0 < 32 ? end - row0 : 32;
+        rows = __builtin_amdgcn_make_buffer_rsrc((void *)(base + row0 * s), 0, n > 0 ? ((n - 1) * stride + dim) * 2 : 0, 0x00027000);
+    }
+    /* the products of the rows and the columns `other` */
+    template <int N> __device__ inline f32x16 times(const typename Mma<T>::frag (&other)[N], int lane) const {
+        int at = (lane & 31) * stride + (lane >> 5) * 8;
+        arrived(at);   /* (places are computed here: kept through a walk, they would take the registers of its sums) */
+        f32x16 acc = {};
+#pragma unroll
+        for (int s = 0; s < N; ++s) {
+            const auto f = __builtin_amdgcn_raw_buffer_load_b128(rows, s * 16 + (lane >> 5) * 8 < dim ? (at + s * 16) * 2 : -1, 0, 0);
+            acc = Mma<T>::go(__builtin_bit_cast(typename Mma<T>::frag, f), other[s], acc);
+        }
+        return acc;
+    }
+    /* element 32 t + lane % 32 of the eight rows result_row(8 k) to result_row(8 k + 7), as `of` makes them */
+    template <class F> __device__ inline typename Mma<T>::frag column(int t, int k, int lane, F of) const {
+        int d = t * 32 + (lane & 31);
+        arrived(d);
+        const int at = (lane >> 5) * 4 * stride + d;
+        typename Mma<T>::frag r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint16_t x = __builtin_amdgcn_raw_buffer_load_b16(rows, d < dim ? (at + result_row(8 * k + e, 0) * stride) * 2 : -1, 0, 0);
+            r[e] = (T)of((float)__builtin_bit_cast(T, x));
+        }
+        return r;
+    }
+};
+/* sum += (the rows, transposed) times `weights`; `sees`: ones for the rows that result_row numbers and the lane's column sees, zeros for others.  SIGNED:
+ * weights are positive, so that an infinite element leaves its sign. */
+template <bool SIGNED, class T, int DT, class Sees> __device__ inline void careful_columns(f32x16 (&sum)[DT], const Rows<T> &rows, const typename Mma<T>::frag (&weights)[2], Sees sees,
+                                                                                           int lane) {
+    const float inf = __builtin_inff();
+    bool some = false;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            sum[t] = Mma<T>::go(rows.column(t, k, lane,
+                                            [&](float x) {
+                                                const bool fine = __builtin_fabsf(x) < inf;
+                                                some = some || !fine;
+                                                return fine ? x : 0.0f;
+                                            }),
+                                weights[k], sum[t]);
+            __builtin_amdgcn_sched_barrier(0);   /* (one operand at a time: these kernels' registers are in use) */
+        }
+    if (!__any(some)) return;
+    float see[16];
+    sees(see);
+    const typename Mma<T>::frag seen[2] = {pack8<T>(see), pack8<T>(see + 8)};
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int sign = 1; sign >= -1; sign -= 2) {
+            f32x16 many = {};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) many = Mma<T>::go(rows.column(t, k, lane, [&](float x) { return !(sign * x < inf) ? 1.0f : 0.0f; }), seen[k], many);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[t][i] += many[i] > 0.0f ? (SIGNED ? sign * inf : __builtin_nanf("")) : 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+}
+/* one block of 32 keys for 32 queries whose weights are taken around `around` */
+template <class T, int DP> __device__ inline void careful_block(f32x16 (&o)[DP / 32], const typename Mma<T>::frag (&qf)[DP / 16], const T *k, const T *v, const Args &a, int length,
+                                                                const Sight &sight, float around, int key0, int lane) {
+    float s[16];
+    const f32x16 acc = Rows<T>(k, a.k_stride[1], key0, length, a.dim).times(qf, lane);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i], a.scale2, -around));
+    hide(s, sight, key0, lane >> 5, key0 < a.sinks, 0.0f);
+    const typename Mma<T>::frag pf[2] = {pack8<T>(s), pack8<T>(s + 8)};
+    careful_columns<true, T>(o, Rows<T>(v, a.v_stride[1], key0, length, a.dim), pf, [&](float (&see)[16]) { show(see, sight, key0, lane >> 5); }, lane);
 }
 
 template <int DP> struct Shape { static constexpr int PITCH = DP <= 64 ? 64 : 128; };
@@ -582,17 +695,32 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(walk.o[t]);
     const float total = sum_halves(walk.total);
-    if (query >= a.queries) return;
     const float by = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total;   /* (nothing visible: zero; not a number: that) */
     T *to = (T *)a.out + b * a.out_stride[0] + (int64_t)query * a.out_stride[1] + head * a.out_stride[2];
+    auto leave = [&] {
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
+        for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = t * 32 + result_row(i, half);
-            if (d < a.dim) store4(to + d, walk.o[t][i] * by, walk.o[t][i + 1] * by, walk.o[t][i + 2] * by, walk.o[t][i + 3] * by);
-        }
-    if (half == 0) a.lse[((int64_t)b * a.heads + head) * a.queries + query] = total == 0.0f ? -__builtin_inff() : walk.top * a.scale + __logf(total);
+            for (int i = 0; i < 16; i += 4) {
+                const int d = t * 32 + result_row(i, half);
+                if (d < a.dim) store4(to + d, walk.o[t][i] * by, walk.o[t][i + 1] * by, walk.o[t][i + 2] * by, walk.o[t][i + 3] * by);
+            }
+    };
+    if (query < a.queries) {
+        leave();
+        if (half == 0) a.lse[((int64_t)b * a.heads + head) * a.queries + query] = total == 0.0f ? -__builtin_inff() : walk.top * a.scale + __logf(total);
+    }
+    const bool odd = query < a.queries && total < __builtin_inff() && any_odd(walk.o);
+    if (__builtin_expect(!__any(odd), 1)) return;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) walk.qf[s] = global_frag<T>(qrow, s * 16 + half * 8, a.dim, query < a.queries);
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) walk.o[t] = f32x16{};
+    for (int t = 0; t < tiles.count; ++t)
+        for (int key0 = tiles.tile(t) * KEYS, n = 0; n < KEYS / 32; ++n, key0 += 32)
+            if (seen.has(key0) || key0 < sinks) careful_block<T, DP>(walk.o, walk.qf, k, v, a, seq.length, sight, walk.around, key0, lane);
+    /* (a query and its sums are with two lanes, of which one may have found nothing) */
+    if (query < a.queries && max_halves(odd ? 1.0f : 0.0f) > 0.0f) leave();
 }
 
 /* Few queries: the queries of a key head's heads are the columns of one block of 32; every wavefront walks over tiles of 32 keys
@@ -647,6 +775,12 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_split
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(run.o[t]);
     run.total = sum_halves(run.total);
+    if (__builtin_expect(__any(row < rows && run.total < __builtin_inff() && any_odd(run.o)), 0)) {
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) run.o[t] = f32x16{};
+        const float around = run.top == -__builtin_inff() ? 0.0f : run.top * a.scale2;
+        for (int t = worker; t < tiles.count; t += workers) careful_block<T, DP>(run.o, qf, k, v, a, seq.length, sight, around, tiles.tile(t) * SPLIT_KEYS, lane);
+    }
     /* join the wavefronts: element d of a row's sum lies at [wave][d][row] */
     float *sums = (float *)lds, *tops = sums + WAVES * DP * 32;
     __syncthreads();
@@ -775,16 +909,8 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
     float sum = 0.0f;
     Fit<T> fit;
     fit.start();
-    for (int walk = few ? 0 : 1; walk < 2; ++walk) {
-        if (walk == 1) {
-            if (few) delta = sum_halves(sum);
-            lse2 -= (float)fit.power;   /* (weights of the first walk are as they are; here their exponent is rounded to 2^-18) */
-            if (there && half == 0) a.delta[flat] = delta;
-        }
-        if (few && walk == 1) {
-            meet();   /* (every wavefront is through with the first walk's last tile) */
-            if (tiles.count > 0) ask(0);
-        }
+    auto walk = [&](auto number) {
+        constexpr int WALK = decltype(number)::value;
         for (int t = 0; t < tiles.count; ++t) {
             wait_tiles<0>();
             meet();
@@ -807,11 +933,11 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
                 in_step<DP / 8, 1, 4>();
                 __builtin_amdgcn_s_setprio(0);
                 float ds[16];
-                const float less = walk == 0 ? 0.0f : delta;
+                const float less = WALK == 0 ? 0.0f : delta;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse2)) * (dp[i] - less);
                 if (!clear.has(key0)) hide(ds, sight, key0, half, key0 < a.sinks, 0.0f);
-                if (walk == 0) {
+                if constexpr (WALK == 0) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sum += ds[i];
                     continue;
@@ -828,10 +954,55 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP)
                 __builtin_amdgcn_s_setprio(0);
             }
         }
+    };
+    if (few) {
+        walk(Number<0>());
+        delta = sum_halves(sum);
+        meet();   /* (every wavefront is through with the first walk's last tile) */
+        if (tiles.count > 0) ask(0);
     }
+    lse2 -= (float)fit.power;   /* (weights of the first walk are as they are; here their exponent is rounded to 2^-18) */
+    if (there && half == 0) a.delta[flat] = delta;
+    walk(Number<1>());
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(dq[t]);
     fit.undo(dq, fit.power);
+    if (__builtin_expect(__any(there && any_odd(dq)), 0)) {
+        const Args &r = args_again();
+        const int work = __builtin_amdgcn_readfirstlane(again(place(r.batch * r.heads * ((r.queries + QUERIES - 1) / QUERIES)))), blocks = (r.queries + QUERIES - 1) / QUERIES;
+        const int head = work / blocks % r.heads, b = work / blocks / r.heads, q0 = (blocks - 1 - work % blocks) * QUERIES, lane = again(threadIdx.x) & 63;
+        const int mine = q0 + __builtin_amdgcn_readfirstlane(again(threadIdx.x) >> 6) * 32, query = mine + (lane & 31), half = lane >> 5;
+        const Sequence seq = sequence(r, b);
+        const bool there = query < r.queries;
+        const T *k = (const T *)r.k + b * r.k_stride[0] + head / r.shared * r.k_stride[2], *v = (const T *)r.v + b * r.v_stride[0] + head / r.shared * r.v_stride[2];
+        const T *qrow = (const T *)r.q + b * r.q_stride[0] + (int64_t)query * r.q_stride[1] + head * r.q_stride[2];
+        const T *grow = (const T *)r.g + b * r.g_stride[0] + (int64_t)query * r.g_stride[1] + head * r.g_stride[2];
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) qf[s] = global_frag<T>(qrow, s * 16 + half * 8, r.dim, there), gf[s] = global_frag<T>(grow, s * 16 + half * 8, r.dim, there);
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) dq[t] = f32x16{};
+        fit.start();
+        const int64_t flat = ((int64_t)b * r.heads + head) * r.queries + query;
+        lse2 = (there ? r.lse[flat] * LOG2E : 0.0f) - (float)fit.power;
+        const Sight sight(r, seq.length, seq.start + query);
+        const Tiles tiles = tiles_of<KEYS>(r, seq, seq.start + q0, seq.start + lesser(q0 + QUERIES, r.queries) - 1);
+        const Range seen = any_see(r, seq.length, seq.start + mine, seq.start + lesser(mine + 32, r.queries) - 1);
+        const int first = r.window > 0 ? r.sinks : 0;
+        for (int t = 0; t < tiles.count; ++t)
+            for (int key0 = tiles.tile(t) * KEYS, n = 0; n < KEYS / 32; ++n, key0 += 32) {
+                if (!seen.has(key0) && key0 >= first) continue;
+                const Rows<T> krows(k, r.k_stride[1], key0, seq.length, r.dim);
+                const f32x16 s = krows.times(qf, lane), dp = Rows<T>(v, r.v_stride[1], key0, seq.length, r.dim).times(gf, lane);
+                float ds[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], r.scale2, -lse2)) * (dp[i] - delta);
+                hide(ds, sight, key0, half, key0 < r.sinks, 0.0f);
+                lse2 -= (float)fit.check(ds, dq);
+                const typename Mma<T>::frag df[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
+                careful_columns<false, T>(dq, krows, df, [&](float (&see)[16]) { show(see, sight, key0, half); }, lane);
+            }
+        fit.undo(dq, fit.power);
+    }
     if (!there) return;
     T *to = (T *)a.dq + (((int64_t)b * a.queries + query) * a.heads + head) * a.dim;
 #pragma unroll
@@ -855,6 +1026,9 @@ template <class T, int DP> struct KeyGrads {
         for (int s = 0; s < DP / 16; ++s) kf[s] = global_frag<T>(krow, s * 16 + half * 8, dim, there), vf[s] = global_frag<T>(vrow, s * 16 + half * 8, dim, there);
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) arrived(kf[s]), arrived(vf[s]);
+        clear();
+    }
+    __device__ inline void clear() {
 #pragma unroll
         for (int t = 0; t < DP / 32; ++t) dk[t] = f32x16{}, dv[t] = f32x16{};
         fit.start();
@@ -905,6 +1079,38 @@ template <class T, int DP> struct KeyGrads {
         in_step<DP / 8, 2, 2>();
         __builtin_amdgcn_s_setprio(0);
     }
+    /* the same with a head's queries from row0 on and what is not finite among them counted for those that see it only */
+    __device__ inline void careful_step(const Args &a, int b, int head, int row0, int t, uint32_t count, int lane) {
+        const int half = lane >> 5;
+        const int64_t flat = ((int64_t)b * a.heads + head) * a.queries + row0;
+        const Rows<T> q((const T *)a.q + b * a.q_stride[0] + head * a.q_stride[2], a.q_stride[1], row0, a.queries, a.dim);
+        const Rows<T> g((const T *)a.g + b * a.g_stride[0] + head * a.g_stride[2], a.g_stride[1], row0, a.queries, a.dim);
+        auto sees = [&](int i) { return row0 + result_row(i, half) < a.queries && (uint32_t)(t + result_row(i, half)) < count; };
+        float prob[16], ds[16];
+        const f32x16 s = q.times(kf, lane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            prob[i] = 0.0f;
+            if (sees(i)) prob[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, __builtin_fmaf(a.lse[flat + result_row(i, half)], -LOG2E, (float)Fit<T>::WEIGHTS)));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const f32x16 dp = g.times(vf, lane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            ds[i] = 0.0f;
+            if (sees(i)) ds[i] = prob[i] * (dp[i] - a.delta[flat + result_row(i, half)]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        fit.apply(ds, dk);
+        const typename Mma<T>::frag pf[2] = {pack8<T>(prob), pack8<T>(prob + 8)}, df[2] = {pack8<T>(ds), pack8<T>(ds + 8)};
+        auto show = [&](float (&see)[16]) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) see[i] = sees(i) ? 1.0f : 0.0f;
+        };
+        careful_columns<true, T>(dv, g, pf, show, lane);
+        careful_columns<false, T>(dk, q, df, show, lane);
+    }
+    __device__ inline bool odd() const { return any_odd(dk) || any_odd(dv); }
 };
 
 /* Tiles of queries: rows of q and of the answer's gradient, then log-sums and deltas, by LANES lanes. */
@@ -937,27 +1143,46 @@ template <class T, int PITCH, int ROWS, int LANES> struct QueryTiles {
  * 1,024: 79 us, 654 TFLOP/s of the pairs that are seen, the matrix units at work a third of the time: all 256 registers of a wavefront are
  * in use, and the four products of a block of 32 x 32 wait for each other. */
 constexpr int query_rows(int share) { return share == 4 ? 128 : 64; }
+/* a wavefront's keys, of a workgroup's from k0 on, and the queries that see them */
+template <int SHARE> struct WaveKeys {
+    static constexpr int OWN = QUERIES / SHARE, OWNERS = WAVES / SHARE, ROWS = query_rows(SHARE);
+    Sequence seq;
+    int mine, key, first, per_head;   /* in tiles of ROWS: the first that the workgroup walks over, and how many of each head */
+    uint32_t sight;                   /* how many queries see this lane's key: from its own position on, for a window's length, those that there are */
+    Range seen, clear;                /* where a block of 32 queries begins of which any sees one of the wavefront's keys, and one of which all see all */
+    __device__ inline WaveKeys(const Args &a, Sequence s, int k0, int wave, int lane) : seq(s), mine(k0 + wave % OWNERS * 32), key(mine + (lane & 31)), seen(0, 0), clear(0, 0) {
+        /* queries from the first key's position on, up to the last key's window */
+        int from = k0 - seq.start, to = a.queries;
+        if (a.window > 0) {
+            const int64_t most = (int64_t)k0 + OWN - 1 + a.window - seq.start;
+            to = most < to ? (int)most : to;
+        }
+        from = from < 0 ? 0 : from;
+        first = from / ROWS, per_head = k0 < seq.length && to > from ? (to + ROWS - 1) / ROWS - first : 0;
+        const int64_t left = (int64_t)seq.start + a.queries - key;
+        sight = key >= seq.length || left <= 0 ? 0 : a.window > 0 && a.window < left ? a.window : (uint32_t)left;
+        const int begin = mine - seq.start;
+        seen = Range(begin - 31, mine < seq.length ? a.window > 0 ? lesser(begin + 31 + a.window, a.queries) : a.queries : begin - 31);
+        clear = Range(begin + 31, mine + 32 <= seq.length ? a.window > 0 ? lesser(begin - 31 + a.window, a.queries - 31) : a.queries - 31 : begin);
+    }
+};
 template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_dkv(const Args a) {
     extern __shared__ char lds[];
-    constexpr int PITCH = Shape<DP>::PITCH, OWN = QUERIES / SHARE, OWNERS = WAVES / SHARE, ROWS = query_rows(SHARE);
+    typedef WaveKeys<SHARE> Mine;
+    constexpr int PITCH = Shape<DP>::PITCH, OWN = Mine::OWN, OWNERS = Mine::OWNERS, ROWS = Mine::ROWS;
     typedef QueryTiles<T, PITCH, ROWS, LANES> Queries;
     const int blocks = (a.keys + OWN - 1) / OWN, count = a.batch * a.kv_heads * blocks;
     const int work = place(count);
     if (work >= count) return;
     const int block = work % blocks, kv = work / blocks % a.kv_heads, b = work / blocks / a.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const Sequence seq = sequence(a, b);
-    const int k0 = block * OWN, mine = k0 + wave % OWNERS * 32, key = mine + (lane & 31);
+    const Mine m(a, sequence(a, b), block * OWN, wave, lane);
+    const Sequence seq = m.seq;
+    const int mine = m.mine, key = m.key, first = m.first, per_head = m.per_head, steps = per_head * a.shared;
+    const uint32_t sight = m.sight;
+    const Range seen = m.seen, clear = m.clear;
     const T *krow = (const T *)a.k + b * a.k_stride[0] + (int64_t)key * a.k_stride[1] + kv * a.k_stride[2];
     const T *vrow = (const T *)a.v + b * a.v_stride[0] + (int64_t)key * a.v_stride[1] + kv * a.v_stride[2];
-    /* queries from the first key's position on, up to the last key's window */
-    int from = k0 - seq.start, to = a.queries;
-    if (a.window > 0) {
-        const int64_t most = (int64_t)k0 + OWN - 1 + a.window - seq.start;
-        to = most < to ? (int)most : to;
-    }
-    from = from < 0 ? 0 : from;
-    const int first = from / ROWS, per_head = k0 < seq.length && to > from ? (to + ROWS - 1) / ROWS - first : 0, steps = per_head * a.shared;
     const uint32_t lds0 = lds_offset(lds);
     const Operands<T, PITCH> ops(lane);
     const Queries queries(a, b, threadIdx.x);
@@ -968,13 +1193,6 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
     };
     KeyGrads<T, DP> grads;
     grads.start(krow, vrow, a.dim, key < seq.length, half);
-    /* this lane's key is seen from its own position on, for a window's length, by queries that there are */
-    const int64_t left = (int64_t)seq.start + a.queries - key;
-    const uint32_t sight = key >= seq.length || left <= 0 ? 0 : a.window > 0 && a.window < left ? a.window : (uint32_t)left;
-    /* where a block of 32 queries begins of which any sees one of the wavefront's keys, and one of which all see all */
-    const int begin = mine - seq.start;
-    const Range seen(begin - 31, mine < seq.length ? a.window > 0 ? lesser(begin + 31 + a.window, a.queries) : a.queries : begin - 31);
-    const Range clear(begin + 31, mine + 32 <= seq.length ? a.window > 0 ? lesser(begin - 31 + a.window, a.queries - 31) : a.queries - 31 : begin);
     if (steps > 0) ask(0);
     int q = first * ROWS;
     for (int t = 0; t < steps; ++t) {
@@ -995,6 +1213,20 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
         q = q + ROWS < (first + per_head) * ROWS ? q + ROWS : first * ROWS;
     }
     grads.stop();
+    if (__builtin_expect(__any(key < a.keys && grads.odd()), 0)) {
+        const Args &r = args_again();
+        const int blocks = (r.keys + OWN - 1) / OWN, work = __builtin_amdgcn_readfirstlane(again(place(r.batch * r.kv_heads * blocks)));
+        const int kv = work / blocks % r.kv_heads, b = work / blocks / r.kv_heads, lane = again(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(again(threadIdx.x) >> 6);
+        const Mine m(r, sequence(r, b), work % blocks * OWN, wave, lane);
+        grads.start((const T *)r.k + b * r.k_stride[0] + (int64_t)m.key * r.k_stride[1] + kv * r.k_stride[2],
+                    (const T *)r.v + b * r.v_stride[0] + (int64_t)m.key * r.v_stride[1] + kv * r.v_stride[2], r.dim, m.key < m.seq.length, lane >> 5);
+        for (int t = 0; t < m.per_head * r.shared; ++t)
+            for (int n = SHARE > 1 ? wave / OWNERS : 0; n < (SHARE > 1 ? wave / OWNERS + 1 : ROWS / 32); ++n) {
+                const int q0 = (m.first + t % m.per_head) * ROWS + n * 32;
+                if (m.seen.has(q0)) grads.careful_step(r, b, kv * r.shared + t / m.per_head, q0, m.seq.start + q0 - m.key, m.sight, lane);
+            }
+        grads.stop();
+    }
     if (SHARE > 1) {
         /* the other wavefronts' sums go to those of the first one or two, in order, dK and then dV */
         float *sums = (float *)lds + (lane & 31);
@@ -1045,7 +1277,7 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
  * over the queries.  A wavefront walks over tiles of 32 queries with buffers of its own; a workgroup's sums, element d of key j at
  * [dk, dv][d][j], are one part, and attend_dkv adds the parts in order.  4 first keys of 2 x 16 heads, 1,024 queries beyond their window: 12 us,
  * two or three tiles for each wavefront, from launch to end a chain of loads, one tile and the sums. */
-template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_far(const Args a) {
+template <class T, int DP> __global__ void __launch_bounds__(LANES) __attribute__((amdgpu_waves_per_eu((DP) <= 64 ? 2 : 1))) attend_far(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH;
     typedef QueryTiles<T, PITCH, 32, 64> Queries;
@@ -1082,6 +1314,14 @@ template <class T, int DP> __global__ void __launch_bounds__(LANES) attend_far(c
         grads.step(ops, qtile, qtile + Queries::BYTES, lse, lse + Queries::ROW_VALUES, a.scale2, seq.start + (first + i % per_head) * 32 - key - a.window, sight, true, half);
     }
     grads.stop();
+    if (__builtin_expect(__any(grads.odd()), 0)) {
+        grads.clear();
+        for (int i = worker; i < items; i += workers) {
+            const int q0 = (first + i % per_head) * 32;
+            grads.careful_step(a, b, kv * a.shared + i / per_head, q0, seq.start + q0 - key - a.window, sight, lane);
+        }
+        grads.stop();
+    }
     float *sums = (float *)lds;
     constexpr int HALF = DP * 32;
     float *to = a.far + ((((int64_t)b * a.kv_heads + kv) * a.far_blocks + block) * a.far_parts + part) * (2 * HALF);

@@ -333,9 +333,9 @@ def window_attention(q, k, v, *, window=None, sinks=0, scale=None, start=None, l
     j < lengths[b], j <= p and (p - j < window or j < sinks); `start` and `lengths` are int32 [batch], by default
     keys - queries and keys: new queries at the end of a full cache.  `window` None: all earlier keys.  `scale`: 1 / sqrt(size)
     by default.  A query that sees no key has out 0 and lse -inf.  Up to 2^28 queries and keys, and 2^22 of batch * heads * (blocks of 128
-    queries + 1) and of batch * kv_heads * (blocks of 128 keys + 1).  What stands at or past lengths[b] is not read; a value
-    of v below it that is not finite can reach queries that do not see it, where their blocks of 128 see a key of the same 64 (so can,
-    in the gradients, one of k, q or d_out)."""
+    queries + 1) and of batch * kv_heads * (blocks of 128 keys + 1).  What a query does not see, a number or not, does not reach it, nor
+    the gradients of a key one that does not see it (a call that finds what is not finite in its answers looks again and
+    takes up to fifteen times as long)."""
     q, k, v, head, strides, rows = _attend_args(q, k, v, window, sinks, scale, start, lengths)
     out = q.new_empty(q.shape)
     lse = q.new_empty(rows, dtype=torch.float32)
