@@ -194,13 +194,18 @@ def measure(w, micro_batch, tp, window=None, sinks=0, vocab=51200, reps=10, devi
 
 def sizes(w, name, micro_batch, tp):
     """(input, output, weights, activations) MB of a row: those of synth, with attention as one operator that keeps its answer and a
-    log-sum for every query."""
+    log-sum for every query, and norms that take the residual stream and a block's output, and keep the stream, its norm and four
+    statistics of every row."""
     u = micro_batch * w.seq * w.hidden * 2 * MB
+    if "layernorm" in name:
+        return 2 * u, 2 * u, 2 * w.hidden * 2 * MB, 2 * u + micro_batch * w.seq * 16 * MB
     if name == "enc-attention-score":
         lse = micro_batch * (w.hidden // HEAD / tp) * w.seq * 4 * MB
         return 4 * u / tp + u, u / tp + u, 0.0, u / tp + lse
     if name in CONTAINED[:3]:
         return u / tp + u, u / tp + u, 0.0, 0.0
+    if name in CONTAINED:
+        return 2 * u, 2 * u, 0.0, 0.0
     return synth._shape_mb(w, name, micro_batch, tp)
 
 

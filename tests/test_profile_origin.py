@@ -1,4 +1,5 @@
-"""What a measured profile database says of itself: times of the card and not of the host, reserved memory, and which rows were measured."""
+"""What a measured profile database says of itself: times of the card and not of the host, reserved memory, what a layer keeps, and which rows were
+measured."""
 import csv
 import json
 import time
@@ -68,6 +69,23 @@ def test_reserved_memory_is_what_a_call_gives_back():
     assert profile_layer._reserved_mb(call) == 96.0
     assert profile_layer._reserved_mb(call, left=40.0) == 120.0
     assert profile_layer._reserved_mb(lambda: mb(32)) == 0.0
+
+
+@gpu
+@pytest.mark.parametrize("tp", [1, 4])
+def test_rows_keep_what_the_layer_keeps(tp):
+    """The activations of a layer's rows add up to what its forward pass leaves for the backward one and the next layer."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    w = synth.WORKLOADS["gpt3_1_3b"]
+    net = profile_layer.GptLayer(w.hidden, tp, window=256, sinks=4)
+    x, block = (torch.randn(3, w.seq, w.hidden, device="cuda").bfloat16() for _ in range(2))
+    r, out, saved = net.forward(x, block)
+    kept = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in [r, out, *saved.values()] if t is not x and t is not block}
+    rows = {n: profile_layer.sizes(w, n, 3, tp) for n in opgraph.GPT_TYPES if n.startswith("enc-")}
+    assert abs(sum(s[3] for s in rows.values()) - sum(kept.values()) / 2 ** 20) < 1e-6
+    assert rows["enc-1st-layernorm"][2] == sum(net.params[n].nbytes for n in ("norm1", "norm1_bias")) / 2 ** 20
+    assert all(rows[n][3] == 0 for n in profile_layer.CONTAINED)
 
 
 @gpu
