@@ -249,8 +249,8 @@ __device__ inline void show(float (&see)[16], const Sight &sight, int key0, int 
  * the dies in turn, so die d gets the d-th eighth of the work.  On a die they go to its 32 CUs in turn: every other 32 are
  * taken in reverse, so that a CU's second workgroup is short where its first is long (blocks at the beginning of a sequence see few
  * keys).  Returns count where a workgroup has nothing to do.  In launch order, by dies, and with every other 32 in reverse: forward, 4 x 40
- * heads of 2,048 tokens, a window of 512: 164, 140 and 140 us, backward 586, 525 and 517; 8 x 16 heads of 512, backward: 55, 51 and 46;
- * 16 heads on 4 of 8,192, no window, backward: 1,733, 1,339 and 1,380. */
+ * heads of 2,048 tokens, a window of 512: 165, 141 and 138 us, backward 516, 476 and 471; 8 x 16 heads of 512, backward: 54, 49 and 44;
+ * 16 heads on 4 of 8,192, no window, backward: 1,470, 1,147 and 1,155. */
 __device__ inline int place(int count) {
     const int per = (count + 7) / 8, turn = (int)(blockIdx.x / 8), group = turn / 32 * 32;
     const int left = per - group < 32 ? per - group : 32;
@@ -335,7 +335,7 @@ template <class T, int DP, int PITCH> __device__ inline void block_step(Running<
  * long sequence makes small.  So they meet their products with a power of two of the lane's query or key, which moves only when a
  * gradient would pass 2^15 (the largest is 2^4 to 2^5 then: what is 2^18 times smaller still has all its bits) and takes the sums along.
  * It begins where no gradient above 2^-49 leaves it.  Normalized weights, 1 at most, meet theirs with 2^12.  The backward pass of 2 x 16
- * heads of 2,048 tokens and size 128, a window of 1,024, takes 164 us with this and 152 without. */
+ * heads of 2,048 tokens and size 128, a window of 1,024, takes 154 us with this and 149 without. */
 template <class T> struct Fit {
     static constexpr bool FITS = __is_same(T, f16);
     static constexpr int FIRST = FITS ? 64 : 0, WEIGHTS = FITS ? 12 : 0;
@@ -490,8 +490,8 @@ template <class T, int DP> __device__ inline void careful_block(f32x16 (&o)[DP /
 template <int DP> struct Shape { static constexpr int PITCH = DP <= 64 ? 64 : 128; };
 
 /* How many wavefronts of a SIMD a kernel is scheduled for: exactly as many as its registers allow, so that what is left of them goes to
- * operands on their way.  Without it: 4 x 40 heads of 2,048 tokens, a window of 512, 228 us instead of 160; 8 heads of 16,384, 2,048:
- * 230 instead of 157; 2 x 16 heads of 2,048, 1,024, forward and backward: 307 instead of 197 (before blocks overlapped in the forward kernel). */
+ * operands on their way.  Without it, forward and backward: 4 x 40 heads of 2,048 tokens, a window of 512, 142 and 638 us instead of 139 and
+ * 475; 8 heads on 2 of 16,384, 2,048: 147 and 841 instead of 141 and 507; 2 x 16 heads of 2,048, 1,024: 42 and 208 instead of 40 and 148. */
 #define RESIDENT(DP) __attribute__((amdgpu_waves_per_eu((DP) <= 64 ? 3 : 2, (DP) <= 64 ? 3 : 2)))
 
 constexpr int WAVES = 4, LANES = WAVES * 64, QUERIES = WAVES * 32, KEYS = 64;
@@ -846,14 +846,14 @@ template <class T> __global__ void __launch_bounds__(LANES) attend_join(const Ar
     if (lane == 0) a.lse[row] = total == 0.0f ? -__builtin_inff() : top * a.scale + __logf(total);
 }
 
-/* Of how many tiles a walk counts as short (attend_dq takes delta differently there): with up to three 64s of keys the error of dQ and
- * dK in half precision is 3.0e-4 of their norm, 3.1e-4 without; at most 0.7% of the backward pass's time (4 x 40 heads of 2,048,
- * a window of 512: 518 us and 515). */
+/* Of how many tiles a walk counts as short (attend_dq takes delta differently there): with up to three 64s of keys (150 tokens) the error of
+ * dQ and dK in half precision is 2.9e-4 of their norm, 3.2e-4 without; at most 0.8% of the backward pass's time (4 x 40 heads of
+ * 2,048, a window of 512: 475 us and 471). */
 constexpr int FEW_TILES = 3;
 
 /* dQ: queries in registers, keys in tiles as in attend_forward; per block of 32 keys S^T = K Q^T, dP^T = V dO^T,
  * dQ^T += K^T dS^T.  It also leaves delta = sum dO O of every query for attend_dkv.  2 x 16 heads of 2,048 tokens and size 128, a window of
- * 1,024: 67 us, 579 TFLOP/s of the pairs that are seen, the matrix units at work a third of the time. */
+ * 1,024: 63 us, 616 TFLOP/s of the pairs that are seen, the matrix units at work a third of the time. */
 template <class T, int DP> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_dq(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
@@ -1275,7 +1275,7 @@ template <class T, int DP, int SHARE> __global__ void __launch_bounds__(LANES) R
 
 /* The first keys and the queries beyond their window: every later query of every head sees those few keys, so the work is split
  * over the queries.  A wavefront walks over tiles of 32 queries with buffers of its own; a workgroup's sums, element d of key j at
- * [dk, dv][d][j], are one part, and attend_dkv adds the parts in order.  4 first keys of 2 x 16 heads, 1,024 queries beyond their window: 12 us,
+ * [dk, dv][d][j], are one part, and attend_dkv adds the parts in order.  4 first keys of 2 x 16 heads, 1,024 queries beyond their window: 13 us,
  * two or three tiles for each wavefront, from launch to end a chain of loads, one tile and the sums. */
 template <class T, int DP> __global__ void __launch_bounds__(LANES) __attribute__((amdgpu_waves_per_eu((DP) <= 64 ? 2 : 1))) attend_far(const Args a) {
     extern __shared__ char lds[];
@@ -1423,8 +1423,8 @@ template <class T, int DP> int forward(Args &k, const ace_attend_t *a, hipStream
 }
 
 /* Blocks of 32 first keys, and over how many workgroups the queries beyond their window go: as many as there are CUs, at least four
- * tiles of queries for a wavefront.  (4 x 40 heads of 2,048 queries, all of the backward pass: 495 us; with two workgroups for every CU
- * 513.  4 heads of 4 x 16,384: 369 us in up to 32 parts, 391 in up to 16.) */
+ * tiles of queries for a wavefront.  (4 x 40 heads of 2,048 queries, all of the backward pass: 475 us; with two workgroups for every CU
+ * 479.  4 heads on 1 of 16,384, a window of 2,048: 344 us in up to 32 parts, 354 in up to 16; 8 on 1 of 32,768, 1,024: 623 and 731.) */
 void far_of(const ace_attend_t *a, Args &k) {
     const int64_t sinks = a->window > 0 ? (a->sinks < a->keys ? a->sinks : a->keys) : 0;
     k.far_blocks = (int)((sinks + 31) / 32), k.far_parts = 0;
@@ -1436,9 +1436,9 @@ void far_of(const ace_attend_t *a, Args &k) {
     k.far_parts = parts < 1 ? 1 : parts > 32 ? 32 : (int)parts;
 }
 /* Fewer workgroups of 128 keys than this: half as many keys for each, or a quarter.  Measured, all of the backward pass, with 128, 64
- * and 32 keys, at 512 workgroups of 128 (2 x 16 heads of 2,048 tokens, a window of 512): 116, 124 and 210 us; at 384 (8 x 4 heads
- * of 1,531 tokens and size 64, 256): 125, 112 and 142; at 256: 84, 77 and 124; at 128 (8 heads): 80, 72 and 88; at 64 (4 key heads of 16):
- * 173, 131 and 117; at 8 (512 tokens, size 64): 81, 58 and 45. */
+ * and 32 keys, at 512 workgroups of 128 (2 x 16 heads of 2,048 tokens, a window of 512): 110, 118 and 190 us; at 384 (8 x 4 heads
+ * of 1,531 tokens and size 64, 256): 49, 49 and 63; at 256 (16 heads): 81, 75 and 115; at 128 (8 heads): 75, 68 and 81; at 64 (16 heads
+ * on 4): 155, 115 and 105; at 8 (2 heads of 512 tokens and size 64, no window): 33, 28 and 25. */
 constexpr int SHARED_BELOW = 448, SHARED_BY_4_BELOW = 96;
 int width_of(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 int64_t delta_floats(const ace_attend_t *a) { return ((int64_t)a->batch * a->heads * a->queries + 3) / 4 * 4; }

@@ -30,7 +30,8 @@ typedef __bf16 bf16;
 typedef _Float16 f16;
 
 /* Eight consecutive elements as they lie in memory.  Addresses are multiples of the element's size only: the loads and stores
- * below are full-width at any alignment (unaligned access is on for every process of this platform). */
+ * below, and those through buffer descriptors of the norms' rows, are full-width at any alignment (unaligned access is on for every
+ * process of this platform). */
 template <class T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
 template <class T> using vec8 = typename Vec8<T>::type;
 typedef float f32x8 __attribute__((ext_vector_type(8)));

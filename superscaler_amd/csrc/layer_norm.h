@@ -23,7 +23,10 @@ int norm_backward_launch(const NormArgs &a, int dtype, hipStream_t stream);
  * Up to 12,288 elements of 16 bits (7,680 of 32) the parameters lie in LDS beside the row and its sums in a lane's registers: one
  * vector per lane of up to 1,024, two of up to 768 lanes, whose 168 registers the backward pass needs.  Longer rows read the
  * parameters where they are and ask for no row ahead: at 12,288 that takes 161 us instead of 155 forward and 737 instead of 285 backward
- * (8,192 rows of bfloat16; at 7,680 of float32 223 and 195, 830 and 314).  Forward, two vectors per lane begin where one would need
+ * (8,192 rows of bfloat16; at 7,680 of float32 223 and 195, 830 and 314).  Their kernels are compiled for 1,024 lanes of 128 registers, which
+ * the backward pass overruns: 16,384 elements of bfloat16 take 1,060 us backward, 12,288 of float32 1,375, 1.5 and 1.8 TB/s of six rows,
+ * where shorter ones reach 4.2 to 4.7.  So do two vectors per lane of rows that do not end with a whole one: 8,193 elements of bfloat16
+ * in 179 and 426 us (8,192 in 104 and 178), 12,289 in 321 and 1,552.  Forward, two vectors per lane begin where one would need
  * more than 768 lanes, of which a CU holds one workgroup: 16,384 rows of 8,192 in 201 us instead of 231, of 6,656 in 177 instead of 216, of
  * 6,144 in 171 against 156.  Backward the sums of a second vector cost more than that: 379 us against 320 at 8,192. */
 struct NormShape { int nv, lanes; };

@@ -12,7 +12,7 @@
  * such pair to the next at least one of the two steps on, so no two share a row).
  *
  * 4 x 2,048 rows of 12,288 elements of bfloat16, both norms and a gate per sequence: 283 us and 19 for the second launch, 4.3 TB/s of six
- * rows' traffic; 16 x 509 of 1,024 of float32: 38 and 13.  A CU holds one workgroup of the wide rows, whose lanes all wait for two
+ * rows' traffic; 16 x 509 of 1,024 of float32: 42 and 8.  A CU holds one workgroup of the wide rows, whose lanes all wait for two
  * sums over the row: that, and not the traffic, is what is left.  (The second launch with one sum to a workgroup, twice as many
  * loads in the air, took 28 us instead of 19.)
  */
