@@ -269,6 +269,9 @@ def main(argv=None):
     graph = synth.make_graph(w)
     base = synth.make_db(w, graph)
     heads = w.hidden // HEAD
+    for what, asked, there in (("--micro-batches", args.micro_batches, base.mbs_list), ("--tp", args.tp, [t for t in base.tp_list if heads % t == 0])):
+        if any(v not in there for v in asked or ()):
+            ap.error(f"{what}: of workload {w.name} there are {there}")
     measured = {(b, tp): measure(w, b, tp, args.window, args.sinks, reps=args.reps)
                 for b in (args.micro_batches or base.mbs_list) for tp in (args.tp or base.tp_list) if heads % tp == 0}
     db = database(w, graph, measured, base)

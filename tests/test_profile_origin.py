@@ -37,6 +37,13 @@ def test_files_say_which_of_them_were_measured(tmp_path):
     assert [r[:2] for r in rows if r[2] == "measured"] == [["2", "4"]]
 
 
+@pytest.mark.parametrize("args", [["--tp", "3"], ["--tp", "1", "16"], ["--micro-batches", "5"]])
+def test_sizes_that_the_database_does_not_have(args, capsys):
+    with pytest.raises(SystemExit) as e:
+        profile_layer.main(["--workload", "gpt3_1_3b"] + args)
+    assert e.value.code == 2 and "gpt3_1_3b there are [1, 2, 4" in capsys.readouterr().err
+
+
 @gpu
 def test_times_are_the_card_s():
     """A call whose host part takes 300 us and whose kernels take a few."""
