@@ -19,7 +19,7 @@
 extern "C" {
 #endif
 
-#define ACE_LAYER_ABI_VERSION 1
+#define ACE_LAYER_ABI_VERSION 2
 
 enum { ACE_T_F32 = 0, ACE_T_BF16 = 1, ACE_T_F16 = 2, ACE_T_NONE = 3 };
 
@@ -123,6 +123,59 @@ int ace_adamw_step(const ace_adamw_t *a, const void *const *grads, const int64_t
 /* The values that 8-bit moments stand for: float[n_blocks * 256] each. */
 int ace_adamw_moments(const int8_t *d_m, const uint8_t *d_v, const float *d_m_scale, const float *d_v_scale, int64_t n_blocks, float *d_m_out,
                       float *d_v_out, void *stream);
+
+/* ---- the norm of many gradients, and clipping --------------------------------------------------------------------------
+ *     norms[t] = |s| sqrt(sum g^2 over tensor t);  norm = sqrt(sum of norms[t]^2);  scale = s min(1, max_norm / (norm + 1e-6))
+ * with s = *d_grad_scale (1 where it is NULL) and max_norm 0: no limit.  Squares and sums in 64 bits, in an order that the sizes alone
+ * decide.  A norm that is no number makes scale none, an infinite one makes it 0, where there is a limit. */
+typedef struct ace_gradient {      /* HOST array, read during the call */
+    void *d_grad;                  /* elements one after the other */
+    int64_t n;
+    int32_t dtype;                 /* ACE_T_F32, _BF16 or _F16 */
+    int32_t reserved;
+} ace_gradient_t;
+
+/* d_result: norm and scale; d_norms: float[n_tensors].  d_workspace: ace_gradient_norm_workspace_bytes(...) bytes, a multiple of 8.  Up to 2^20
+ * tensors of up to 2^37 elements. */
+size_t ace_gradient_norm_workspace_bytes(const ace_gradient_t *grads, int64_t n_tensors);
+int ace_gradient_norm(const ace_gradient_t *grads, int64_t n_tensors, double max_norm, const float *d_grad_scale, float *d_result, float *d_norms,
+                      void *d_workspace, size_t workspace_bytes, void *stream);
+/* g = g scale, in place, rounded to g's type; nothing is written where scale is 1.  No two tensors may overlap. */
+int ace_gradient_scale(const ace_gradient_t *grads, int64_t n_tensors, const float *d_scale, void *stream);
+
+/* ---- log-probabilities of taken tokens, and the clipped policy loss ----------------------------------------------------------
+ * Of every row z of `vocab` logits, with its target t:
+ *     top = max z;  total = sum exp(z - top);  logp = z_t - top - log total
+ *     ratio = exp(logp - old);  gain = min(ratio A, clamp(ratio, ratio_low, ratio_high) A);  away = ref - logp
+ *     loss += w (kl_weight (exp(away) - away - 1) - gain)                     (without d_ref: no term of it)
+ *     d_logp = w (kl_weight (1 - exp(away)) - ratio A where the gain is not clipped)
+ *     d_z = g d_logp ([it is the target] - exp(z - top) / total)
+ * A row whose target is not in [0, vocab) has none: logp 0, no loss, gradients 0, statistics 0; its logits may be anything.  Nor does a row
+ * of weight 0 take part in the loss, whatever its numbers are; where d_logp is 0, d_z is.
+ * Exponentials in 32 bits, sums over lanes and what follows from them for a row in 64. */
+#define ACE_LOSS_MAX_VOCAB (1 << 28)
+typedef struct ace_token_loss {
+    int64_t rows, row_stride;      /* row_stride: elements between consecutive rows of d_logits, at least vocab */
+    int32_t vocab, dtype;          /* ACE_T_* */
+    int32_t target_bits;           /* 32 or 64 */
+    int32_t reserved;
+    const void *d_logits;
+    const void *d_targets;         /* int32 or int64 [rows] */
+    /* for the policy's loss: float [rows] each; d_ref and d_weight may be NULL (every row's weight is even_weight then) */
+    const float *d_old, *d_advantage, *d_ref, *d_weight;
+    double ratio_low, ratio_high, kl_weight, even_weight;
+} ace_token_loss_t;
+
+/* d_logp: float[rows]; d_stats: float[rows][2] = top and total. */
+int ace_token_logprobs(const ace_token_loss_t *a, float *d_logp, float *d_stats, void *stream);
+/* d_dlogits: of the logits' type, rows out_stride elements apart; may be the logits themselves, row for row.  g_logp: float[rows]. */
+int ace_token_logprobs_backward(const ace_token_loss_t *a, const float *g_logp, const float *d_stats, void *d_dlogits, int64_t out_stride, void *stream);
+/* d_loss: one float; d_dlogp: float[rows], for g = 1.  d_workspace: ace_policy_loss_workspace_bytes(a) bytes, a multiple of 8. */
+size_t ace_policy_loss_workspace_bytes(const ace_token_loss_t *a);
+int ace_policy_loss(const ace_token_loss_t *a, float *d_loss, float *d_logp, float *d_stats, float *d_dlogp, void *d_workspace, size_t workspace_bytes, void *stream);
+/* The same with the gradient of the logits, for a gradient of the loss of *g_loss (1 where it is NULL). */
+int ace_policy_loss_gradient(const ace_token_loss_t *a, const float *g_loss, float *d_loss, float *d_logp, float *d_stats, float *d_dlogp, void *d_dlogits,
+                             int64_t out_stride, void *d_workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,261 @@
+/*
+ * Log-probabilities of taken tokens and the clipped policy loss (ace_token_logprobs, ace_policy_loss), with gradients.
+ *
+ * Rows of logits, thousands to a hundred thousand elements each, are read once. A lane keeps a maximum of its own and the sum of exponentials
+ * around it, 32 bits each; lanes and wavefronts are joined in 64 bits, and one lane goes on in 64 bits from the row's maximum and sum to its
+ * log-probability, loss and derivative: a ratio that stands next to the border of its clipping falls on the side that it belongs to.
+ */
+#include "layer_common.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LOG2E_REST = (float)(1.4426950408889634 - (double)1.4426950408889634f);
+
+struct Loss {
+    int64_t rows, stride, out_stride;
+    int vocab, wide;                     /* wide: targets of 64 bits */
+    const void *logits, *targets;
+    const float *old, *advantage, *ref, *weight, *g;
+    double low, high, kl_weight, even_weight;
+    float *logp, *stats, *d_logp, *loss;
+    double *row_loss;
+    void *d_logits;
+};
+
+__device__ inline int64_t target_of(const Loss &a, int64_t row) { return a.wide ? ((const int64_t *)a.targets)[row] : ((const int32_t *)a.targets)[row]; }
+__device__ inline bool there(const Loss &a, int64_t target) { return (uint64_t)target < (uint64_t)a.vocab; }
+
+/* What a row has come to: its largest logit, and the sum of exponentials around it. */
+struct Row {
+    float top;
+    double total;
+};
+/* The rows' part in 64 bits, by one lane: results of the row, and its derivative. */
+template <bool POLICY> __device__ inline float settle(const Loss &a, int64_t row, const Row &r, float taken) {
+    const double logp = (double)taken - (double)r.top - log(r.total);
+    a.logp[row] = (float)logp;
+    a.stats[2 * row] = r.top, a.stats[2 * row + 1] = (float)r.total;
+    if (!POLICY) return 0.0f;
+    const double w = a.weight ? (double)a.weight[row] : a.even_weight, A = a.advantage[row], ratio = exp(logp - (double)a.old[row]);
+    if (w == 0.0) {   /* (it takes no part, whatever its numbers are) */
+        a.row_loss[row] = 0.0, a.d_logp[row] = 0.0f;
+        return 0.0f;
+    }
+    const double held = ratio < a.low ? a.low : ratio > a.high ? a.high : ratio;   /* (what is no number stays none) */
+    const bool clipped = A > 0.0 ? ratio > a.high : ratio < a.low;
+    double loss = -(clipped ? held : ratio) * A, d = -(clipped ? 0.0 : ratio) * A;
+    if (a.ref) {
+        const double away = (double)a.ref[row] - logp, e = expm1(away);
+        loss += a.kl_weight * (e - away), d -= a.kl_weight * e;
+    }
+    a.row_loss[row] = w * loss;
+    a.d_logp[row] = (float)(w * d);
+    return (float)(w * d);
+}
+/* a row without a target */
+template <bool POLICY> __device__ inline void settle_none(const Loss &a, int64_t row) {
+    a.logp[row] = 0.0f, a.stats[2 * row] = 0.0f, a.stats[2 * row + 1] = 0.0f;
+    if (POLICY) a.row_loss[row] = 0.0, a.d_logp[row] = 0.0f;
+}
+
+__device__ inline float around(float top) { return top == -__builtin_inff() ? 0.0f : top; }
+/* exp(x), x a difference of two logits, so that nothing is lost before.  (Without the rest of log2 e all terms of a row are off to one side, by
+ * 1.3e-8 of x each, and its log-probability by some 1e-7.) */
+__device__ inline float power(float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, LOG2E, x * LOG2E_REST)); }
+
+/* Joins the lanes' maxima and sums; all lanes know the result.  `tops`, `sums`: one for each wavefront, not in use. */
+template <int LANES> __device__ inline Row join(float top, float total, float *tops, double *sums) {
+    float most = top;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    double x = (double)(total * power(top - around(most)));
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = most, sums[threadIdx.x >> 6] = x;
+    __syncthreads();
+    Row r = {-__builtin_inff(), 0.0};
+#pragma unroll
+    for (int w = 0; w < LANES / 64; ++w) r.top = fmaxf(r.top, tops[w]);
+#pragma unroll
+    for (int w = 0; w < LANES / 64; ++w) r.total += sums[w] * (double)power(tops[w] - around(r.top));
+    return r;
+}
+
+/* A row per workgroup, 32 elements per lane and pass. */
+template <class T, int LANES, bool POLICY> __global__ void __launch_bounds__(LANES) loss_rows(const Loss a) {
+    __shared__ float tops[LANES / 64];
+    __shared__ double sums[LANES / 64];
+    const float inf = __builtin_inff();
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *z = (const T *)a.logits + row * a.stride;
+        const int64_t target = target_of(a, row);
+        if (!there(a, target)) {
+            if (threadIdx.x == 0) settle_none<POLICY>(a, row);
+            continue;
+        }
+        const float taken = (float)z[target];
+        float top = -inf, total = 0.0f;
+        constexpr int PASS = LANES * 8 * 4;
+        for (int at = threadIdx.x * 8; at < a.vocab; at += PASS) {
+            float x[32], most = -inf;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int from = at + k * LANES * 8, left = a.vocab - from;
+                const vec8<T> v = left > 0 ? load_some(z + from, left) : vec8<T>{};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[8 * k + i] = i < left ? (float)v[i] : -inf, most = fmaxf(most, x[8 * k + i]);
+            }
+            if (most > top) total *= power(top - most), top = most;
+            const float base = around(top);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) total += power(x[i] - base);
+        }
+        const Row r = join<LANES>(top, total, tops, sums);
+        if (threadIdx.x == 0) settle<POLICY>(a, row, r, taken);
+        __syncthreads();
+    }
+}
+
+/* Gradients of a row's logits, COLUMNS of them per workgroup. */
+constexpr int BACK_LANES = 256, COLUMNS = BACK_LANES * 8 * 4;
+template <class T> __global__ void __launch_bounds__(BACK_LANES) loss_back(const Loss a, bool policy) {
+    const int parts = (a.vocab + COLUMNS - 1) / COLUMNS;
+    const int64_t items = a.rows * parts;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t row = item / parts, target = target_of(a, row);
+        const int first = (int)(item - row * parts) * COLUMNS;
+        const T *z = (const T *)a.logits + row * a.stride;
+        T *to = (T *)a.d_logits + row * a.out_stride;
+        const float d = !there(a, target) ? 0.0f : policy ? a.d_logp[row] * (a.g ? *a.g : 1.0f) : a.g[row], top = a.stats[2 * row], by = 1.0f / a.stats[2 * row + 1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int at = first + (k * BACK_LANES + threadIdx.x) * 8, left = a.vocab - at;
+            if (left <= 0) break;
+            vec8<T> r = {};
+            if (d != 0.0f) {   /* (of a row that takes no part nothing is read) */
+                const vec8<T> v = load_some(z + at, left);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[i] = (T)(d * ((at + i == target ? 1.0f : 0.0f) - power((float)v[i] - top) * by));
+            }
+            store_some(to + at, r, left);
+        }
+    }
+}
+
+/* the sum of the rows' losses */
+constexpr int SUM_LANES = 1024;
+__global__ void __launch_bounds__(SUM_LANES) loss_sum(const double *each, int64_t rows, float *loss) {
+    __shared__ double sums[SUM_LANES / 64];
+    double x = 0.0;
+    for (int64_t i = threadIdx.x; i < rows; i += SUM_LANES) x += each[i];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = x;
+    __syncthreads();
+    if (threadIdx.x > 0) return;
+    x = 0.0;
+    for (int w = 0; w < SUM_LANES / 64; ++w) x += sums[w];
+    *loss = (float)x;
+}
+
+int check(const ace_token_loss_t *a, bool policy) {
+    if (!a || a->rows < 0 || a->vocab < 1 || a->dtype < ACE_T_F32 || a->dtype > ACE_T_F16 || (a->target_bits != 32 && a->target_bits != 64)) return ACE_EINVAL;
+    if (a->vocab > ACE_LOSS_MAX_VOCAB || a->rows > (int64_t)1 << 40) return ACE_ETOOBIG;
+    if (policy && !(a->ratio_low >= 0.0 && a->ratio_low <= 1.0 && a->ratio_high >= 1.0 && a->kl_weight >= 0.0)) return ACE_EINVAL;
+    if (a->rows == 0) return ACE_OK;
+    if (!a->d_logits || !a->d_targets || (a->rows > 1 && a->row_stride < a->vocab) || (policy && (!a->d_old || !a->d_advantage))) return ACE_EINVAL;
+    if (((uintptr_t)a->d_logits & (a->dtype == ACE_T_F32 ? 3 : 1)) || ((uintptr_t)a->d_targets & (a->target_bits / 8 - 1))) return ACE_EINVAL;
+    return ACE_OK;
+}
+
+Loss args_of(const ace_token_loss_t *a) {
+    Loss k = {};
+    k.rows = a->rows, k.stride = a->row_stride, k.vocab = a->vocab, k.wide = a->target_bits == 64, k.logits = a->d_logits, k.targets = a->d_targets;
+    k.old = a->d_old, k.advantage = a->d_advantage, k.ref = a->d_ref, k.weight = a->d_weight;
+    k.low = a->ratio_low, k.high = a->ratio_high, k.kl_weight = a->kl_weight, k.even_weight = a->even_weight;
+    return k;
+}
+
+constexpr int64_t MOST_GROUPS = (int64_t)1 << 21;   /* of a launch: 2^31 lanes */
+uint32_t groups(int64_t n) { return (uint32_t)(n < MOST_GROUPS ? n : MOST_GROUPS); }
+
+/* go(one of the type's values) */
+template <class Go> int by_type(int dtype, Go go) { return dtype == ACE_T_F32 ? go(float()) : dtype == ACE_T_BF16 ? go(bf16()) : go(f16()); }
+
+template <bool POLICY> int forward(const Loss &k, int dtype, hipStream_t s) {
+    if (k.rows == 0) return ACE_OK;
+    return by_type(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        if (k.rows < 512 && k.vocab > 8192) loss_rows<T, 1024, POLICY><<<groups(k.rows), 1024, 0, s>>>(k);
+        else loss_rows<T, 256, POLICY><<<groups(k.rows), 256, 0, s>>>(k);
+        return layer_launched();
+    });
+}
+int backward(const Loss &k, int dtype, bool policy, hipStream_t s) {
+    if (k.rows == 0) return ACE_OK;
+    const uint32_t grid = groups(k.rows * ((k.vocab + COLUMNS - 1) / COLUMNS));
+    return by_type(dtype, [&](auto t) {
+        loss_back<decltype(t)><<<grid, BACK_LANES, 0, s>>>(k, policy);
+        return layer_launched();
+    });
+}
+int check_out(const ace_token_loss_t *a, const void *out, int64_t stride) {
+    if (a->rows == 0) return ACE_OK;
+    if (!out || ((uintptr_t)out & (a->dtype == ACE_T_F32 ? 3 : 1)) || (a->rows > 1 && stride < a->vocab)) return ACE_EINVAL;
+    return out == a->d_logits && a->rows > 1 && stride != a->row_stride ? ACE_EINVAL : ACE_OK;
+}
+
+}  // namespace
+
+extern "C" int ace_token_logprobs(const ace_token_loss_t *a, float *d_logp, float *d_stats, void *stream) {
+    const int rc = check(a, false);
+    if (rc != ACE_OK || a->rows == 0) return rc;
+    if (!d_logp || !d_stats) return ACE_EINVAL;
+    Loss k = args_of(a);
+    k.logp = d_logp, k.stats = d_stats;
+    return forward<false>(k, a->dtype, (hipStream_t)stream);
+}
+
+extern "C" int ace_token_logprobs_backward(const ace_token_loss_t *a, const float *g_logp, const float *d_stats, void *d_dlogits, int64_t out_stride, void *stream) {
+    int rc = check(a, false);
+    if (rc != ACE_OK || a->rows == 0) return rc;
+    if (!g_logp || !d_stats || (rc = check_out(a, d_dlogits, out_stride)) != ACE_OK) return ACE_EINVAL;
+    Loss k = args_of(a);
+    k.g = g_logp, k.stats = (float *)d_stats, k.d_logits = d_dlogits, k.out_stride = out_stride;
+    return backward(k, a->dtype, false, (hipStream_t)stream);
+}
+
+extern "C" size_t ace_policy_loss_workspace_bytes(const ace_token_loss_t *a) { return check(a, true) == ACE_OK ? (size_t)a->rows * sizeof(double) : 0; }
+
+static int policy(const ace_token_loss_t *a, Loss &k, float *d_loss, float *d_logp, float *d_stats, float *d_dlogp, void *d_workspace, size_t workspace_bytes) {
+    const int rc = check(a, true);
+    if (rc != ACE_OK) return rc;
+    if (!d_loss || (a->rows > 0 && (!d_logp || !d_stats || !d_dlogp || !d_workspace))) return ACE_EINVAL;
+    if (((uintptr_t)d_workspace & 7) || workspace_bytes < ace_policy_loss_workspace_bytes(a)) return ACE_EINVAL;
+    k = args_of(a);
+    k.logp = d_logp, k.stats = d_stats, k.d_logp = d_dlogp, k.row_loss = (double *)d_workspace, k.loss = d_loss;
+    return ACE_OK;
+}
+static int sum(const Loss &k, hipStream_t s) {
+    loss_sum<<<1, SUM_LANES, 0, s>>>(k.row_loss, k.rows, k.loss);
+    return layer_launched();
+}
+
+extern "C" int ace_policy_loss(const ace_token_loss_t *a, float *d_loss, float *d_logp, float *d_stats, float *d_dlogp, void *d_workspace, size_t workspace_bytes,
+                               void *stream) {
+    Loss k;
+    int rc = policy(a, k, d_loss, d_logp, d_stats, d_dlogp, d_workspace, workspace_bytes);
+    if (rc != ACE_OK || (rc = forward<true>(k, a->dtype, (hipStream_t)stream)) != ACE_OK) return rc;
+    return sum(k, (hipStream_t)stream);
+}
+
+extern "C" int ace_policy_loss_gradient(const ace_token_loss_t *a, const float *g_loss, float *d_loss, float *d_logp, float *d_stats, float *d_dlogp, void *d_dlogits,
+                                        int64_t out_stride, void *d_workspace, size_t workspace_bytes, void *stream) {
+    Loss k;
+    int rc = policy(a, k, d_loss, d_logp, d_stats, d_dlogp, d_workspace, workspace_bytes);
+    if (rc != ACE_OK || (rc = check_out(a, d_dlogits, out_stride)) != ACE_OK) return rc;
+    k.g = g_loss, k.d_logits = d_dlogits, k.out_stride = out_stride;
+    if ((rc = forward<true>(k, a->dtype, (hipStream_t)stream)) != ACE_OK) return rc;
+    if ((rc = backward(k, a->dtype, true, (hipStream_t)stream)) != ACE_OK) return rc;
+    return sum(k, (hipStream_t)stream);
+}

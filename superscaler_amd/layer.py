@@ -5,6 +5,9 @@ whose state bytes the memory model counts:
 
   block_norm, block_norm_backward               norm at a block's exit, gate, scaled residual, norm at the next block's entry
   window_attention, window_attention_backward   causal attention over a window of keys and a few first ones; prompts and single tokens
+  token_logprobs, token_logprobs_backward       log-probabilities of the tokens that were taken
+  policy_loss, policy_loss_gradient             a policy's clipped loss with a term that keeps it near to another one
+  gradient_norm, clip_gradients                 the norm of many tensors, and the factor that AdamW.step or clipping in place takes
   AdamW                                         one step over many tensors at once, moments in 32 or 8 bits
 
 Tensors live on a GPU; work goes to the stream that is current on their device, and nothing waits for it.  A tensor last used on
@@ -14,6 +17,7 @@ sizes raise ValueError, other types TypeError, a missing library or a HIP failur
 Gradients come from the *_backward calls; torch's automatic differentiation records nothing of these operators.  Where it is on and an
 input requires a gradient, so do the results, and going backward through them raises AceError: no gradient is lost unnoticed.
 """
+import array
 import ctypes
 import math
 import os
@@ -30,17 +34,19 @@ _lib = None
 
 EXPORTS = ["ace_layer_abi_version", "ace_layer_strerror", "ace_layer_last_hip_error", "ace_block_norm_forward", "ace_block_norm_workspace_bytes",
            "ace_block_norm_backward", "ace_attend_workspace_bytes", "ace_attend_forward", "ace_attend_backward_workspace_bytes",
-           "ace_attend_backward", "ace_adamw_step", "ace_adamw_moments"]
-ABI_VERSION = 1
+           "ace_attend_backward", "ace_adamw_step", "ace_adamw_moments", "ace_gradient_norm_workspace_bytes", "ace_gradient_norm", "ace_gradient_scale",
+           "ace_token_logprobs", "ace_token_logprobs_backward", "ace_policy_loss_workspace_bytes", "ace_policy_loss", "ace_policy_loss_gradient"]
+ABI_VERSION = 2
 MAX_WIDTH = 32768       # ACE_NORM_MAX_WIDTH
 MAX_HEAD = 128
+MAX_VOCAB = 1 << 28     # ACE_LOSS_MAX_VOCAB
 ADAMW_BLOCK, ADAMW_CHUNK = 256, 8192
 
 _NONE = 3
 _LONGEST = (1 << 31) - 1
 _HALVES = (torch.bfloat16, torch.float16)
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_vp, _i32, _i64, _f32 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float
+_vp, _i32, _i64, _f32, _f64, _size = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_size_t
 
 
 # ace_block_norm_t: rows, rows_per_gate; width, dtype, layer; residual_scale, eps; seven pointers (packed: a third of the time that a
@@ -49,6 +55,10 @@ _BLOCK_NORM = struct.Struct("=2q3i2f4x7Q")
 # ace_attend_t: batch, queries, keys, heads, kv_heads, dim, dtype, window, sinks; scale; start and length; four times three strides;
 # q, k, v, out and lse
 _ATTEND = struct.Struct("=9if2Q12q5Q")
+
+# ace_token_loss_t: rows, row_stride; vocab, dtype, target_bits; logits, targets, old, advantage, ref, weight; the ratio's bounds, the term's
+# weight, an even weight of rows
+_TOKEN_LOSS = struct.Struct("=2q3i4x6Q4d")
 
 
 class _AdamW(ctypes.Structure):
@@ -68,7 +78,8 @@ def load_library():
         getattr(lib, name).restype = ctypes.c_int
     for name in ("ace_layer_strerror", "ace_layer_last_hip_error"):
         getattr(lib, name).restype = ctypes.c_char_p
-    for name in ("ace_block_norm_workspace_bytes", "ace_attend_workspace_bytes", "ace_attend_backward_workspace_bytes"):
+    for name in ("ace_block_norm_workspace_bytes", "ace_attend_workspace_bytes", "ace_attend_backward_workspace_bytes", "ace_gradient_norm_workspace_bytes",
+                 "ace_policy_loss_workspace_bytes"):
         getattr(lib, name).restype = ctypes.c_size_t
     lib.ace_layer_strerror.argtypes = [ctypes.c_int]
     lib.ace_block_norm_forward.argtypes = [_vp] * 5
@@ -80,6 +91,14 @@ def load_library():
     lib.ace_attend_backward.argtypes = [_vp] * 7 + [ctypes.c_size_t, _vp]
     lib.ace_adamw_step.argtypes = [_vp] * 4 + [_f32] * 8 + [_vp]
     lib.ace_adamw_moments.argtypes = [_vp] * 4 + [_i64, _vp, _vp, _vp]
+    lib.ace_gradient_norm_workspace_bytes.argtypes = [_vp, _i64]
+    lib.ace_gradient_norm.argtypes = [_vp, _i64, _f64] + [_vp] * 4 + [_size, _vp]
+    lib.ace_gradient_scale.argtypes = [_vp, _i64, _vp, _vp]
+    lib.ace_token_logprobs.argtypes = [_vp] * 4
+    lib.ace_token_logprobs_backward.argtypes = [_vp] * 4 + [_i64, _vp]
+    lib.ace_policy_loss_workspace_bytes.argtypes = [_vp]
+    lib.ace_policy_loss.argtypes = [_vp] * 6 + [_size, _vp]
+    lib.ace_policy_loss_gradient.argtypes = [_vp] * 7 + [_i64, _vp, _size, _vp]
     if lib.ace_layer_abi_version() != ABI_VERSION:
         raise AceError("libace_layer.so has a different ABI version")
     _lib = lib
@@ -364,6 +383,270 @@ def window_attention_backward(d_out, q, k, v, out, lse, *, window=None, sinks=0,
     workspace = q.new_empty(size, dtype=torch.uint8)
     _call(q.device, "ace_attend_backward", a, d_out.data_ptr(), (_i64 * 3)(*d_strides), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), size)
     return dq, dk, dv
+
+
+# ---- log-probabilities of taken tokens, and the policy's loss -----------------------------------------------------------------
+class TokenLogprobs(NamedTuple):
+    """`logp`: float32 of the targets' shape, `stats`: float32 [..., 2], each row's largest logit and sum of exponentials around it, for
+    token_logprobs_backward."""
+    logp: torch.Tensor
+    stats: torch.Tensor
+
+
+class PolicyLoss(NamedTuple):
+    """`loss`: float32 of no dimension, `logp` and `stats`: as token_logprobs returns them, `d_logp`: the loss's derivative by each
+    log-probability, float32."""
+    loss: torch.Tensor
+    logp: torch.Tensor
+    stats: torch.Tensor
+    d_logp: torch.Tensor
+
+
+def _flat_rows(t):
+    """Elements between consecutive rows of a [..., width] tensor whose rows lie evenly, each one's elements adjacent; otherwise None."""
+    shape, strides = t.shape, t.stride()
+    if shape[-1] > 1 and strides[-1] != 1:
+        return None
+    step, rows = None, 1
+    for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if n == 1:
+            continue
+        if step is None:
+            step = s
+        elif s != step * rows:
+            return None
+        rows *= n
+    if step is None:
+        return shape[-1]
+    return step if step >= shape[-1] else None
+
+
+def _token_loss_args(logits, targets, old_logp=None, advantages=None, ref_logp=None, weights=None, bounds=(0.0, 1.0), kl_weight=0.0):
+    """(packed arguments, logits as the kernels read them, the tensors whose addresses the arguments hold)"""
+    _on_gpu(logits, "logits")
+    _on_gpu(targets, "targets")
+    if logits.dtype not in _TYPES:
+        raise TypeError(f"logits: float32, bfloat16 or float16 expected, not {logits.dtype}")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_VOCAB:
+        raise ValueError(f"logits: rows of 1 to {MAX_VOCAB} elements expected, got shape {tuple(logits.shape)}")
+    if targets.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"targets: int64 or int32 expected, not {targets.dtype}")
+    shape, device = logits.shape[:-1], logits.device
+    if targets.shape != shape or targets.device != device:
+        raise ValueError(f"targets: {tuple(shape)} on {device} expected, got {tuple(targets.shape)} on {targets.device}")
+    rows = [old_logp, advantages, ref_logp, weights]
+    for i, (name, t) in enumerate(zip(("old_logp", "advantages", "ref_logp", "weights"), rows)):
+        if t is None:
+            continue
+        _on_gpu(t, name)
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name}: float32 expected, not {t.dtype}")
+        if t.shape != shape or t.device != device:
+            raise ValueError(f"{name}: {tuple(shape)} on {device} expected, got {tuple(t.shape)} on {t.device}")
+        rows[i] = t.contiguous()
+    stride = _flat_rows(logits)
+    if stride is None:
+        logits = logits.contiguous()
+        stride = logits.shape[-1]
+    targets, n = targets.contiguous(), targets.numel()
+    a = _TOKEN_LOSS.pack(n, stride, logits.shape[-1], _TYPES[logits.dtype], 64 if targets.dtype is torch.int64 else 32, logits.data_ptr(), targets.data_ptr(),
+                         *[0 if t is None else t.data_ptr() for t in rows], *bounds, kl_weight, 1 / n if n else 0.0)
+    return a, logits, [targets] + rows
+
+
+def _gradient_of(logits, out):
+    """Where the logits' gradient goes: (tensor, elements between its rows)"""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        return out, logits.shape[-1]
+    _on_gpu(out, "out")
+    if out.dtype != logits.dtype:
+        raise TypeError(f"out: {logits.dtype} expected like logits, not {out.dtype}")
+    stride = _flat_rows(out)
+    if out.shape != logits.shape or out.device != logits.device or stride is None:
+        raise ValueError(f"out: rows {tuple(logits.shape)} on {logits.device} expected, got {tuple(out.shape)} on {out.device}")
+    rows, size = math.prod(out.shape[:-1]), out.element_size()
+
+    def end(t, step):
+        return t.data_ptr() + ((rows - 1) * step + t.shape[-1]) * size
+    own = _flat_rows(logits)
+    if rows and not (out.data_ptr() == logits.data_ptr() and (stride == own or rows == 1)) and out.data_ptr() < end(logits, own) and logits.data_ptr() < end(out, stride):
+        raise ValueError("out: the logits themselves or memory of its own expected")
+    return out, stride
+
+
+def token_logprobs(logits, targets) -> TokenLogprobs:
+    """Log-probability of each target under the softmax of its row of logits: logp = logits[target] - log sum exp(logits), in one pass.
+
+    logits [..., vocab] float32, bfloat16 or float16, targets [...] int64 or int32.  A target that is not in [0, vocab) stands for none (a
+    token of the prompt, a padded place): its logp is 0, and its logits may be anything.  Logits of -inf are tokens that cannot be taken."""
+    a, z, keep = _token_loss_args(logits, targets)
+    logp = torch.empty(targets.shape, dtype=torch.float32, device=z.device)
+    stats = torch.empty(targets.shape + (2,), dtype=torch.float32, device=z.device)
+    _call(z.device, "ace_token_logprobs", a, logp.data_ptr(), stats.data_ptr())
+    if _lost(logits):
+        logp, stats = _untracked("token_logprobs", (logp, stats), (logits,))
+    return TokenLogprobs(logp, stats)
+
+
+def token_logprobs_backward(d_logp, logits, targets, stats, *, out=None):
+    """Gradient of token_logprobs' logits from that of its `logp` (float32) and its `stats`: d_logp ([target] - softmax), 0 where d_logp is or
+    there is no target.  Cross entropy, averaged over n tokens, has d_logp = -1 / n; policy_loss has d_loss times its own `d_logp`.
+    `out`: None, or where the gradient goes, which may be the logits themselves."""
+    if out is logits and _flat_rows(logits) is None:
+        raise ValueError("out: logits of rows that lie evenly expected")
+    a, z, keep = _token_loss_args(logits, targets, d_logp)
+    _on_gpu(stats, "stats")
+    if stats.dtype != torch.float32 or stats.shape != targets.shape + (2,) or not stats.is_contiguous() or stats.device != z.device:
+        raise ValueError("stats: what token_logprobs returned expected")
+    grad, stride = _gradient_of(z, out)
+    _call(z.device, "ace_token_logprobs_backward", a, keep[1].data_ptr(), stats.data_ptr(), grad.data_ptr(), stride)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+    return grad
+
+
+def _policy_args(logits, targets, old_logp, advantages, ref_logp, weights, clip, kl_weight):
+    low, high = clip
+    if not (0 <= low <= 1 and 0 <= high < math.inf):
+        raise ValueError(f"clip: how far a ratio may fall, up to 1, and rise expected, got {clip}")
+    if not 0 <= kl_weight < math.inf:
+        raise ValueError(f"kl_weight: a number from 0 on expected, got {kl_weight}")
+    for name, t in (("old_logp", old_logp), ("advantages", advantages)):
+        if t is None:
+            raise TypeError(f"{name}: a tensor expected")
+    a, z, keep = _token_loss_args(logits, targets, old_logp, advantages, ref_logp, weights, (1 - low, 1 + high), kl_weight)
+    made = PolicyLoss(*(torch.empty(size, dtype=torch.float32, device=z.device) for size in ((), targets.shape, targets.shape + (2,), targets.shape)))
+    return a, z, keep, made, torch.empty(targets.numel(), dtype=torch.float64, device=z.device)
+
+
+def policy_loss(logits, targets, old_logp, advantages, *, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_weight=0.0) -> PolicyLoss:
+    """A policy's clipped loss over the tokens that an earlier one took, from its logits, in one pass:
+
+        ratio = exp(logp - old_logp);  gain = min(ratio A, clamp(ratio, 1 - clip[0], 1 + clip[1]) A)
+        loss = sum of weights (kl_weight (exp(ref_logp - logp) - (ref_logp - logp) - 1) - gain)
+
+    logp: of `targets`, as in token_logprobs; A: `advantages`.  `ref_logp`: log-probabilities by the policy that this one is to stay near to
+    (None: no such term); `weights`: None (1 / tokens each), or the tokens' parts in the loss, 0 for tokens that take none, whose other numbers
+    may be anything.  All are float32 of the targets' shape.  Tokens without a target count as in token_logprobs and take no part.  The
+    gradient of logits is token_logprobs_backward(d_loss * d_logp, logits, targets, stats), or comes along from policy_loss_gradient."""
+    a, z, keep, made, workspace = _policy_args(logits, targets, old_logp, advantages, ref_logp, weights, clip, kl_weight)
+    _call(z.device, "ace_policy_loss", a, *map(_pointer, (made.loss, made.logp, made.stats, made.d_logp, workspace)), workspace.numel() * 8)
+    if _lost(logits, old_logp, advantages, ref_logp, weights):
+        made = PolicyLoss(*_untracked("policy_loss", tuple(made), tuple(t for t in (logits, old_logp, advantages, ref_logp, weights) if t is not None)))
+    return made
+
+
+def policy_loss_gradient(logits, targets, old_logp, advantages, *, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_weight=0.0, d_loss=None, out=None):
+    """(policy_loss, gradient of the logits) in one call.  `d_loss`: None (1), or the loss's gradient, a float32 tensor of one element (a loss
+    scale).  `out`: None, or where the gradient goes, which may be the logits themselves."""
+    if out is logits and _flat_rows(logits) is None:
+        raise ValueError("out: logits of rows that lie evenly expected")
+    a, z, keep, made, workspace = _policy_args(logits, targets, old_logp, advantages, ref_logp, weights, clip, kl_weight)
+    if d_loss is not None:
+        _one_float(d_loss, "d_loss", z.device)
+    grad, stride = _gradient_of(z, out)
+    _call(z.device, "ace_policy_loss_gradient", a, _pointer(d_loss), *map(_pointer, (made.loss, made.logp, made.stats, made.d_logp, grad)), stride, workspace.data_ptr(),
+          workspace.numel() * 8)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+    return made, grad
+
+
+# ---- the norm of many gradients, and clipping ----------------------------------------------------------------------------------
+class GradientNorm(NamedTuple):
+    """`norm` of all gradients and `scale`, the factor for them (float32 [1], as AdamW.step's grad_scale takes it); `norms`: each tensor's."""
+    norm: torch.Tensor
+    scale: torch.Tensor
+    norms: torch.Tensor
+
+
+def _one_float(t, what, device):
+    _on_gpu(t, what)
+    if t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+        raise ValueError(f"{what}: one float32 on {device} expected")
+
+
+def _dense(t):
+    """Whether a tensor's elements lie one after the other in memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    size = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if s != size:
+            return False
+        size *= n
+    return True
+
+
+def _gradients(grads, in_place):
+    """(the tensors, ace_gradient_t for each as 64-bit numbers)"""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("no gradients")
+    flat, index = [], None
+    for i, g in enumerate(grads):
+        if not (isinstance(g, torch.Tensor) and g.is_cuda):
+            _on_gpu(g, f"grads[{i}]")
+        kind = _TYPES.get(g.dtype)
+        if kind is None:
+            raise TypeError(f"grads[{i}]: float32, bfloat16 or float16 expected, not {g.dtype}")
+        if index is None:
+            index = g.get_device()
+        elif g.get_device() != index:
+            raise ValueError(f"grads[{i}] is on {g.device}, grads[0] on {grads[0].device}")
+        if not _dense(g):
+            if in_place:
+                raise ValueError(f"grads[{i}]: elements that lie one after the other expected, got strides {g.stride()} for {tuple(g.shape)}")
+            g = grads[i] = g.contiguous()
+        flat += g.data_ptr(), g.numel(), kind
+    return grads, array.array("q", flat)
+
+
+def _norm_of(grads, table, max_norm, grad_scale):
+    if max_norm is not None and not max_norm > 0:
+        raise ValueError(f"max_norm: None or a positive number expected, got {max_norm}")
+    device, n, at = grads[0].device, len(grads), table.buffer_info()[0]
+    if grad_scale is not None:
+        _one_float(grad_scale, "grad_scale", device)
+    made = torch.empty(2 + n, dtype=torch.float32, device=device)
+    lib = load_library()
+    size = lib.ace_gradient_norm_workspace_bytes(at, n)
+    workspace = torch.empty(max(size, 8) // 8, dtype=torch.float64, device=device)
+    result = made.data_ptr()
+    limit = 0.0 if max_norm is None or max_norm == math.inf else max_norm
+    _call(device, "ace_gradient_norm", at, n, limit, _pointer(grad_scale), result, result + 8, workspace.data_ptr(), size)
+    return GradientNorm(made[0:1], made[1:2], made[2:])
+
+
+def gradient_norm(grads, *, max_norm=None, grad_scale=None) -> GradientNorm:
+    """The norm of many gradients as one vector, and the factor that brings it down to `max_norm`:
+
+        norm = |s| sqrt(sum of g^2);  scale = s min(1, max_norm / (norm + 1e-6))
+
+    `grads`: float32, bfloat16 and float16 tensors of one device, in any mixture and of any size.  s: `grad_scale`, None (1) or a float32 tensor of
+    one element (the inverse of a loss scale).  `max_norm` None: no limit.  Squares and sums are taken in 64 bits and in an order that the sizes
+    alone decide: nothing overflows, and the same call gives the same bits.  A norm that is not finite is returned as it is; with a limit, an
+    infinite one makes `scale` 0, one that is no number makes it none.  Nothing waits: AdamW.step takes `scale` where it lies."""
+    given = list(grads)
+    grads, table = _gradients(given, False)
+    made = _norm_of(grads, table, max_norm, grad_scale)
+    if _lost(*given):
+        made = GradientNorm(*_untracked("gradient_norm", tuple(made), tuple(given)))
+    return made
+
+
+def clip_gradients(grads, max_norm, *, grad_scale=None) -> GradientNorm:
+    """gradient_norm, and every gradient multiplied with its `scale` in place (nothing is written where that is 1).  The tensors' elements lie one
+    after the other, in whatever order, and no two tensors overlap."""
+    grads, table = _gradients(grads, True)
+    places = sorted((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()) for g in grads if g.numel())
+    if any(end > begin for (_, end), (begin, _) in zip(places, places[1:])):
+        raise ValueError("grads: two of them overlap")
+    r = _norm_of(grads, table, max_norm, grad_scale)
+    _call(grads[0].device, "ace_gradient_scale", table.buffer_info()[0], len(grads), r.scale.data_ptr())
+    torch.autograd.graph.increment_version(grads)
+    return r
 
 
 # ---- AdamW over many tensors ------------------------------------------------------------------------------------------------
