@@ -87,6 +87,38 @@ size_t ace_attend_backward_workspace_bytes(const ace_attend_t *a);
 int ace_attend_backward(const ace_attend_t *a, const void *d_gout, const int64_t gout_stride[3], void *d_dq, void *d_dk, void *d_dv,
                         void *d_workspace, size_t workspace_bytes, void *stream);
 
+/* ---- the same over sequences that lie one after the other ---------------------------------------------------------------
+ * Tokens [tokens][heads][dim]; a sequence is a run of them, and its queries see its own keys only, query i key j where j <= i and
+ * (i - j < window or j < sinks).  Tokens behind the last sequence are of none: out 0, lse -inf, gradients 0.
+ *
+ * A table says where sequences lie and in which order their blocks of ACE_PACKED_BLOCK tokens are worked on, the longest walks first; it is made
+ * once on the host (ace_packing_table) and copied to the device by the caller: first the blocks of queries, `blocks` of them, then those of
+ * keys, then the sequences. */
+#define ACE_PACKED_BLOCK 128
+typedef struct ace_packed_block {
+    int32_t first, tokens;         /* of the sequence */
+    int32_t block;                 /* tokens block * 128 to block * 128 + 127 of it */
+    int32_t sequence;              /* its number, or -1: tokens of none */
+} ace_packed_block_t;
+typedef struct ace_packed_sequence { int32_t first, tokens; } ace_packed_sequence_t;
+typedef struct ace_packing {
+    int32_t tokens, sequences;     /* all tokens, those of no sequence among them; sequences that are not empty */
+    int32_t blocks, longest;
+    const void *d_table;           /* at a multiple of 16 bytes */
+} ace_packing_t;
+
+/* lengths: HOST int64[n], 0 and more, `tokens` at most in all, which is 2^28 at most.  Fills in *p but d_table; table: HOST memory of
+ * table_bytes bytes, or NULL (then only *p is filled in).  The table takes 32 blocks + 8 sequences bytes. */
+int ace_packing_table(const int64_t *lengths, int64_t n, int64_t tokens, ace_packing_t *p, void *table, size_t table_bytes);
+
+/* As ace_attend_forward and ace_attend_backward: batch is 1, queries and keys are all tokens, d_start and d_length NULL; lse is
+ * [heads][tokens].  Up to 2^22 of heads * (blocks + 1), and for gradients of sequences * kv_heads * (blocks of 32 first keys) where a sequence is
+ * longer than the window. */
+int ace_packed_attend_forward(const ace_attend_t *a, const ace_packing_t *p, void *stream);
+size_t ace_packed_attend_backward_workspace_bytes(const ace_attend_t *a, const ace_packing_t *p);
+int ace_packed_attend_backward(const ace_attend_t *a, const ace_packing_t *p, const void *d_gout, const int64_t gout_stride[3], void *d_dq, void *d_dk, void *d_dv,
+                               void *d_workspace, size_t workspace_bytes, void *stream);
+
 /* ---- AdamW over many tensors -------------------------------------------------------------------------------------------
  *     g = grad_scale * grad;  m = m b1 + g (1 - b1);  v = v b2 + g^2 (1 - b2)
  *     p = p decay - m step_size / (sqrt(v) root_scale + eps);  copy = p rounded

@@ -1,0 +1,102 @@
+/*
+ * Attention over sequences that lie one after the other (ace_packed_attend_forward, ace_packed_attend_backward): the kernels of layer_attend.h
+ * over a table of the sequences' blocks, which the host makes once for all the layers that see them (ace_packing_table).
+ *
+ * Nothing is padded: a workgroup takes a block of 128 tokens of one sequence, whichever comes next by the length of its walk, so that what
+ * is dispatched last is short. A sequence's rows are a range of a buffer descriptor: what stands behind them, the next sequence's rows, is
+ * out of range and arrives as zeros.
+ */
+#include <algorithm>
+#include "layer_attend.h"
+
+namespace {
+
+int check(const ace_attend_t *a, const ace_packing_t *p) {
+    if (!p || !a || a->batch != 1 || a->queries != a->keys || a->queries != p->tokens || a->d_start || a->d_length) return ACE_EINVAL;
+    const int rc = check_call(a);
+    if (rc != ACE_OK || p->tokens == 0) return rc;
+    if (p->blocks < 1 || p->sequences < 0 || p->longest < 0 || p->longest > p->tokens || !p->d_table || ((uintptr_t)p->d_table & 15)) return ACE_EINVAL;
+    return (int64_t)a->heads * ((int64_t)p->blocks + 1) > (1 << 22) ? ACE_ETOOBIG : ACE_OK;
+}
+
+Args packed_args(const ace_attend_t *a, const ace_packing_t *p) {
+    Args k = args_of(a);
+    k.batch = p->sequences, k.blocks = p->blocks;
+    k.query_blocks = (const ace_packed_block_t *)p->d_table, k.key_blocks = k.query_blocks + p->blocks;
+    k.sequences = (const ace_packed_sequence_t *)(k.key_blocks + p->blocks);
+    return k;
+}
+
+/* attend_far's part of the arguments: none where no sequence is longer than the window */
+int packed_far(const ace_attend_t *a, const ace_packing_t *p, Args &k) {
+    if (p->longest <= a->window) return ACE_OK;
+    far_of(a, p->sequences, p->longest, p->longest, k);
+    return (int64_t)p->sequences * a->kv_heads * k.far_blocks > (1 << 22) ? ACE_ETOOBIG : ACE_OK;
+}
+
+}  // namespace
+
+extern "C" int ace_packing_table(const int64_t *lengths, int64_t n, int64_t tokens, ace_packing_t *p, void *table, size_t table_bytes) {
+    if (n < 0 || (n > 0 && !lengths) || tokens < 0 || !p) return ACE_EINVAL;
+    if (tokens > MOST) return ACE_ETOOBIG;
+    static_assert(ACE_PACKED_BLOCK == QUERIES, "a workgroup's queries");
+    int64_t used = 0, blocks = 0, longest = 0, sequences = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        if (lengths[i] < 0 || lengths[i] > tokens - used) return ACE_EINVAL;
+        used += lengths[i], blocks += (lengths[i] + QUERIES - 1) / QUERIES, sequences += lengths[i] > 0;
+        longest = lengths[i] > longest ? lengths[i] : longest;
+    }
+    blocks += (tokens - used + QUERIES - 1) / QUERIES;
+    *p = {(int32_t)tokens, (int32_t)sequences, (int32_t)blocks, (int32_t)longest, nullptr};
+    if (!table) return ACE_OK;
+    if (table_bytes < (size_t)blocks * 2 * sizeof(ace_packed_block_t) + (size_t)sequences * sizeof(ace_packed_sequence_t)) return ACE_EINVAL;
+    ace_packed_block_t *q = (ace_packed_block_t *)table, *k = q + blocks, *at = q;
+    ace_packed_sequence_t *s = (ace_packed_sequence_t *)(k + blocks);
+    int32_t first = 0, index = 0;
+    for (int64_t i = 0; i <= n; ++i) {
+        const int32_t length = (int32_t)(i < n ? lengths[i] : tokens - used);
+        for (int32_t b = 0; b * QUERIES < length; ++b) *at++ = {first, length, b, i < n ? index : -1};
+        if (i < n && length > 0) s[index++] = {first, length};
+        first += length;
+    }
+    std::copy(q, k, k);
+    /* the longest walks first: of queries those that have the most keys before them, of keys those that have the most queries behind them */
+    std::sort(q, k, [](const ace_packed_block_t &x, const ace_packed_block_t &y) {
+        if ((x.sequence < 0) != (y.sequence < 0)) return y.sequence < 0;
+        return x.block != y.block ? x.block > y.block : x.first < y.first;
+    });
+    std::sort(k, k + blocks, [](const ace_packed_block_t &x, const ace_packed_block_t &y) {
+        if ((x.sequence < 0) != (y.sequence < 0)) return y.sequence < 0;
+        const int32_t left = x.tokens - x.block * QUERIES, other = y.tokens - y.block * QUERIES;
+        return left != other ? left > other : x.first != y.first ? x.first < y.first : x.block < y.block;
+    });
+    return ACE_OK;
+}
+
+extern "C" int ace_packed_attend_forward(const ace_attend_t *a, const ace_packing_t *p, void *stream) {
+    const int rc = check(a, p);
+    if (rc != ACE_OK || p->tokens == 0) return rc;
+    const Args k = packed_args(a, p);
+    const hipStream_t s = (hipStream_t)stream;
+    if (a->dtype == ACE_T_BF16)
+        return a->dim <= 64 ? forward_blocks<bf16, 64, true>(k, s) : a->dim <= 96 ? forward_blocks<bf16, 96, true>(k, s) : forward_blocks<bf16, 128, true>(k, s);
+    return a->dim <= 64 ? forward_blocks<f16, 64, true>(k, s) : a->dim <= 96 ? forward_blocks<f16, 96, true>(k, s) : forward_blocks<f16, 128, true>(k, s);
+}
+
+extern "C" size_t ace_packed_attend_backward_workspace_bytes(const ace_attend_t *a, const ace_packing_t *p) {
+    Args k = {};
+    return check(a, p) != ACE_OK || p->tokens == 0 || packed_far(a, p, k) != ACE_OK ? 0 : backward_workspace(a, p->sequences, k);
+}
+
+extern "C" int ace_packed_attend_backward(const ace_attend_t *a, const ace_packing_t *p, const void *d_gout, const int64_t gout_stride[3], void *d_dq, void *d_dk,
+                                          void *d_dv, void *d_workspace, size_t workspace_bytes, void *stream) {
+    int rc = check(a, p);
+    if (rc != ACE_OK || p->tokens == 0) return rc;
+    Args k = packed_args(a, p);
+    if ((rc = packed_far(a, p, k)) != ACE_OK) return rc;
+    if (workspace_bytes < backward_workspace(a, p->sequences, k)) return ACE_EINVAL;
+    if ((rc = backward_args(a, d_gout, gout_stride, d_dq, d_dk, d_dv, d_workspace, k)) != ACE_OK) return rc;
+    const hipStream_t s = (hipStream_t)stream;
+    if (a->dtype == ACE_T_BF16) return a->dim <= 64 ? backward<bf16, 64, true>(k, s) : a->dim <= 96 ? backward<bf16, 96, true>(k, s) : backward<bf16, 128, true>(k, s);
+    return a->dim <= 64 ? backward<f16, 64, true>(k, s) : a->dim <= 96 ? backward<f16, 96, true>(k, s) : backward<f16, 128, true>(k, s);
+}

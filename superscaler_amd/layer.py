@@ -5,6 +5,7 @@ whose state bytes the memory model counts:
 
   block_norm, block_norm_backward               norm at a block's exit, gate, scaled residual, norm at the next block's entry
   window_attention, window_attention_backward   causal attention over a window of keys and a few first ones; prompts and single tokens
+  Packing, packed_attention, packed_attention_backward   the same over sequences that lie one after the other
   token_logprobs, token_logprobs_backward       log-probabilities of the tokens that were taken
   policy_loss, policy_loss_gradient             a policy's clipped loss with a term that keeps it near to another one
   gradient_norm, clip_gradients                 the norm of many tensors, and the factor that AdamW.step or clipping in place takes
@@ -35,10 +36,12 @@ _lib = None
 EXPORTS = ["ace_layer_abi_version", "ace_layer_strerror", "ace_layer_last_hip_error", "ace_block_norm_forward", "ace_block_norm_workspace_bytes",
            "ace_block_norm_backward", "ace_attend_workspace_bytes", "ace_attend_forward", "ace_attend_backward_workspace_bytes",
            "ace_attend_backward", "ace_adamw_step", "ace_adamw_moments", "ace_gradient_norm_workspace_bytes", "ace_gradient_norm", "ace_gradient_scale",
-           "ace_token_logprobs", "ace_token_logprobs_backward", "ace_policy_loss_workspace_bytes", "ace_policy_loss", "ace_policy_loss_gradient"]
+           "ace_token_logprobs", "ace_token_logprobs_backward", "ace_policy_loss_workspace_bytes", "ace_policy_loss", "ace_policy_loss_gradient",
+           "ace_packing_table", "ace_packed_attend_forward", "ace_packed_attend_backward_workspace_bytes", "ace_packed_attend_backward"]
 ABI_VERSION = 2
 MAX_WIDTH = 32768       # ACE_NORM_MAX_WIDTH
 MAX_HEAD = 128
+MAX_TOKENS = 1 << 28
 MAX_VOCAB = 1 << 28     # ACE_LOSS_MAX_VOCAB
 ADAMW_BLOCK, ADAMW_CHUNK = 256, 8192
 
@@ -55,7 +58,8 @@ _BLOCK_NORM = struct.Struct("=2q3i2f4x7Q")
 # ace_attend_t: batch, queries, keys, heads, kv_heads, dim, dtype, window, sinks; scale; start and length; four times three strides;
 # q, k, v, out and lse
 _ATTEND = struct.Struct("=9if2Q12q5Q")
-
+# ace_packing_t: tokens, sequences, blocks, longest; table
+_PACKING = struct.Struct("=4iQ")
 # ace_token_loss_t: rows, row_stride; vocab, dtype, target_bits; logits, targets, old, advantage, ref, weight; the ratio's bounds, the term's
 # weight, an even weight of rows
 _TOKEN_LOSS = struct.Struct("=2q3i4x6Q4d")
@@ -79,7 +83,7 @@ def load_library():
     for name in ("ace_layer_strerror", "ace_layer_last_hip_error"):
         getattr(lib, name).restype = ctypes.c_char_p
     for name in ("ace_block_norm_workspace_bytes", "ace_attend_workspace_bytes", "ace_attend_backward_workspace_bytes", "ace_gradient_norm_workspace_bytes",
-                 "ace_policy_loss_workspace_bytes"):
+                 "ace_policy_loss_workspace_bytes", "ace_packed_attend_backward_workspace_bytes"):
         getattr(lib, name).restype = ctypes.c_size_t
     lib.ace_layer_strerror.argtypes = [ctypes.c_int]
     lib.ace_block_norm_forward.argtypes = [_vp] * 5
@@ -91,6 +95,10 @@ def load_library():
     lib.ace_attend_backward.argtypes = [_vp] * 7 + [ctypes.c_size_t, _vp]
     lib.ace_adamw_step.argtypes = [_vp] * 4 + [_f32] * 8 + [_vp]
     lib.ace_adamw_moments.argtypes = [_vp] * 4 + [_i64, _vp, _vp, _vp]
+    lib.ace_packing_table.argtypes = [_vp, _i64, _i64, _vp, _vp, _size]
+    lib.ace_packed_attend_forward.argtypes = [_vp] * 3
+    lib.ace_packed_attend_backward_workspace_bytes.argtypes = [_vp] * 2
+    lib.ace_packed_attend_backward.argtypes = [_vp] * 8 + [_size, _vp]
     lib.ace_gradient_norm_workspace_bytes.argtypes = [_vp, _i64]
     lib.ace_gradient_norm.argtypes = [_vp, _i64, _f64] + [_vp] * 4 + [_size, _vp]
     lib.ace_gradient_scale.argtypes = [_vp, _i64, _vp, _vp]
@@ -383,6 +391,99 @@ def window_attention_backward(d_out, q, k, v, out, lse, *, window=None, sinks=0,
     workspace = q.new_empty(size, dtype=torch.uint8)
     _call(q.device, "ace_attend_backward", a, d_out.data_ptr(), (_i64 * 3)(*d_strides), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), workspace.data_ptr(), size)
     return dq, dk, dv
+
+
+class Packing:
+    """Where sequences of different lengths lie one after the other among `tokens` tokens (by default their sum; those behind the last sequence are
+    of none). Made once on the host for all the layers that see them: `lengths` are numbers, 0 or more, of the host. It holds a table on
+    `device`, some 40 bytes for every 128 tokens and sequence."""
+
+    def __init__(self, lengths, *, tokens=None, device="cuda:0"):
+        if isinstance(lengths, torch.Tensor):
+            if lengths.device.type != "cpu":
+                raise ValueError("lengths: numbers of the host expected (nothing here waits for a GPU)")
+            lengths = lengths.numpy()
+        given = np.asarray(lengths if isinstance(lengths, np.ndarray) else list(lengths))
+        if given.ndim != 1 or (given.size and given.dtype.kind not in "iu"):
+            raise TypeError("lengths: whole numbers in one dimension expected")
+        sizes = np.ascontiguousarray(given, dtype=np.int64)
+        if (sizes < 0).any():
+            raise ValueError("lengths: 0 or more expected")
+        used = sum(map(int, sizes))
+        tokens = used if tokens is None else int(tokens)
+        if not used <= tokens <= MAX_TOKENS:
+            raise ValueError(f"tokens: the {used} of the sequences to {MAX_TOKENS} expected, got {tokens}")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"device: a GPU expected, not {device}")
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
+        self.lengths, self.tokens = tuple(map(int, sizes)), tokens
+        lib, head = load_library(), ctypes.create_string_buffer(_PACKING.size)
+        self._refused(lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, None, 0))
+        _, sequences, blocks, self.longest, _ = _PACKING.unpack(head.raw)
+        table = np.zeros(max(1, blocks * 8 + sequences * 2), dtype=np.int32)
+        self._refused(lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, table.ctypes.data, table.nbytes))
+        self._table = torch.from_numpy(table).to(self.device)
+        self._args = _PACKING.pack(tokens, sequences, blocks, self.longest, self._table.data_ptr())
+
+    @staticmethod
+    def _refused(rc):
+        if rc != 0:
+            raise ValueError(f"ace_packing_table: {load_library().ace_layer_strerror(rc).decode()}")
+
+
+def _packed_args(q, k, v, packing, window, sinks, scale):
+    """As _attend_args, with the tokens as those of one sequence."""
+    if not isinstance(packing, Packing):
+        raise TypeError(f"packing: a Packing expected, not {type(packing).__name__}")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _on_gpu(t, name)
+        if t.dim() != 3:
+            raise ValueError(f"{name}: [tokens, heads, size] expected, got shape {tuple(t.shape)}")
+        if t.shape[0] != packing.tokens or t.device != packing.device:
+            raise ValueError(f"{name}: the {packing.tokens} tokens of the packing on {packing.device} expected, got {t.shape[0]} on {t.device}")
+    q, k, v, head, strides, (_, heads, tokens) = _attend_args(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), window, sinks, scale, None, None)
+    return q, k, v, head, strides, (heads, tokens)
+
+
+def packed_attention(q, k, v, packing, *, window=None, sinks=0, scale=None):
+    """Causal attention over sequences that lie one after the other: (out [tokens, heads, size] of q's type, lse float32 [heads, tokens]).
+
+    q [tokens, heads, size], k and v [tokens, kv_heads, size], bfloat16 or float16, in any strides; consecutive heads // kv_heads heads share a
+    head of keys. Token i of a sequence sees token j of the same one where j <= i and (i - j < window or j < sinks), as in window_attention.
+    Tokens of no sequence have out 0 and lse -inf. Up to 2^28 tokens, and 2^22 of heads * (blocks of 128 tokens of each sequence + 1). What a token
+    does not see, a number or not, does not reach it."""
+    q, k, v, head, strides, rows = _packed_args(q, k, v, packing, window, sinks, scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(rows, dtype=torch.float32, device=q.device)
+    a = _ATTEND.pack(*head, *strides, *out.stride()[:3], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
+    _call(q.device, "ace_packed_attend_forward", a, packing._args)
+    out = out[0]
+    if _lost(q, k, v):
+        out, lse = _untracked("packed_attention", (out, lse), (q, k, v))
+    return out, lse
+
+
+def packed_attention_backward(d_out, q, k, v, out, lse, packing, *, window=None, sinks=0, scale=None):
+    """Gradients (dq, dk, dv) of packed_attention's q, k and v from that of its `out`; `out` and `lse` are what it returned. Those of tokens of no
+    sequence are 0. Up to 2^22 of sequences * kv_heads * (blocks of 32 first keys) where a sequence is longer than the window. The same call gives the
+    same bits."""
+    q, k, v, head, strides, rows = _packed_args(q, k, v, packing, window, sinks, scale)
+    for name, t in (("d_out", d_out), ("out", out)):
+        _on_gpu(t, name)
+        if t.shape != q.shape[1:]:
+            raise ValueError(f"{name}: {tuple(q.shape[1:])} expected, got {tuple(t.shape)}")
+    (d_out, d_strides), (out, out_strides) = _heads(d_out.unsqueeze(0), "d_out", q), _heads(out.unsqueeze(0), "out", q)
+    _on_gpu(lse, "lse")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != rows or not lse.is_contiguous() or lse.device != q.device:
+        raise ValueError("lse: what packed_attention returned expected")
+    a = _ATTEND.pack(*head, *strides, *out_strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
+    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    size = load_library().ace_packed_attend_backward_workspace_bytes(a, packing._args)
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    _call(q.device, "ace_packed_attend_backward", a, packing._args, d_out.data_ptr(), (_i64 * 3)(*d_strides), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+          workspace.data_ptr(), size)
+    return dq[0], dk[0], dv[0]
 
 
 # ---- log-probabilities of taken tokens, and the policy's loss -----------------------------------------------------------------
