@@ -220,6 +220,11 @@ template <int PRODUCTS, int READS, int LEAD> __device__ inline void in_step() {
 struct Tiles {
     int first, at, count;
     __device__ inline int tile(int t) const { return t < first ? t : at + t - first; }
+    /* how many of them begin before key `end` */
+    template <int SIZE> __device__ inline int upto(int end) const {
+        const int last = (end + SIZE - 1) / SIZE, some = first + (last > at ? last - at : 0);
+        return end <= 0 ? 0 : some < count ? some : count;
+    }
 };
 template <int SIZE> __device__ inline Tiles tiles_of(const Args &a, const Sequence &s, int lo, int hi) {
     const int end = s.length < hi + 1 ? s.length : hi + 1;
@@ -293,6 +298,9 @@ __device__ inline int place(int count, int group) {
     const int per = (count + 7) / 8, turn = group / 8, at = group % 8 * per + in_turn(turn, per);
     return turn < per && at < count ? at : count;
 }
+/* Which rows of a block a wavefront takes: the other way round in the second of two workgroups on a CU.  The wavefronts of the first rows see the least,
+ * and wavefronts of one number share a SIMD. */
+__device__ inline int in_pairs(int wave) { return blockIdx.x >> 8 & 1 ? 3 - wave : wave; }
 inline int places(int64_t count) { return (int)((count + 7) / 8 * 8); }
 
 /* PACKED: the table's blocks come with the longest walks first, and a die takes the same blocks of each of its heads, longest first, in turn
@@ -717,7 +725,7 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
     const int head = job.head, queries = span.queries(a);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const Sequence seq = span.sequence(a);
-    const int q0 = job.block * QUERIES, mine = q0 + wave * 32, query = mine + (lane & 31);
+    const int q0 = job.block * QUERIES, mine = q0 + in_pairs(wave) * 32, query = mine + (lane & 31);
     const int last = (q0 + QUERIES < queries ? q0 + QUERIES : queries) - 1;
     const T *k = (const T *)a.k + span.lead(a.k_stride) + head / a.shared * a.k_stride[2], *v = (const T *)a.v + span.lead(a.v_stride) + head / a.shared * a.v_stride[2];
     const Tiles tiles = tiles_of<KEYS>(a, seq, seq.start + q0, seq.start + last);
@@ -750,8 +758,10 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
         if (t < tiles.count) ask(t + 1);
     };
     constexpr int BLOCK = 32 * PITCH * 2;
-    if (tiles.count > 0) {
-        arrive(0);
+    const int own = mine < queries ? tiles.upto<KEYS>(lesser(hi + 1, seq.length)) : 0;   /* (the wavefront sees none of the later ones) */
+    if (tiles.count > 0) arrive(0);
+    int t = 0;
+    if (own > 0) {
         walk.s = walk.scores(0);
         mask(tiles.tile(0) * KEYS);
         walk.softmax();
@@ -766,9 +776,8 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
             walk.step(at + BLOCK, at + TILE + BLOCK);
             mask(key0 + 32);
         };
-        int t = 1;
-        for (; t + 1 < tiles.count; t += 2) middle(t, 2 * TILE), middle(t + 1, 0);
-        if (t < tiles.count) middle(t, 2 * TILE), ++t;
+        for (t = 1; t + 1 < own; t += 2) middle(t, 2 * TILE), middle(t + 1, 0);
+        if (t < own) middle(t, 2 * TILE), ++t;
         arrive(t);
         const uint32_t at = (t & 1) * 2 * TILE + TILE;
         const int key0 = tiles.tile(t - 1) * KEYS;
@@ -778,6 +787,7 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
             walk.weigh(at + BLOCK);
         }
     }
+    while (t < tiles.count) arrive(++t);   /* (its part of the others' tiles) */
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) arrived(walk.o[t]);
     const float total = sum_halves(walk.total);
