@@ -475,6 +475,24 @@ template <class T> __device__ inline void store4(T *to, float a, float b, float 
     *(vec *)to = vec{(T)a, (T)b, (T)c, (T)d};
 }
 
+/* A row's sums as two lanes hold them, times `by`, to `to`: the halves exchange every other four, so that a lane has eight neighbours, 16 bytes, and a
+ * row's two lanes 32. */
+template <class T, int DT> __device__ inline void store_row(T *to, const f32x16 (&sum)[DT], float by, int dim, int half) {
+    typedef T four __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; i += 8) {
+            u32x2 x[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                x[k] = __builtin_bit_cast(u32x2, four{(T)(sum[t][i + 4 * k] * by), (T)(sum[t][i + 4 * k + 1] * by), (T)(sum[t][i + 4 * k + 2] * by), (T)(sum[t][i + 4 * k + 3] * by)});
+            const auto a = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false), b = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
+            const int d = t * 32 + 2 * i + 8 * half;
+            if (d < dim) *(u32x4 *)(to + d) = u32x4{a[0], b[0], a[1], b[1]};
+        }
+}
+
 /* A kernel's arguments and a value as if not known so far: what a rare path computes from these is computed there, and not kept in
  * registers through the loops before it. */
 __device__ inline const Args &args_again() {
@@ -793,15 +811,7 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
     const float total = sum_halves(walk.total);
     const float by = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : total;   /* (nothing visible: zero; not a number: that) */
     T *to = (T *)a.out + span.lead(a.out_stride) + (int64_t)query * a.out_stride[1] + head * a.out_stride[2];
-    auto leave = [&] {
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = t * 32 + result_row(i, half);
-                if (d < a.dim) store4(to + d, walk.o[t][i] * by, walk.o[t][i + 1] * by, walk.o[t][i + 2] * by, walk.o[t][i + 3] * by);
-            }
-    };
+    auto leave = [&] { store_row(to, walk.o, by, a.dim, half); };
     if (query < queries) {
         leave();
         if (half == 0) a.lse[span.values(a, head) + query] = total == 0.0f ? -__builtin_inff() : walk.top * a.scale + __logf(total);
@@ -1101,14 +1111,7 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
         fit.undo(dq, fit.power);
     }
     if (!there) return;
-    T *to = (T *)a.dq + ((span.first_query(a) + query) * a.heads + head) * a.dim;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = t * 32 + result_row(i, half);
-            if (d < a.dim) store4(to + d, dq[t][i] * a.scale, dq[t][i + 1] * a.scale, dq[t][i + 2] * a.scale, dq[t][i + 3] * a.scale);
-        }
+    store_row((T *)a.dq + ((span.first_query(a) + query) * a.heads + head) * a.dim, dq, a.scale, a.dim, half);
 }
 
 /* dK and dV: 32 keys of a key head in a wavefront's registers, 32 queries at a time: S = Q K^T, dP = dO V^T, dV^T += dO^T P,
@@ -1360,16 +1363,9 @@ template <class T, int DP, int SHARE, bool PACKED> __global__ void __launch_boun
                     grads.dk[t][i] += part[d * 32], grads.dv[t][i] += part[(DP + d) * 32];
                 }
     }
-    T *dkrow = (T *)a.dk + ((span.first_key(a) + key) * a.kv_heads + kv) * a.dim, *dvrow = (T *)a.dv + ((span.first_key(a) + key) * a.kv_heads + kv) * a.dim;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = t * 32 + result_row(i, half);
-            if (d >= a.dim) continue;
-            store4(dkrow + d, grads.dk[t][i] * a.scale, grads.dk[t][i + 1] * a.scale, grads.dk[t][i + 2] * a.scale, grads.dk[t][i + 3] * a.scale);
-            store4(dvrow + d, grads.dv[t][i], grads.dv[t][i + 1], grads.dv[t][i + 2], grads.dv[t][i + 3]);
-        }
+    const int64_t row = ((span.first_key(a) + key) * a.kv_heads + kv) * a.dim;
+    store_row((T *)a.dk + row, grads.dk, a.scale, a.dim, half);
+    store_row((T *)a.dv + row, grads.dv, 1.0f, a.dim, half);
 }
 
 /* The first keys and the queries beyond their window: every later query of every head sees those few keys, so the work is split
