@@ -91,8 +91,8 @@ int ace_attend_backward(const ace_attend_t *a, const void *d_gout, const int64_t
  * Tokens [tokens][heads][dim]; a sequence is a run of them, and its queries see its own keys only, query i key j where j <= i and
  * (i - j < window or j < sinks).  Tokens behind the last sequence are of none: out 0, lse -inf, gradients 0.
  *
- * A table says where sequences lie and in which order their blocks of ACE_PACKED_BLOCK tokens are worked on, the longest walks first; it is made
- * once on the host (ace_packing_table) and copied to the device by the caller: first the blocks of queries, `blocks` of them, then those of
+ * A table says where sequences lie and in which order their blocks of ACE_PACKED_BLOCK tokens are worked on, the longest walks first as a rule; it is
+ * made once on the host (ace_packing_table) and copied to the device by the caller: first the blocks of queries, `blocks` of them, then those of
  * keys, then the sequences. */
 #define ACE_PACKED_BLOCK 128
 typedef struct ace_packed_block {

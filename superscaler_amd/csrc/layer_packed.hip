@@ -60,16 +60,22 @@ extern "C" int ace_packing_table(const int64_t *lengths, int64_t n, int64_t toke
         first += length;
     }
     std::copy(q, k, k);
-    /* the longest walks first: of queries those that have the most keys before them, of keys those that have the most queries behind them */
-    std::sort(q, k, [](const ace_packed_block_t &x, const ace_packed_block_t &y) {
-        if ((x.sequence < 0) != (y.sequence < 0)) return y.sequence < 0;
-        return x.block != y.block ? x.block > y.block : x.first < y.first;
-    });
-    std::sort(k, k + blocks, [](const ace_packed_block_t &x, const ace_packed_block_t &y) {
-        if ((x.sequence < 0) != (y.sequence < 0)) return y.sequence < 0;
-        const int32_t left = x.tokens - x.block * QUERIES, other = y.tokens - y.block * QUERIES;
-        return left != other ? left > other : x.first != y.first ? x.first < y.first : x.block < y.block;
-    });
+    /* Walks from the longest to the shortest, so that what is dispatched last is short: of queries the longest are those that have the most keys before
+     * them, of keys those that have the most queries behind them.  But blocks of one sequence whose walks differ by a few blocks stay together, for they
+     * read the same rows, which a die's cache holds for as long as that.  Strictly by their walks, by runs of 3 (keys: of 2) and by sequences, forward and
+     * backward: 16,384 tokens in 24 sequences, 40 heads: 299 and 975, 285 and 972, 280 and 947 us; in 128, 16 heads: 64 and 256, 58 and 252, 58 and 249; 8,192
+     * in 12, 16 heads: 51 and 179, 50 and 177, 52 and 192; 16,384 in 8, 16 heads on 4, a window of 1,024: 132 and 502, 133 and 497, 138 and 508. */
+    const auto order = [](const bool keys, const int run) {
+        return [keys, run](const ace_packed_block_t &x, const ace_packed_block_t &y) {
+            if ((x.sequence < 0) != (y.sequence < 0)) return y.sequence < 0;
+            const int walk_x = keys ? (x.tokens - 1) / QUERIES - x.block : x.block, walk_y = keys ? (y.tokens - 1) / QUERIES - y.block : y.block;
+            if (walk_x / run != walk_y / run) return walk_x > walk_y;
+            if (x.first != y.first) return x.tokens != y.tokens ? x.tokens > y.tokens : x.first < y.first;
+            return walk_x > walk_y;
+        };
+    };
+    std::sort(q, k, order(false, 3));
+    std::sort(k, k + blocks, order(true, 2));
     return ACE_OK;
 }
 

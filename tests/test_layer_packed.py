@@ -58,10 +58,10 @@ def test_the_table_has_every_token_once_and_long_walks_first(lengths, tail):
             assert (first, n) == ((sum(lengths), tail) if s < 0 else (begins[s], some[s])) and 0 <= b * 128 < n
             seen[first + b * 128:first + min(n, b * 128 + 128)] += 1
         assert (seen == 1).all()
-    walks = [0 if s < 0 else b + 1 for _, _, b, s in queries.tolist()]
-    assert walks == sorted(walks, reverse=True)
-    walks = [0 if s < 0 else n - 128 * b for _, n, b, s in keys.tolist()]
-    assert walks == sorted(walks, reverse=True)
+    # long walks first, in runs of blocks of one sequence; tokens of no sequence last
+    for blocks, run, walk in ((queries, 3, lambda n, b: b), (keys, 2, lambda n, b: (n - 1) // 128 - b)):
+        order = [(s < 0, -(walk(n, b) // run), -n, first, -walk(n, b)) for first, n, b, s in blocks.tolist()]
+        assert order == sorted(order)
 
 
 def pack(tokens=300, sequences=2, blocks=4, longest=200, at=host.AT):
