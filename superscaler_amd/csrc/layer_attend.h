@@ -747,22 +747,24 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
     const int last = (q0 + QUERIES < queries ? q0 + QUERIES : queries) - 1;
     const T *k = (const T *)a.k + span.lead(a.k_stride) + head / a.shared * a.k_stride[2], *v = (const T *)a.v + span.lead(a.v_stride) + head / a.shared * a.v_stride[2];
     const Tiles tiles = tiles_of<KEYS>(a, seq, seq.start + q0, seq.start + last);
-    const uint32_t lds0 = lds_offset(lds);
+    /* in LDS: what of the queries' tile is not in the first buffer, and two buffers, which hold the values of a tile and the keys of the tile after it */
+    const uint32_t qtile = lds_offset(lds), lds0 = qtile + QUERIES * PITCH * 2 - TILE;
     const Tile<T, PITCH, KEYS, LANES> ktiles(k, a.k_stride[1], a.dim, threadIdx.x), vtiles(v, a.v_stride[1], a.dim, threadIdx.x);
-    /* a buffer holds a tile's keys and the values of the tile before it: those of two blocks behind */
     auto ask = [&](int t) {
         const uint32_t to = lds0 + (t & 1) * 2 * TILE;
-        if (t < tiles.count) ktiles.ask(to, tiles.tile(t) * KEYS, seq.length);
-        if (t > 0) vtiles.ask(to + TILE, tiles.tile(t - 1) * KEYS, seq.length);
+        if (t < tiles.count) ktiles.ask(to + TILE, tiles.tile(t) * KEYS, seq.length);
+        if (t > 0) vtiles.ask(to, tiles.tile(t - 1) * KEYS, seq.length);
     };
-    if (tiles.count > 0) ask(0);
+    /* the queries, the first keys, and the first values and second keys are on their way together */
+    if (tiles.count > 0) {
+        const T *q = (const T *)a.q + span.lead(a.q_stride) + head * a.q_stride[2];
+        Tile<T, PITCH, QUERIES, LANES>(q, a.q_stride[1], a.dim, threadIdx.x).ask(qtile, q0, queries);
+        ask(0), ask(1);
+    }
     const T *qrow = (const T *)a.q + span.lead(a.q_stride) + (int64_t)query * a.q_stride[1] + head * a.q_stride[2];
     Walk<T, DP, PITCH> walk;
-    walk.start(Operands<T, PITCH>(lane), lds0, a.scale2);
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) walk.qf[s] = global_frag<T>(qrow, s * 16 + half * 8, a.dim, query < queries);
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) arrived(walk.qf[s]);
+    const Operands<T, PITCH> ops(lane);
+    walk.start(ops, lds0, a.scale2);
     const Sight sight(a, seq.length, seq.start + query);
     const int lo = seq.start + mine, hi = seq.start + (mine + 31 < queries ? mine + 31 : queries - 1);
     const Range clear = all_see(a, seq.length, lo, hi), seen = any_see(a, seq.length, lo, hi);
@@ -775,29 +777,35 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
         meet();
         if (t < tiles.count) ask(t + 1);
     };
-    constexpr int BLOCK = 32 * PITCH * 2;
+    constexpr int BLOCK = 32 * PITCH * 2, LOADS = Tile<T, PITCH, KEYS, LANES>::LOADS;
     const int own = mine < queries ? tiles.upto<KEYS>(lesser(hi + 1, seq.length)) : 0;   /* (the wavefront sees none of the later ones) */
-    if (tiles.count > 0) arrive(0);
+    if (tiles.count > 0) {
+        if (tiles.count > 1) wait_tiles<2 * LOADS>();
+        else wait_tiles<LOADS>();
+        meet();
+    }
     int t = 0;
     if (own > 0) {
-        walk.s = walk.scores(0);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) walk.qf[s] = ops.rows(qtile, mine - q0, s);
+        walk.s = walk.scores(TILE);
         mask(tiles.tile(0) * KEYS);
         walk.softmax();
         /* (a tile of first keys is often one block only, and the last tile's blocks are not seen by the first wavefronts) */
-        if (seen.has(tiles.tile(0) * KEYS + 32) || tiles.tile(0) * KEYS + 32 < sinks) walk.s = walk.scores(BLOCK);
+        if (seen.has(tiles.tile(0) * KEYS + 32) || tiles.tile(0) * KEYS + 32 < sinks) walk.s = walk.scores(TILE + BLOCK);
         mask(tiles.tile(0) * KEYS + 32);
         auto middle = [&](int t, uint32_t at) {
             arrive(t);
             const int key0 = tiles.tile(t) * KEYS;
-            walk.step(at, at + TILE);
+            walk.step(at + TILE, at);
             mask(key0);
-            walk.step(at + BLOCK, at + TILE + BLOCK);
+            walk.step(at + TILE + BLOCK, at + BLOCK);
             mask(key0 + 32);
         };
         for (t = 1; t + 1 < own; t += 2) middle(t, 2 * TILE), middle(t + 1, 0);
         if (t < own) middle(t, 2 * TILE), ++t;
         arrive(t);
-        const uint32_t at = (t & 1) * 2 * TILE + TILE;
+        const uint32_t at = (t & 1) * 2 * TILE;
         const int key0 = tiles.tile(t - 1) * KEYS;
         if (seen.has(key0) || key0 < sinks) walk.weigh(at);
         if (seen.has(key0 + 32) || key0 + 32 < sinks) {
@@ -1506,7 +1514,7 @@ template <bool PACKED> uint32_t grid(const Args &k, int heads, int rows, int siz
 }
 
 template <class T, int DP, bool PACKED> int forward_blocks(const Args &k, hipStream_t stream) {
-    constexpr int LDS = 4 * KEYS * Shape<DP>::PITCH * 2;
+    constexpr int LDS = (QUERIES + 3 * KEYS) * Shape<DP>::PITCH * 2;
     const int ready = with_lds<attend_forward<T, DP, PACKED>>(LDS);
     if (ready != ACE_OK) return ready;
     attend_forward<T, DP, PACKED><<<grid<PACKED>(k, k.heads, k.queries, QUERIES), LANES, LDS, stream>>>(k);
