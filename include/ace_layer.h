@@ -91,9 +91,9 @@ int ace_attend_backward(const ace_attend_t *a, const void *d_gout, const int64_t
  * Tokens [tokens][heads][dim]; a sequence is a run of them, and its queries see its own keys only, query i key j where j <= i and
  * (i - j < window or j < sinks).  Tokens behind the last sequence are of none: out 0, lse -inf, gradients 0.
  *
- * A table says where sequences lie and in which order their blocks of ACE_PACKED_BLOCK tokens are worked on, the longest walks first as a rule; it is
- * made once on the host (ace_packing_table) and copied to the device by the caller: first the blocks of queries, `blocks` of them, then those of
- * keys, then the sequences. */
+ * A table says where sequences lie and in which order their blocks of ACE_PACKED_BLOCK tokens are worked on; it is made once on the host
+ * (ace_packing_table) and copied to the device by the caller: the blocks of queries, `blocks` of them, those of keys, both in another order, and the
+ * sequences. */
 #define ACE_PACKED_BLOCK 128
 typedef struct ace_packed_block {
     int32_t first, tokens;         /* of the sequence */
@@ -108,7 +108,7 @@ typedef struct ace_packing {
 } ace_packing_t;
 
 /* lengths: HOST int64[n], 0 and more, `tokens` at most in all, which is 2^28 at most.  Fills in *p but d_table; table: HOST memory of
- * table_bytes bytes, or NULL (then only *p is filled in).  The table takes 32 blocks + 8 sequences bytes. */
+ * table_bytes bytes, or NULL (then only *p is filled in).  The table takes 64 blocks + 8 sequences bytes. */
 int ace_packing_table(const int64_t *lengths, int64_t n, int64_t tokens, ace_packing_t *p, void *table, size_t table_bytes);
 
 /* As ace_attend_forward and ace_attend_backward: batch is 1, queries and keys are all tokens, d_start and d_length NULL; lse is

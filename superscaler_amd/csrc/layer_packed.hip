@@ -19,11 +19,19 @@ int check(const ace_attend_t *a, const ace_packing_t *p) {
     return (int64_t)a->heads * ((int64_t)p->blocks + 1) > (1 << 22) ? ACE_ETOOBIG : ACE_OK;
 }
 
+/* Walks from the longest to the shortest, so that what is dispatched last is short: of queries the longest are those that have the most keys before them,
+ * of keys those that have the most queries behind them.  But blocks of one sequence read the same rows, which a die's cache holds for a while: in
+ * the first order those of them whose walks differ by a few blocks stay together, in the second all of them do, the longest sequence first.  That is for
+ * calls of many workgroups, which end together anyway.  Strictly by their walks, and in the two orders, forward and backward: 16,384 tokens in 24 sequences, 40
+ * heads (5,720 workgroups): 299 and 975, 285 and 972, 280 and 947 us; in 128, 16 heads (3,056): 64 and 256, 58 and 252, 58 and 249; in 8, 16 heads on 4, a window of
+ * 1,024 (2,112): 132 and 502, 133 and 497, 138 and 508; 8,192 in 12, 16 heads (1,088): 51 and 179, 50 and 177, 52 and 192. */
+constexpr int64_t BY_SEQUENCE = 2560;
 Args packed_args(const ace_attend_t *a, const ace_packing_t *p) {
     Args k = args_of(a);
     k.batch = p->sequences, k.blocks = p->blocks;
-    k.query_blocks = (const ace_packed_block_t *)p->d_table, k.key_blocks = k.query_blocks + p->blocks;
-    k.sequences = (const ace_packed_sequence_t *)(k.key_blocks + p->blocks);
+    const ace_packed_block_t *table = (const ace_packed_block_t *)p->d_table;
+    k.sequences = (const ace_packed_sequence_t *)(table + 4 * (int64_t)p->blocks);
+    k.query_blocks = table + ((int64_t)p->blocks * a->heads < BY_SEQUENCE ? 0 : 2 * (int64_t)p->blocks), k.key_blocks = k.query_blocks + p->blocks;
     return k;
 }
 
@@ -49,9 +57,9 @@ extern "C" int ace_packing_table(const int64_t *lengths, int64_t n, int64_t toke
     blocks += (tokens - used + QUERIES - 1) / QUERIES;
     *p = {(int32_t)tokens, (int32_t)sequences, (int32_t)blocks, (int32_t)longest, nullptr};
     if (!table) return ACE_OK;
-    if (table_bytes < (size_t)blocks * 2 * sizeof(ace_packed_block_t) + (size_t)sequences * sizeof(ace_packed_sequence_t)) return ACE_EINVAL;
+    if (table_bytes < (size_t)blocks * 4 * sizeof(ace_packed_block_t) + (size_t)sequences * sizeof(ace_packed_sequence_t)) return ACE_EINVAL;
     ace_packed_block_t *q = (ace_packed_block_t *)table, *k = q + blocks, *at = q;
-    ace_packed_sequence_t *s = (ace_packed_sequence_t *)(k + blocks);
+    ace_packed_sequence_t *s = (ace_packed_sequence_t *)(k + 3 * blocks);
     int32_t first = 0, index = 0;
     for (int64_t i = 0; i <= n; ++i) {
         const int32_t length = (int32_t)(i < n ? lengths[i] : tokens - used);
@@ -59,23 +67,20 @@ extern "C" int ace_packing_table(const int64_t *lengths, int64_t n, int64_t toke
         if (i < n && length > 0) s[index++] = {first, length};
         first += length;
     }
-    std::copy(q, k, k);
-    /* Walks from the longest to the shortest, so that what is dispatched last is short: of queries the longest are those that have the most keys before
-     * them, of keys those that have the most queries behind them.  But blocks of one sequence whose walks differ by a few blocks stay together, for they
-     * read the same rows, which a die's cache holds for as long as that.  Strictly by their walks, by runs of 3 (keys: of 2) and by sequences, forward and
-     * backward: 16,384 tokens in 24 sequences, 40 heads: 299 and 975, 285 and 972, 280 and 947 us; in 128, 16 heads: 64 and 256, 58 and 252, 58 and 249; 8,192
-     * in 12, 16 heads: 51 and 179, 50 and 177, 52 and 192; 16,384 in 8, 16 heads on 4, a window of 1,024: 132 and 502, 133 and 497, 138 and 508. */
+    for (ace_packed_block_t *to = k; to < (ace_packed_block_t *)s; to += blocks) std::copy(q, k, to);
     const auto order = [](const bool keys, const int run) {
         return [keys, run](const ace_packed_block_t &x, const ace_packed_block_t &y) {
             if ((x.sequence < 0) != (y.sequence < 0)) return y.sequence < 0;
             const int walk_x = keys ? (x.tokens - 1) / QUERIES - x.block : x.block, walk_y = keys ? (y.tokens - 1) / QUERIES - y.block : y.block;
-            if (walk_x / run != walk_y / run) return walk_x > walk_y;
+            if (run > 0 && walk_x / run != walk_y / run) return walk_x > walk_y;
             if (x.first != y.first) return x.tokens != y.tokens ? x.tokens > y.tokens : x.first < y.first;
             return walk_x > walk_y;
         };
     };
-    std::sort(q, k, order(false, 3));
+    std::sort(q, q + blocks, order(false, 3));
     std::sort(k, k + blocks, order(true, 2));
+    std::sort(k + blocks, k + 2 * blocks, order(false, 0));
+    std::sort(k + 2 * blocks, k + 3 * blocks, order(true, 0));
     return ACE_OK;
 }
 

@@ -396,7 +396,7 @@ def window_attention_backward(d_out, q, k, v, out, lse, *, window=None, sinks=0,
 class Packing:
     """Where sequences of different lengths lie one after the other among `tokens` tokens (by default their sum; those behind the last sequence are
     of none). Made once on the host for all the layers that see them: `lengths` are numbers, 0 or more, of the host. It holds a table on
-    `device`, some 40 bytes for every 128 tokens and sequence."""
+    `device`, some 72 bytes for every 128 tokens and sequence."""
 
     def __init__(self, lengths, *, tokens=None, device="cuda:0"):
         if isinstance(lengths, torch.Tensor):
@@ -421,7 +421,7 @@ class Packing:
         lib, head = load_library(), ctypes.create_string_buffer(_PACKING.size)
         self._refused(lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, None, 0))
         _, sequences, blocks, self.longest, _ = _PACKING.unpack(head.raw)
-        table = np.zeros(max(1, blocks * 8 + sequences * 2), dtype=np.int32)
+        table = np.zeros(max(1, blocks * 16 + sequences * 2), dtype=np.int32)
         self._refused(lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, table.ctypes.data, table.nbytes))
         self._table = torch.from_numpy(table).to(self.device)
         self._args = _PACKING.pack(tokens, sequences, blocks, self.longest, self._table.data_ptr())

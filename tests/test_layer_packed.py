@@ -34,32 +34,32 @@ def table(lengths, tokens):
     lib, sizes, head = layer.load_library(), np.array(lengths, dtype=np.int64), ctypes.create_string_buffer(layer._PACKING.size)
     assert lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, None, 0) == 0
     t, sequences, blocks, longest, _ = layer._PACKING.unpack(head.raw)
-    out = np.full(blocks * 8 + sequences * 2 + 4, -7, dtype=np.int32)
-    size = blocks * 32 + sequences * 8
+    out = np.full(blocks * 16 + sequences * 2 + 4, -7, dtype=np.int32)
+    size = blocks * 64 + sequences * 8
     if size:
         assert lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, out.ctypes.data, size - 1) == -1
     assert lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, out.ctypes.data, size) == 0
     assert (out[size // 4:] == -7).all()
-    return (t, sequences, blocks, longest), out[:blocks * 4].reshape(-1, 4), out[blocks * 4:blocks * 8].reshape(-1, 4), out[blocks * 8:size // 4].reshape(-1, 2)
+    return (t, sequences, blocks, longest), *out[:blocks * 16].reshape(4, -1, 4), out[blocks * 16:size // 4].reshape(-1, 2)
 
 
 @pytest.mark.parametrize("lengths,tail", [([], 0), ([], 5), ([0, 0], 0), ([1], 0), ([128], 1), ([129, 0, 127, 1, 1000], 300), ([5] * 300, 128),
                                           ([pyrandom.Random(i).randint(0, 900) for i in range(50)], 77)])
 def test_the_table_has_every_token_once_and_long_walks_first(lengths, tail):
     tokens = sum(lengths) + tail
-    head, queries, keys, sequences = table(lengths, tokens)
+    head, queries, keys, queries2, keys2, sequences = table(lengths, tokens)
     some = [n for n in lengths if n]
     assert head[0] == tokens and head[1] == len(some) and head[3] == max(some, default=0)
     begins = np.cumsum([0] + some)[:-1].tolist()
     assert sequences.tolist() == [[a, n] for a, n in zip(begins, some)]
-    for blocks in (queries, keys):
+    for blocks in (queries, keys, queries2, keys2):
         seen = np.zeros(tokens, dtype=int)
         for first, n, b, s in blocks.tolist():
             assert (first, n) == ((sum(lengths), tail) if s < 0 else (begins[s], some[s])) and 0 <= b * 128 < n
             seen[first + b * 128:first + min(n, b * 128 + 128)] += 1
         assert (seen == 1).all()
-    # long walks first, in runs of blocks of one sequence; tokens of no sequence last
-    for blocks, run, walk in ((queries, 3, lambda n, b: b), (keys, 2, lambda n, b: (n - 1) // 128 - b)):
+    # long walks first, in runs of blocks of one sequence or all of them together; tokens of no sequence last
+    for blocks, run, walk in ((queries, 3, lambda n, b: b), (keys, 2, lambda n, b: (n - 1) // 128 - b), (queries2, 1 << 30, lambda n, b: b), (keys2, 1 << 30, lambda n, b: (n - 1) // 128 - b)):
         order = [(s < 0, -(walk(n, b) // run), -n, first, -walk(n, b)) for first, n, b, s in blocks.tolist()]
         assert order == sorted(order)
 
