@@ -1472,15 +1472,15 @@ Args args_of(const ace_attend_t *a) {
     return k;
 }
 
-/* Blocks of 32 first keys, and over how many workgroups the queries beyond their window go: as many as there are CUs, at least four
+/* Blocks of 32 first keys, and over how many workgroups the queries beyond their window go: `workgroups` in all, as many as there are CUs, at least four
  * tiles of queries for a wavefront.  (4 x 40 heads of 2,048 queries, all of the backward pass: 475 us; with two workgroups for every CU
  * 479.  4 heads on 1 of 16,384, a window of 2,048: 344 us in up to 32 parts, 354 in up to 16; 8 on 1 of 32,768, 1,024: 623 and 731.) */
-void far_of(const ace_attend_t *a, int64_t batch, int64_t queries, int64_t keys, Args &k) {
+void far_of(const ace_attend_t *a, int64_t batch, int64_t queries, int64_t keys, int64_t workgroups, Args &k) {
     const int64_t sinks = a->window > 0 ? (a->sinks < keys ? a->sinks : keys) : 0;
     k.far_blocks = (int)((sinks + 31) / 32), k.far_parts = 0;
     if (sinks == 0 || batch == 0 || queries == 0) return;
     const int64_t groups = batch * a->kv_heads * k.far_blocks, tiles = (int64_t)(a->heads / a->kv_heads) * ((queries + 31) / 32);
-    int64_t parts = 256 / groups;
+    int64_t parts = workgroups / groups;
     const int64_t most = (tiles + WAVES * 4 - 1) / (WAVES * 4);
     parts = parts < most ? parts : most;
     k.far_parts = parts < 1 ? 1 : parts > 32 ? 32 : (int)parts;

@@ -82,7 +82,7 @@ extern "C" int ace_attend_forward(const ace_attend_t *a, void *d_workspace, size
 extern "C" size_t ace_attend_backward_workspace_bytes(const ace_attend_t *a) {
     if (check(a) != ACE_OK || a->batch == 0) return 0;
     Args k = {};
-    far_of(a, a->batch, a->queries, a->keys, k);
+    far_of(a, a->batch, a->queries, a->keys, 256, k);
     return backward_workspace(a, a->batch, k);
 }
 
@@ -92,7 +92,7 @@ extern "C" int ace_attend_backward(const ace_attend_t *a, const void *d_gout, co
     if (rc != ACE_OK || a->batch == 0) return rc;
     if (workspace_bytes < ace_attend_backward_workspace_bytes(a)) return ACE_EINVAL;
     Args k = args_of(a);
-    far_of(a, a->batch, a->queries, a->keys, k);
+    far_of(a, a->batch, a->queries, a->keys, 256, k);
     if ((rc = backward_args(a, d_gout, gout_stride, d_dq, d_dk, d_dv, d_workspace, k)) != ACE_OK) return rc;
     const hipStream_t s = (hipStream_t)stream;
     if (a->dtype == ACE_T_BF16) return a->dim <= 64 ? backward<bf16, 64, false>(k, s) : a->dim <= 96 ? backward<bf16, 96, false>(k, s) : backward<bf16, 128, false>(k, s);
