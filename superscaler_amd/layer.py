@@ -49,6 +49,7 @@ _NONE = 3
 _LONGEST = (1 << 31) - 1
 _HALVES = (torch.bfloat16, torch.float16)
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_TARGETS = (torch.int64, torch.int32)
 _vp, _i32, _i64, _f32, _f64, _size = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_size_t
 
 
@@ -321,15 +322,10 @@ def _heads(t, what, like=None):
     return t, (b, n, h)
 
 
-def _attend_args(q, k, v, window, sinks, scale, start, lengths):
-    """(q, k and v as the kernels read them, the arguments' part before the strides, q's, k's and v's strides, (batch, heads, queries))"""
-    q, q_strides = _heads(q, "q")
-    (k, k_strides), (v, v_strides) = _heads(k, "k", q), _heads(v, "v", q)
-    (batch, queries, heads, dim), (_, keys, kv_heads, _) = q.shape, k.shape
+def _attend_head(batch, queries, keys, heads, kv_heads, dim, dtype, window, sinks, scale, start, lengths):
+    """ace_attend_t's part before the strides."""
     if not 8 <= dim <= MAX_HEAD or dim % 8:
         raise ValueError(f"q: heads of a multiple of 8 elements up to {MAX_HEAD} expected, got {dim}")
-    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim:
-        raise ValueError(f"k and v: [{batch}, keys, heads, {dim}] expected, got {tuple(k.shape)} and {tuple(v.shape)}")
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"{heads} heads do not share {kv_heads} heads of keys evenly")
     if window is not None and window < 1 or sinks < 0:
@@ -337,6 +333,17 @@ def _attend_args(q, k, v, window, sinks, scale, start, lengths):
     scale = 1 / math.sqrt(dim) if scale is None else float(scale)
     if not 0 < scale <= 1e30:
         raise ValueError(f"scale: a positive number expected, got {scale}")
+    # (no key is outside of a window of 2^31 - 1)
+    return (batch, queries, keys, heads, kv_heads, dim, _TYPES[dtype], 0 if window is None else min(int(window), _LONGEST), min(int(sinks), _LONGEST), scale, start, lengths)
+
+
+def _attend_args(q, k, v, window, sinks, scale, start, lengths):
+    """(q, k and v as the kernels read them, the arguments' part before the strides, q's, k's and v's strides, (batch, heads, queries))"""
+    q, q_strides = _heads(q, "q")
+    (k, k_strides), (v, v_strides) = _heads(k, "k", q), _heads(v, "v", q)
+    (batch, queries, heads, dim), (_, keys, kv_heads, _) = q.shape, k.shape
+    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim:
+        raise ValueError(f"k and v: [{batch}, keys, heads, {dim}] expected, got {tuple(k.shape)} and {tuple(v.shape)}")
     for name, t in (("start", start), ("lengths", lengths)):
         if t is None:
             continue
@@ -345,9 +352,8 @@ def _attend_args(q, k, v, window, sinks, scale, start, lengths):
             raise TypeError(f"{name}: int32 expected, not {t.dtype}")
         if tuple(t.shape) != (batch,) or t.device != q.device or not t.is_contiguous():
             raise ValueError(f"{name}: [{batch}] on {q.device} expected, got {tuple(t.shape)} on {t.device}")
-    # (no key is outside of a window of 2^31 - 1)
-    head = (batch, queries, keys, heads, kv_heads, dim, _TYPES[q.dtype], 0 if window is None else min(int(window), _LONGEST), min(int(sinks), _LONGEST), scale,
-            0 if start is None else start.data_ptr(), 0 if lengths is None else lengths.data_ptr())
+    head = _attend_head(batch, queries, keys, heads, kv_heads, dim, q.dtype, window, sinks, scale, 0 if start is None else start.data_ptr(),
+                        0 if lengths is None else lengths.data_ptr())
     return q, k, v, head, q_strides + k_strides + v_strides, (batch, heads, queries)
 
 
@@ -432,18 +438,35 @@ class Packing:
             raise ValueError(f"ace_packing_table: {load_library().ace_layer_strerror(rc).decode()}")
 
 
+def _token_heads(t, what, packing, dtype=None):
+    """A [tokens, heads, size] tensor as _heads has it."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 3 and t.device == packing.device and t.shape[0] == packing.tokens and
+            (t.dtype in _HALVES if dtype is None else t.dtype is dtype)):
+        _on_gpu(t, what)
+        if t.dim() != 3:
+            raise ValueError(f"{what}: [tokens, heads, size] expected, got shape {tuple(t.shape)}")
+        if t.dtype not in _HALVES or (dtype is not None and t.dtype != dtype):
+            raise TypeError(f"{what}: {'bfloat16 or float16' if dtype is None else dtype} expected, not {t.dtype}")
+        raise ValueError(f"{what}: the {packing.tokens} tokens of the packing on {packing.device} expected, got {t.shape[0]} on {t.device}")
+    (tokens, heads, size), (n, h, e) = t.shape, t.stride()
+    n, h = n if tokens > 1 else 0, h if heads > 1 else 0
+    if (size > 1 and e != 1) or (n | h) & 7 or n >= 1 << 23 or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        n, h, _ = t.stride()
+    return t, (0, n, h)
+
+
 def _packed_args(q, k, v, packing, window, sinks, scale):
     """As _attend_args, with the tokens as those of one sequence."""
     if not isinstance(packing, Packing):
         raise TypeError(f"packing: a Packing expected, not {type(packing).__name__}")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _on_gpu(t, name)
-        if t.dim() != 3:
-            raise ValueError(f"{name}: [tokens, heads, size] expected, got shape {tuple(t.shape)}")
-        if t.shape[0] != packing.tokens or t.device != packing.device:
-            raise ValueError(f"{name}: the {packing.tokens} tokens of the packing on {packing.device} expected, got {t.shape[0]} on {t.device}")
-    q, k, v, head, strides, (_, heads, tokens) = _attend_args(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), window, sinks, scale, None, None)
-    return q, k, v, head, strides, (heads, tokens)
+    q, q_strides = _token_heads(q, "q", packing)
+    (k, k_strides), (v, v_strides) = _token_heads(k, "k", packing, q.dtype), _token_heads(v, "v", packing, q.dtype)
+    tokens, heads, dim = q.shape
+    if k.shape != v.shape or k.shape[2] != dim:
+        raise ValueError(f"k and v: [{tokens}, heads, {dim}] expected, got {tuple(k.shape)} and {tuple(v.shape)}")
+    head = _attend_head(1, tokens, tokens, heads, k.shape[1], dim, q.dtype, window, sinks, scale, 0, 0)
+    return q, k, v, head, q_strides + k_strides + v_strides, (heads, tokens)
 
 
 def packed_attention(q, k, v, packing, *, window=None, sinks=0, scale=None):
@@ -454,11 +477,9 @@ def packed_attention(q, k, v, packing, *, window=None, sinks=0, scale=None):
     Tokens of no sequence have out 0 and lse -inf. Up to 2^28 tokens, and 2^22 of heads * (blocks of 128 tokens of each sequence + 1). What a token
     does not see, a number or not, does not reach it."""
     q, k, v, head, strides, rows = _packed_args(q, k, v, packing, window, sinks, scale)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(rows, dtype=torch.float32, device=q.device)
-    a = _ATTEND.pack(*head, *strides, *out.stride()[:3], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
+    out, lse = q.new_empty(q.shape), q.new_empty(rows, dtype=torch.float32)
+    a = _ATTEND.pack(*head, *strides, 0, *out.stride()[:2], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
     _call(q.device, "ace_packed_attend_forward", a, packing._args)
-    out = out[0]
     if _lost(q, k, v):
         out, lse = _untracked("packed_attention", (out, lse), (q, k, v))
     return out, lse
@@ -469,21 +490,19 @@ def packed_attention_backward(d_out, q, k, v, out, lse, packing, *, window=None,
     sequence are 0. Up to 2^22 of sequences * kv_heads * (blocks of 32 first keys) where a sequence is longer than the window. The same call gives the
     same bits."""
     q, k, v, head, strides, rows = _packed_args(q, k, v, packing, window, sinks, scale)
-    for name, t in (("d_out", d_out), ("out", out)):
-        _on_gpu(t, name)
-        if t.shape != q.shape[1:]:
-            raise ValueError(f"{name}: {tuple(q.shape[1:])} expected, got {tuple(t.shape)}")
-    (d_out, d_strides), (out, out_strides) = _heads(d_out.unsqueeze(0), "d_out", q), _heads(out.unsqueeze(0), "out", q)
+    (d_out, d_strides), (out, out_strides) = _token_heads(d_out, "d_out", packing, q.dtype), _token_heads(out, "out", packing, q.dtype)
+    if d_out.shape != q.shape or out.shape != q.shape:
+        raise ValueError(f"d_out and out: {tuple(q.shape)} expected, got {tuple(d_out.shape)} and {tuple(out.shape)}")
     _on_gpu(lse, "lse")
     if lse.dtype != torch.float32 or tuple(lse.shape) != rows or not lse.is_contiguous() or lse.device != q.device:
         raise ValueError("lse: what packed_attention returned expected")
     a = _ATTEND.pack(*head, *strides, *out_strides, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     size = load_library().ace_packed_attend_backward_workspace_bytes(a, packing._args)
-    workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+    workspace = q.new_empty(size, dtype=torch.uint8)
     _call(q.device, "ace_packed_attend_backward", a, packing._args, d_out.data_ptr(), (_i64 * 3)(*d_strides), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
           workspace.data_ptr(), size)
-    return dq[0], dk[0], dv[0]
+    return dq, dk, dv
 
 
 # ---- log-probabilities of taken tokens, and the policy's loss -----------------------------------------------------------------
@@ -522,8 +541,8 @@ def _flat_rows(t):
     return step if step >= shape[-1] else None
 
 
-def _token_loss_args(logits, targets, old_logp=None, advantages=None, ref_logp=None, weights=None, bounds=(0.0, 1.0), kl_weight=0.0):
-    """(packed arguments, logits as the kernels read them, the tensors whose addresses the arguments hold)"""
+def _refuse_token_loss(logits, targets, rows):
+    """Says what is wrong with arguments that do not fit together."""
     _on_gpu(logits, "logits")
     _on_gpu(targets, "targets")
     if logits.dtype not in _TYPES:
@@ -532,27 +551,37 @@ def _token_loss_args(logits, targets, old_logp=None, advantages=None, ref_logp=N
         raise ValueError(f"logits: rows of 1 to {MAX_VOCAB} elements expected, got shape {tuple(logits.shape)}")
     if targets.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"targets: int64 or int32 expected, not {targets.dtype}")
-    shape, device = logits.shape[:-1], logits.device
-    if targets.shape != shape or targets.device != device:
-        raise ValueError(f"targets: {tuple(shape)} on {device} expected, got {tuple(targets.shape)} on {targets.device}")
-    rows = [old_logp, advantages, ref_logp, weights]
-    for i, (name, t) in enumerate(zip(("old_logp", "advantages", "ref_logp", "weights"), rows)):
+    shape, device = tuple(logits.shape[:-1]), logits.device
+    if tuple(targets.shape) != shape or targets.device != device:
+        raise ValueError(f"targets: {shape} on {device} expected, got {tuple(targets.shape)} on {targets.device}")
+    for name, t in zip(("old_logp", "advantages", "ref_logp", "weights"), rows):
         if t is None:
             continue
         _on_gpu(t, name)
         if t.dtype != torch.float32:
             raise TypeError(f"{name}: float32 expected, not {t.dtype}")
-        if t.shape != shape or t.device != device:
-            raise ValueError(f"{name}: {tuple(shape)} on {device} expected, got {tuple(t.shape)} on {t.device}")
-        rows[i] = t.contiguous()
-    stride = _flat_rows(logits)
+        if tuple(t.shape) != shape or t.device != device:
+            raise ValueError(f"{name}: {shape} on {device} expected, got {tuple(t.shape)} on {t.device}")
+
+
+def _token_loss_args(logits, targets, *rows, bounds=(0.0, 1.0), kl_weight=0.0):
+    """(packed arguments, logits as the kernels read them, the other tensors whose addresses the arguments hold); `rows`: old_logp, advantages,
+    ref_logp and weights, or none of them"""
+    if not (isinstance(logits, torch.Tensor) and isinstance(targets, torch.Tensor) and logits.is_cuda and logits.dtype in _TYPES and logits.dim() > 0 and
+            1 <= logits.shape[-1] <= MAX_VOCAB and targets.dtype in _TARGETS):
+        _refuse_token_loss(logits, targets, rows)
+    shape, device = targets.shape, logits.device
+    if logits.shape[:-1] != shape or targets.device != device or not all(t is None or _fits(t, torch.float32, device, shape) for t in rows):
+        _refuse_token_loss(logits, targets, rows)
+    vocab, n = logits.shape[-1], targets.numel()
+    stride = vocab if logits.is_contiguous() else _flat_rows(logits)
     if stride is None:
-        logits = logits.contiguous()
-        stride = logits.shape[-1]
-    targets, n = targets.contiguous(), targets.numel()
-    a = _TOKEN_LOSS.pack(n, stride, logits.shape[-1], _TYPES[logits.dtype], 64 if targets.dtype is torch.int64 else 32, logits.data_ptr(), targets.data_ptr(),
-                         *[0 if t is None else t.data_ptr() for t in rows], *bounds, kl_weight, 1 / n if n else 0.0)
-    return a, logits, [targets] + rows
+        logits, stride = logits.contiguous(), vocab
+    keep = [targets.contiguous()] + [None if t is None else t.contiguous() for t in rows]
+    pointers = [0 if t is None else t.data_ptr() for t in keep]
+    a = _TOKEN_LOSS.pack(n, stride, vocab, _TYPES[logits.dtype], 64 if targets.dtype is torch.int64 else 32, logits.data_ptr(), *pointers, *(0,) * (5 - len(pointers)),
+                         *bounds, kl_weight, 1 / n if n else 0.0)
+    return a, logits, keep
 
 
 def _gradient_of(logits, out):
@@ -582,8 +611,8 @@ def token_logprobs(logits, targets) -> TokenLogprobs:
     logits [..., vocab] float32, bfloat16 or float16, targets [...] int64 or int32.  A target that is not in [0, vocab) stands for none (a
     token of the prompt, a padded place): its logp is 0, and its logits may be anything.  Logits of -inf are tokens that cannot be taken."""
     a, z, keep = _token_loss_args(logits, targets)
-    logp = torch.empty(targets.shape, dtype=torch.float32, device=z.device)
-    stats = torch.empty(targets.shape + (2,), dtype=torch.float32, device=z.device)
+    shape = targets.shape
+    logp, stats = z.new_empty(shape, dtype=torch.float32), z.new_empty((*shape, 2), dtype=torch.float32)
     _call(z.device, "ace_token_logprobs", a, logp.data_ptr(), stats.data_ptr())
     if _lost(logits):
         logp, stats = _untracked("token_logprobs", (logp, stats), (logits,))
@@ -596,12 +625,18 @@ def token_logprobs_backward(d_logp, logits, targets, stats, *, out=None):
     `out`: None, or where the gradient goes, which may be the logits themselves."""
     if out is logits and _flat_rows(logits) is None:
         raise ValueError("out: logits of rows that lie evenly expected")
-    a, z, keep = _token_loss_args(logits, targets, d_logp)
+    a, z, keep = _token_loss_args(logits, targets)
+    _on_gpu(d_logp, "d_logp")
+    if d_logp.dtype != torch.float32:
+        raise TypeError(f"d_logp: float32 expected, not {d_logp.dtype}")
+    if d_logp.shape != targets.shape or d_logp.device != z.device:
+        raise ValueError(f"d_logp: {tuple(targets.shape)} on {z.device} expected, got {tuple(d_logp.shape)} on {d_logp.device}")
+    d_logp = d_logp.contiguous()
     _on_gpu(stats, "stats")
     if stats.dtype != torch.float32 or stats.shape != targets.shape + (2,) or not stats.is_contiguous() or stats.device != z.device:
         raise ValueError("stats: what token_logprobs returned expected")
     grad, stride = _gradient_of(z, out)
-    _call(z.device, "ace_token_logprobs_backward", a, keep[1].data_ptr(), stats.data_ptr(), grad.data_ptr(), stride)
+    _call(z.device, "ace_token_logprobs_backward", a, d_logp.data_ptr(), stats.data_ptr(), grad.data_ptr(), stride)
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return grad
@@ -616,9 +651,10 @@ def _policy_args(logits, targets, old_logp, advantages, ref_logp, weights, clip,
     for name, t in (("old_logp", old_logp), ("advantages", advantages)):
         if t is None:
             raise TypeError(f"{name}: a tensor expected")
-    a, z, keep = _token_loss_args(logits, targets, old_logp, advantages, ref_logp, weights, (1 - low, 1 + high), kl_weight)
-    made = PolicyLoss(*(torch.empty(size, dtype=torch.float32, device=z.device) for size in ((), targets.shape, targets.shape + (2,), targets.shape)))
-    return a, z, keep, made, torch.empty(targets.numel(), dtype=torch.float64, device=z.device)
+    a, z, keep = _token_loss_args(logits, targets, old_logp, advantages, ref_logp, weights, bounds=(1 - low, 1 + high), kl_weight=kl_weight)
+    like = keep[1]      # (contiguous: so is what is made like it)
+    made = PolicyLoss(like.new_empty(()), torch.empty_like(like), like.new_empty((*like.shape, 2)), torch.empty_like(like))
+    return a, z, keep, made, like.new_empty(like.shape, dtype=torch.float64)
 
 
 def policy_loss(logits, targets, old_logp, advantages, *, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_weight=0.0) -> PolicyLoss:
@@ -672,7 +708,7 @@ def _one_float(t, what, device):
 def _dense(t):
     """Whether a tensor's elements lie one after the other in memory, in whatever order."""
     if t.is_contiguous():
-        return True
+        return True      # (an empty one too)
     size = 1
     for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
         if s != size:
@@ -686,22 +722,23 @@ def _gradients(grads, in_place):
     grads = list(grads)
     if not grads:
         raise ValueError("no gradients")
-    flat, index = [], None
+    try:
+        if all([g.is_contiguous() for g in grads]) and {g.get_device() for g in grads} == {grads[0].device.index}:
+            return grads, array.array("q", [v for g in grads for v in (g.data_ptr(), g.numel(), _TYPES[g.dtype])])
+    except (AttributeError, KeyError):
+        pass
+    flat = []
     for i, g in enumerate(grads):
-        if not (isinstance(g, torch.Tensor) and g.is_cuda):
-            _on_gpu(g, f"grads[{i}]")
-        kind = _TYPES.get(g.dtype)
-        if kind is None:
+        _on_gpu(g, f"grads[{i}]")
+        if g.dtype not in _TYPES:
             raise TypeError(f"grads[{i}]: float32, bfloat16 or float16 expected, not {g.dtype}")
-        if index is None:
-            index = g.get_device()
-        elif g.get_device() != index:
+        if g.device != grads[0].device:
             raise ValueError(f"grads[{i}] is on {g.device}, grads[0] on {grads[0].device}")
         if not _dense(g):
             if in_place:
                 raise ValueError(f"grads[{i}]: elements that lie one after the other expected, got strides {g.stride()} for {tuple(g.shape)}")
             g = grads[i] = g.contiguous()
-        flat += g.data_ptr(), g.numel(), kind
+        flat += g.data_ptr(), g.numel(), _TYPES[g.dtype]
     return grads, array.array("q", flat)
 
 
@@ -711,14 +748,13 @@ def _norm_of(grads, table, max_norm, grad_scale):
     device, n, at = grads[0].device, len(grads), table.buffer_info()[0]
     if grad_scale is not None:
         _one_float(grad_scale, "grad_scale", device)
-    made = torch.empty(2 + n, dtype=torch.float32, device=device)
-    lib = load_library()
-    size = lib.ace_gradient_norm_workspace_bytes(at, n)
-    workspace = torch.empty(max(size, 8) // 8, dtype=torch.float64, device=device)
+    made = grads[0].new_empty((2 + n,), dtype=torch.float32)
+    size = load_library().ace_gradient_norm_workspace_bytes(at, n)
+    workspace = made.new_empty((size // 8,), dtype=torch.float64)
     result = made.data_ptr()
     limit = 0.0 if max_norm is None or max_norm == math.inf else max_norm
     _call(device, "ace_gradient_norm", at, n, limit, _pointer(grad_scale), result, result + 8, workspace.data_ptr(), size)
-    return GradientNorm(made[0:1], made[1:2], made[2:])
+    return GradientNorm(*made.split_with_sizes((1, 1, n)))
 
 
 def gradient_norm(grads, *, max_norm=None, grad_scale=None) -> GradientNorm:
