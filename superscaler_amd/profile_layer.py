@@ -7,6 +7,9 @@ tensor-parallel degree of the workload: products by the matrix library, norms wi
 The times go into a database of the form that ProfileDB.from_directory loads; seeded plans are scored with it twice, with the
 optimizer's moments in 32 bits and in 8.  `--steps` trains the layer for that many steps with both, as a check that what was
 timed works together.  Collectives and bandwidths between GPUs cannot be taken on one card: they are those of the synthetic database.
+`--documents` fills every row of tokens with so many documents of different lengths, one after the other, whose tokens do not see each other's;
+`--loss` measures the output layer with the log-probabilities of its targets, forward and backward; `--clip` clips the gradients' norm in `--steps`.
+`--policy-steps` trains a layer with an output layer as a policy: packed documents, the clipped loss on what it took, gradients clipped to `--clip` or 1.
 Where only some sizes and degrees are measured, the others are the synthetic database's, too: the line names them and no best plan.
 Prints one JSON line; `--out` writes the database as files, and beside them which of them were measured.
 
@@ -59,13 +62,17 @@ class GptLayer:
     def _norm(self, name):
         return dict(entry_weight=self.params[name], entry_bias=self.params[name + "_bias"], kind="layer")
 
-    def forward(self, x, block):
+    def forward(self, x, block, packing=None):
+        """`packing`: None (a sequence in every row of x), or where sequences lie among x's tokens."""
         p, s = self.params, {"x": x, "block": block}
+        if packing is not None:
+            s["packing"] = packing
         s["r1"], s["y1"], s["st1"] = layer.block_norm(x, block, **self._norm("norm1"))
         qkv = (s["y1"] @ p["qkv"]).unflatten(-1, (3, self.heads, HEAD))
-        s["q"], s["k"], s["v"] = qkv.unbind(2)
-        s["o"], s["lse"] = layer.window_attention(s["q"], s["k"], s["v"], window=self.window, sinks=self.sinks)
-        s["a"] = s["o"].flatten(2) @ p["dense"]
+        s["q"], s["k"], s["v"] = qkv.unbind(-3) if packing is None else (t.flatten(0, -3) for t in qkv.unbind(-3))
+        how = dict(window=self.window, sinks=self.sinks)
+        s["o"], s["lse"] = layer.window_attention(s["q"], s["k"], s["v"], **how) if packing is None else layer.packed_attention(s["q"], s["k"], s["v"], packing, **how)
+        s["a"] = (s["o"].flatten(-2) @ p["dense"]).view_as(x)
         s["r2"], s["y2"], s["st2"] = layer.block_norm(s["r1"], s["a"], **self._norm("norm2"))
         s["u"] = s["y2"] @ p["up"]
         s["g"] = torch.nn.functional.gelu(s["u"])
@@ -85,30 +92,87 @@ class GptLayer:
             return g.x, g.block
         d = torch.ops.aten.gelu_backward(product("down", s["g"], d_block), s["u"])
         d_r1, d_a = norm("norm2", d_residual, product("up", s["y2"], d), s["r1"], s["a"], s["st2"])
-        d_o = product("dense", s["o"].flatten(2), d_a).view_as(s["o"])
-        dqkv = layer.window_attention_backward(d_o, s["q"], s["k"], s["v"], s["o"], s["lse"], window=self.window, sinks=self.sinks)
-        d_x, d_in = norm("norm1", d_r1, product("qkv", s["y1"], torch.stack(dqkv, 2).flatten(2)), s["x"], s["block"], s["st1"])
+        d_o = product("dense", s["o"].flatten(-2), d_a).view_as(s["o"])
+        tensors, how = (d_o, s["q"], s["k"], s["v"], s["o"], s["lse"]), dict(window=self.window, sinks=self.sinks)
+        dqkv = layer.window_attention_backward(*tensors, **how) if "packing" not in s else layer.packed_attention_backward(*tensors, s["packing"], **how)
+        d_x, d_in = norm("norm1", d_r1, product("qkv", s["y1"], torch.stack(dqkv, -3).flatten(-3)).view_as(s["x"]), s["x"], s["block"], s["st1"])
         return d_x, d_in, grads
 
 
-def train(hidden, seq, batch, steps, state_bits, window=None, sinks=0, device="cuda:0"):
-    """A layer trained to make its output rows what another layer's are: the losses, step by step."""
+def cut(rows, seq, documents, seed=0):
+    """Lengths of documents that fill `rows` rows of `seq` tokens, `documents` in each, cut at random places."""
+    rng = np.random.Generator(np.random.PCG64(seed))
+    return [int(n) for _ in range(rows) for n in np.diff(np.concatenate([[0], np.sort(rng.integers(0, seq + 1, documents - 1)), [seq]]))]
+
+
+def train(hidden, seq, batch, steps, state_bits, window=None, sinks=0, device="cuda:0", documents=0, clip=None):
+    """A layer trained to make its output rows what another layer's are: the losses, step by step.  `documents`: how many fill a row, one
+    after the other (0: the row is one sequence); `clip`: the gradients' largest norm."""
     net, goal = (GptLayer(hidden, 1, window, sinks, device, seed) for seed in (1, 2))
+    packing = layer.Packing(cut(batch, seq, documents), device=device) if documents else None
     names = list(net.params)
     main = [net.params[n].float() for n in names]
     opt = layer.AdamW(main, copies=[net.params[n] for n in names], state_bits=state_bits)
     gen = torch.Generator(device=device).manual_seed(3)
     x, block = (torch.randn(batch, seq, hidden, device=device, generator=gen).bfloat16() for _ in range(2))
-    want = sum(goal.forward(x, block)[:2]).float()
+    want = sum(goal.forward(x, block, packing)[:2]).float()
     losses = []
     for t in range(1, steps + 1):
-        r, b, saved = net.forward(x, block)
+        r, b, saved = net.forward(x, block, packing)
         off = r.float() + b.float() - want
         losses.append(off.square().mean())
         d = (off * (2 / off.numel())).bfloat16()
         grads = net.backward(d, d, saved)[2]
-        opt.step([grads[n] for n in names], lr=1e-3, betas=(0.9, 0.95), step=t)
+        grads = [grads[n] for n in names]
+        opt.step(grads, lr=1e-3, betas=(0.9, 0.95), step=t, grad_scale=layer.gradient_norm(grads, max_norm=clip).scale if clip else None)
     return [float(v) for v in losses]
+
+
+class Policy:
+    """A layer and an output layer over `vocab` tokens: packed rows in, logits out."""
+
+    def __init__(self, hidden, vocab, window=None, sinks=0, device="cuda:0", seed=0):
+        self.net = GptLayer(hidden, 1, window, sinks, device, seed)
+        gen = torch.Generator(device=device).manual_seed(seed + 1)
+        self.params = dict(self.net.params, head=torch.randn(hidden, vocab, device=device, generator=gen).mul_(hidden ** -0.5).bfloat16())
+
+    def forward(self, x, block, packing):
+        r, b, saved = self.net.forward(x, block, packing)
+        h = r + b
+        return h @ self.params["head"], (h, saved)
+
+    def backward(self, d_logits, saved):
+        """Gradients of the parameters, by name."""
+        h, saved = saved
+        d = d_logits @ self.params["head"].t()
+        return dict(self.net.backward(d, d, saved)[2], head=h.t() @ d_logits)
+
+
+def train_policy(hidden, vocab, lengths, steps, state_bits=32, clip=1.0, window=None, sinks=0, device="cuda:0", seed=0):
+    """A policy trained on what it took at the start: documents of `lengths` tokens, the first quarter of each a prompt, the rest tokens that it
+    drew, with an advantage each.  (losses, norms of the gradients), step by step."""
+    policy, gen = Policy(hidden, vocab, window, sinks, device, seed), torch.Generator(device=device).manual_seed(seed + 2)
+    packing, tokens = layer.Packing(lengths, device=device), sum(lengths)
+    x, block = (torch.randn(tokens, hidden, device=device, generator=gen).bfloat16() for _ in range(2))
+    prompt = torch.tensor([i < n // 4 for n in lengths for i in range(n)], device=device)
+    logits = policy.forward(x, block, packing)[0]
+    targets = torch.where(prompt, -100, torch.multinomial(logits.float().softmax(-1), 1, generator=gen)[:, 0])
+    before = layer.token_logprobs(logits, targets).logp
+    advantages, weights = torch.randn(tokens, device=device, generator=gen), (~prompt).float() / max(1, int((~prompt).sum()))
+    names = list(policy.params)
+    main = [policy.params[n].float() for n in names]
+    opt = layer.AdamW(main, copies=[policy.params[n] for n in names], state_bits=state_bits)
+    losses, norms = [], []
+    for t in range(1, steps + 1):
+        logits, saved = policy.forward(x, block, packing)
+        r, d_logits = layer.policy_loss_gradient(logits, targets, before, advantages, ref_logp=before, weights=weights, kl_weight=0.05, out=logits)
+        grads = policy.backward(d_logits, saved)
+        grads = [grads[n] for n in names]
+        norm = layer.gradient_norm(grads, max_norm=clip)
+        opt.step(grads, lr=1e-3, betas=(0.9, 0.95), step=t, grad_scale=norm.scale)
+        losses.append(r.loss)
+        norms.append(norm.norm)
+    return [float(v) for v in losses], [float(v) for v in norms]
 
 
 def _time_us(call, reps, device="cuda:0"):
@@ -155,13 +219,15 @@ def _reserved_mb(call, device="cuda:0", left=None):
     return max(0.0, (peak - after) * MB if left is None else (peak - before) * MB - left)
 
 
-def measure(w, micro_batch, tp, window=None, sinks=0, vocab=51200, reps=10, device="cuda:0"):
+def measure(w, micro_batch, tp, window=None, sinks=0, vocab=51200, reps=10, device="cuda:0", documents=0, loss=False):
     """{operator name: (forward us, backward us, reserved forward MB, backward MB)} of a layer's shard of workload `w`, for the rows of
-    opgraph.GPT_TYPES."""
+    opgraph.GPT_TYPES.  `documents`: how many fill a row of tokens (0: it is one sequence); `loss`: the output layer's row has the
+    log-probabilities of its targets, too."""
     net, h, s = GptLayer(w.hidden, tp, window, sinks, device), w.hidden, w.seq
     x = torch.randn(micro_batch, s, h, device=device).bfloat16()
     block, d = torch.randn_like(x), torch.randn_like(x)
-    r2, m, saved = net.forward(x, block)
+    packing = layer.Packing(cut(micro_batch, s, documents), device=device) if documents else None
+    r2, m, saved = net.forward(x, block, packing)
     out = {name: (0.0,) * 4 for name in CONTAINED}
 
     def both(name, forward, backward):
@@ -179,8 +245,11 @@ def measure(w, micro_batch, tp, window=None, sinks=0, vocab=51200, reps=10, devi
     product("enc-attention-qkv", saved["y1"], p["qkv"])
     how = dict(window=window, sinks=sinks)
     q, k, v, o, lse = (saved[n] for n in ("q", "k", "v", "o", "lse"))
-    both("enc-attention-score", lambda: layer.window_attention(q, k, v, **how), lambda: layer.window_attention_backward(o, q, k, v, o, lse, **how))
-    product("enc-attention-dense", saved["o"].flatten(2), p["dense"])
+    if packing is None:
+        both("enc-attention-score", lambda: layer.window_attention(q, k, v, **how), lambda: layer.window_attention_backward(o, q, k, v, o, lse, **how))
+    else:
+        both("enc-attention-score", lambda: layer.packed_attention(q, k, v, packing, **how), lambda: layer.packed_attention_backward(o, q, k, v, o, lse, packing, **how))
+    product("enc-attention-dense", o.flatten(-2), p["dense"])
     product("enc-MLP-GEMM-1", saved["y2"], p["up"])
     both("enc-MLP-gelu", lambda: torch.nn.functional.gelu(saved["u"]), lambda: torch.ops.aten.gelu_backward(saved["g"], saved["u"]))
     product("enc-MLP-GEMM-2", saved["g"], p["down"])
@@ -188,7 +257,17 @@ def measure(w, micro_batch, tp, window=None, sinks=0, vocab=51200, reps=10, devi
     tokens = torch.randint(0, table.shape[0], (micro_batch * s,), device=device)
     rows = d.view(-1, h)
     both("encoder-embedding", lambda: table[tokens], lambda: torch.zeros_like(table).index_add_(0, tokens, rows))
-    product("gpt-post-process", x, table.t())
+    if not loss:
+        product("gpt-post-process", x, table.t())
+        return out
+    a, even = x.flatten(0, -2), torch.full((micro_batch * s,), -1.0 / (micro_batch * s), device=device)
+    logits = a @ table.t()
+    stats = layer.token_logprobs(logits, tokens).stats
+
+    def back():
+        g = layer.token_logprobs_backward(even, logits, tokens, stats)
+        return g @ table, a.t() @ g
+    both("gpt-post-process", lambda: layer.token_logprobs(a @ table.t(), tokens), back)
     return out
 
 
@@ -261,6 +340,10 @@ def main(argv=None):
     ap.add_argument("--reps", type=int, default=10)
     ap.add_argument("--plans", type=int, default=65536)
     ap.add_argument("--steps", type=int, default=0, help="train one layer for this many steps, moments in 32 and in 8 bits")
+    ap.add_argument("--documents", type=int, default=0, help="documents in a row of tokens (default: it is one sequence)")
+    ap.add_argument("--loss", action="store_true", help="measure the output layer with the log-probabilities of its targets")
+    ap.add_argument("--clip", type=float, default=None, help="largest norm of the gradients in training")
+    ap.add_argument("--policy-steps", type=int, default=0, help="train a policy for this many steps")
     ap.add_argument("--out", default=None, help="directory for the database's files")
     args = ap.parse_args(argv)
 
@@ -272,7 +355,9 @@ def main(argv=None):
     for what, asked, there in (("--micro-batches", args.micro_batches, base.mbs_list), ("--tp", args.tp, [t for t in base.tp_list if heads % t == 0])):
         if any(v not in there for v in asked or ()):
             ap.error(f"{what}: of workload {w.name} there are {there}")
-    measured = {(b, tp): measure(w, b, tp, args.window, args.sinks, reps=args.reps)
+    if args.documents < 0 or (args.clip is not None and not args.clip > 0):
+        ap.error("--documents: 0 or more, and --clip: a positive number expected")
+    measured = {(b, tp): measure(w, b, tp, args.window, args.sinks, reps=args.reps, documents=args.documents, loss=args.loss)
                 for b in (args.micro_batches or base.mbs_list) for tp in (args.tp or base.tp_list) if heads % tp == 0}
     db = database(w, graph, measured, base)
     result = {"workload": w.name, "ops": graph.num_ops, "window": args.window, "sinks": args.sinks, "measured": len(measured)}
@@ -289,8 +374,13 @@ def main(argv=None):
                                                     "best_ms": float(best.min()) if np.isfinite(best.min()) else None, "median_peak_mb": float(np.nanmedian(mb))}
         cm.close()
         if args.steps:
-            losses = train(min(w.hidden, 2048), 512, 2, args.steps, bits, args.window, args.sinks)
+            losses = train(min(w.hidden, 2048), 512, 2, args.steps, bits, args.window, args.sinks, documents=args.documents, clip=args.clip)
             result[f"losses_with_{bits}_bit_moments"] = [losses[0], losses[-1]]
+    if args.documents:
+        result["documents"] = args.documents
+    if args.policy_steps:
+        losses, norms = train_policy(min(w.hidden, 2048), 51200, cut(2, 512, max(2, args.documents)), args.policy_steps, clip=args.clip or 1.0, window=args.window, sinks=args.sinks)
+        result["policy"] = {"losses": [losses[0], losses[-1]], "gradient_norms": [norms[0], norms[-1]]}
     print(json.dumps(result))
 
 
