@@ -669,8 +669,12 @@ def policy_loss(logits, targets, old_logp, advantages, *, ref_logp=None, weights
     gradient of logits is token_logprobs_backward(d_loss * d_logp, logits, targets, stats), or comes along from policy_loss_gradient."""
     a, z, keep, made, workspace = _policy_args(logits, targets, old_logp, advantages, ref_logp, weights, clip, kl_weight)
     _call(z.device, "ace_policy_loss", a, *map(_pointer, (made.loss, made.logp, made.stats, made.d_logp, workspace)), workspace.numel() * 8)
-    if _lost(logits, old_logp, advantages, ref_logp, weights):
-        made = PolicyLoss(*_untracked("policy_loss", tuple(made), tuple(t for t in (logits, old_logp, advantages, ref_logp, weights) if t is not None)))
+    return _policy_result("policy_loss", made, logits, old_logp, advantages, ref_logp, weights)
+
+
+def _policy_result(name, made, *inputs):
+    if _lost(*inputs):
+        made = PolicyLoss(*_untracked(name, tuple(made), inputs))
     return made
 
 
@@ -686,6 +690,7 @@ def policy_loss_gradient(logits, targets, old_logp, advantages, *, ref_logp=None
     grad, stride = _gradient_of(z, out)
     _call(z.device, "ace_policy_loss_gradient", a, _pointer(d_loss), *map(_pointer, (made.loss, made.logp, made.stats, made.d_logp, grad)), stride, workspace.data_ptr(),
           workspace.numel() * 8)
+    made = _policy_result("policy_loss", made, logits, old_logp, advantages, ref_logp, weights)
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return made, grad

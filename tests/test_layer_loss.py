@@ -209,6 +209,33 @@ def test_rows_of_other_strides_and_places(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("vocab", [5, 64, 1001, 20003])
+def test_the_policy_s_gradient_goes_anywhere(dtype, vocab):
+    """Rows of logits and of their gradient that begin at any element, as far from 16 bytes as there are; into the logits; what is beside them stays.  Where a
+    row's pieces begin, other lanes add up other elements: results differ by what the sums' order gives."""
+    device = cuda_or_skip()
+    z, t, c = policy_case(vocab, 9, vocab, dtype)
+    given = (t.to(device), c["old_logp"].to(device), c["advantages"].to(device))
+    how = dict(ref_logp=c["ref_logp"].to(device), weights=c["weights"].to(device), kl_weight=0.1)
+    want, grad = layer.policy_loss_gradient(z.to(device), *given, **how)
+    bound = 2 * logp_bound(z)
+    for at in range(0, 9):
+        wide = torch.full((9, vocab + 19), 5.0, dtype=dtype, device=device)
+        view = wide[:, at:at + vocab]
+        view.copy_(z)
+        out = torch.full((9, vocab + 13), 7.0, dtype=dtype, device=device)
+        got, g = layer.policy_loss_gradient(view, *given, **how, out=out[:, 9 - at:9 - at + vocab])
+        close(got.logp, want.logp.double(), torch.full((9,), bound))
+        # (both are rounded, and their derivatives are as far apart as ratios of these log-probabilities)
+        close(g, grad.double(), (grad.double().abs().amax(-1, keepdim=True) * (8 * bound) + grad.double().abs() * UNIT[dtype]).cpu() + 2 * SMALLEST[dtype])
+        assert (out[:, :9 - at] == 7).all() and (out[:, 9 - at + vocab:] == 7).all() and (wide[:, :at] == 5).all() and (wide[:, at + vocab:] == 5).all()
+        inside, same = layer.policy_loss_gradient(view, *given, **how, out=view)
+        assert torch.equal(view, g) and torch.equal(inside.loss, got.loss) and same is view
+        assert (wide[:, :at] == 5).all() and (wide[:, at + vocab:] == 5).all()
+
+
+@gpu
 def test_refused_on_the_gpu():
     device = cuda_or_skip()
     z, t = (x.to(device) for x in case(3, 6, 64, F32))
@@ -408,6 +435,8 @@ def test_automatic_differentiation_is_told():
         layer.token_logprobs(z, t).logp.sum().backward()
     with pytest.raises(AceError):
         layer.policy_loss(z, t, f, f).loss.backward()
+    with pytest.raises(AceError):
+        layer.policy_loss_gradient(z, t, f, f)[0].loss.backward()
     with torch.no_grad():
         assert not layer.policy_loss(z, t, f, f).loss.requires_grad
     x = z.detach().clone()
