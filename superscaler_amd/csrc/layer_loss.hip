@@ -92,41 +92,6 @@ template <int LANES> __device__ inline Row join(float top, float total, float *t
     return r;
 }
 
-/* A row per workgroup, 32 elements per lane and pass. */
-template <class T, int LANES, bool POLICY> __global__ void __launch_bounds__(LANES) loss_rows(const Loss a) {
-    __shared__ float tops[LANES / 64];
-    __shared__ double sums[LANES / 64];
-    const float inf = __builtin_inff();
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T *z = (const T *)a.logits + row * a.stride;
-        const int64_t target = target_of(a, row);
-        if (!there(a, target)) {
-            if (threadIdx.x == 0) settle_none<POLICY>(a, row);
-            continue;
-        }
-        const float taken = (float)z[target];
-        float top = -inf, total = 0.0f;
-        constexpr int PASS = LANES * 8 * 4;
-        for (int at = threadIdx.x * 8; at < a.vocab; at += PASS) {
-            float x[32], most = -inf;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int from = at + k * LANES * 8, left = a.vocab - from;
-                const vec8<T> v = left > 0 ? load_some(z + from, left) : vec8<T>{};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[8 * k + i] = i < left ? (float)v[i] : -inf, most = fmaxf(most, x[8 * k + i]);
-            }
-            if (most > top) total *= power(top - most), top = most;
-            const float base = around(top);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) total += power(x[i] - base);
-        }
-        const Row r = join<LANES>(top, total, tops, sums);
-        if (threadIdx.x == 0) settle<POLICY>(a, row, r, taken);
-        __syncthreads();
-    }
-}
-
 /* (elements stay as they lie in memory: they are converted once more wherever they are used, which takes an operation and no register) */
 template <class V> __device__ inline void keep(V &v) {
     union { V v; uint32_t u[sizeof(V) / 4]; } x;
@@ -259,6 +224,61 @@ template <class T, int LANES, int HELD, int WHAT> __global__ void __launch_bound
     if (lane == layout.owner((int)target, LANES)) to[target] = (T)t.at_target;
 }
 
+/* A row per workgroup, AHEAD pieces for each lane on their way while as many are worked on.  8 rows of 200,000 in bfloat16 19.5 us, 1,225 98, 5.0 TB/s (256 lanes: 22.9 and
+ * 97; 1,024: 20.5 and 121). */
+constexpr int AHEAD = 4;
+template <class T, int LANES, bool POLICY> __global__ void __launch_bounds__(LANES) loss_rows(const Loss a, int64_t first) {
+    __shared__ float tops[LANES / 64];
+    __shared__ double sums[LANES / 64];
+    const float inf = __builtin_inff();
+    const int lane = threadIdx.x;
+    const int64_t row = first + blockIdx.x, target = target_of(a, row);
+    if (!there(a, target)) {
+        if (lane == 0) settle_none<POLICY>(a, row);
+        return;
+    }
+    const T *z = (const T *)a.logits + row * a.stride;
+    const float taken = (float)z[target];
+    const Layout<T> layout(z, a.vocab);
+    const int pieces = layout.pieces;
+    const RowPieces<T, LANES> from(z + layout.before, pieces);
+    auto ask = [&](piece<T> (&v)[AHEAD], int k) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if ((k + i) * LANES + lane < pieces) v[i] = from.get(k + i);
+            else
+#pragma unroll
+                for (int e = 0; e < PIECE<T>; ++e) v[i][e] = (T)-inf;
+        }
+    };
+    float top = lane < layout.rest ? (float)z[layout.edge(lane)] : -inf, total = lane < layout.rest ? power(top - around(top)) : 0.0f;
+    auto use = [&](piece<T> (&v)[AHEAD]) {
+        float most = -inf;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+            for (int e = 0; e < PIECE<T>; ++e) most = fmaxf(most, (float)v[i][e]);
+        if (most > top) total *= power(top - most), top = most;
+        const float base = around(top);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            keep(v[i]);
+#pragma unroll
+            for (int e = 0; e < PIECE<T>; ++e) total += power((float)v[i][e] - base);
+        }
+    };
+    piece<T> x[AHEAD], y[AHEAD];
+    ask(x, 0);
+    for (int k = 0; k * LANES < pieces; k += 2 * AHEAD) {
+        ask(y, k + AHEAD);
+        use(x);
+        ask(x, k + 2 * AHEAD);
+        use(y);
+    }
+    const Row r = join<LANES>(top, total, tops, sums);
+    if (lane == 0) settle<POLICY>(a, row, r, taken);
+}
+
 /* Gradients of a row's logits, from its statistics: BACK_HELD pieces for each of a workgroup's lanes. */
 constexpr int BACK_LANES = 256, BACK_HELD = 4;
 /* (a row that begins anywhere has as many whole pieces or one fewer than one that does not) */
@@ -376,11 +396,13 @@ template <bool POLICY> int forward(const Loss &k, int dtype, hipStream_t s) {
     if (k.rows == 0) return ACE_OK;
     return by_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        int rc;
-        if (held<POLICY ? POLICY_LOSS : LOGPROBS, T>(k, s, &rc)) return rc;
-        if (k.rows < 512) loss_rows<T, 1024, POLICY><<<groups(k.rows), 1024, 0, s>>>(k);
-        else loss_rows<T, 256, POLICY><<<groups(k.rows), 256, 0, s>>>(k);
-        return layer_launched();
+        int rc = ACE_OK;
+        if (held<(POLICY ? POLICY_LOSS : LOGPROBS), T>(k, s, &rc)) return rc;
+        for (int64_t first = 0; first < k.rows && rc == ACE_OK; first += MOST_GROUPS) {
+            loss_rows<T, 512, POLICY><<<groups(k.rows - first), 512, 0, s>>>(k, first);
+            rc = layer_launched();
+        }
+        return rc;
     });
 }
 int backward(const Loss &k, int dtype, bool policy, hipStream_t s) {
