@@ -726,14 +726,15 @@ template <class T, int DP, int PITCH> struct Walk {
 };
 
 /* Prompts: a workgroup takes 128 queries of a head, 32 per wavefront, and walks over its keys in tiles of 64, the next tile on its
- * way while one is worked on; blocks that a wavefront does not see are masked like others, but for the second and the last two
- * (passing over the rest took 1% off where a window is 512 and added 3% where it is 2,048).  Tiles of 32 keys, which leave registers for a third wavefront per SIMD, took 3% off with
- * a window of 512 and added 6% with 2,048.
+ * way while one is worked on, up to the last tile that the wavefront sees; blocks before that which it does not see are masked like others, but for the second
+ * and the last two (passing over the rest took 1% off where a window is 512 and added 3% where it is 2,048).  Tiles of 32 keys, which leave registers for a
+ * third wavefront per SIMD, took 3% off with a window of 512 and added 6% with 2,048.
  *
- * 4 x 40 heads of 2,048 tokens and size 128, a window of 512: 139 us, 545 TFLOP/s of the pairs that are seen; 8 heads of 16,384, 2,048:
- * 140 us, 926 (a large product of the matrix library: 1,250).  The card lowers its clock under this load: on zeros the same calls take
- * 12% and 20% less, the library's product 25%; how operands and softmax are ordered further makes no difference.  A short walk pays for
- * its first loads and last stores as well, some 5 us of 27.  LDS has no conflicts and is at work for less than a quarter of the time. */
+ * 4 x 40 heads of 2,048 tokens and size 128, a window of 512: 122 us, 620 TFLOP/s of the pairs that are seen; 8 heads of 16,384, 2,048:
+ * 137 us, 945 (a large product of the matrix library: 1,250).  The card lowers its clock under this load: on zeros long walks take
+ * a third less, the library's product 25%; how operands and softmax are ordered further makes no difference.  Short walks are bound by memory: 128 sequences of 128
+ * tokens, 40 heads, read and write their 674 MB in 126 us; in between, the two take turns: of 1,024 tokens 227 us, 130 of which the bytes alone and 140 the products
+ * alone would take.  LDS has no conflicts and is at work for less than a quarter of the time. */
 template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_forward(const Args a) {
     extern __shared__ char lds[];
     constexpr int PITCH = Shape<DP>::PITCH, TILE = KEYS * PITCH * 2;
