@@ -731,9 +731,9 @@ template <class T, int DP, int PITCH> struct Walk {
  * third wavefront per SIMD, took 3% off with a window of 512 and added 6% with 2,048.
  *
  * 4 x 40 heads of 2,048 tokens and size 128, a window of 512: 122 us, 620 TFLOP/s of the pairs that are seen; 8 heads of 16,384, 2,048:
- * 137 us, 945 (a large product of the matrix library: 1,250).  The card lowers its clock under this load: on zeros long walks take
- * a third less, the library's product 25%; how operands and softmax are ordered further makes no difference.  Short walks are bound by memory: 128 sequences of 128
- * tokens, 40 heads, read and write their 674 MB in 126 us; in between, the two take turns: of 1,024 tokens 227 us, 130 of which the bytes alone and 140 the products
+ * 137 us, 945 (a large product of the matrix library: 1,250), the least of three runs; 143 to 156 and 142 in another process.  The card lowers its clock
+ * under this load: on zeros these take 17 to 23% less, whole prompts of 32,768 31%, the library's product 25%; how operands and softmax are ordered further makes no difference.  Short walks are bound by memory: 128 sequences of 128
+ * tokens, 40 heads, read and write their 674 MB in 126 us; in between, times are near the sum of both: of 1,024 tokens 227 us, 130 of which the bytes alone and 140 the products
  * alone would take.  LDS has no conflicts and is at work for less than a quarter of the time. */
 template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES) RESIDENT(DP) attend_forward(const Args a) {
     extern __shared__ char lds[];
