@@ -130,15 +130,16 @@ template <class T> struct Layout {
     }
 };
 
-/* What lanes need for a row's gradient: d (exp(x - top) / total), taken with an exponential of `less` where the type has 16 bits: an operation fewer,
- * and log2(|d| / total) - top log2 e, rounded, is 2^-20 of a result at most. */
+/* What lanes need for a row's gradient: d (exp(x - top) / total), where the type has 16 bits as an exponential of (x - top) log2 e + more with
+ * more = log2(|d| / total): an operation fewer, and what is rounded on the way, a difference of logits, more and the sum of both, is 2^-24 of at most
+ * some 250, so 2^-16 of a result. (top is taken off before anything is rounded: the gradient of a row does not change with what all its logits share.) */
 struct Told {
-    float d, at_target, top, by, less;
+    float d, at_target, top, by, more;
 };
 template <class T> __device__ inline piece<T> gradients(const Told &t, piece<T> x) {
     piece<T> r;
 #pragma unroll
-    for (int i = 0; i < PIECE<T>; ++i) r[i] = sizeof(T) == 4 ? (T)(power((float)x[i] - t.top) * t.by * -t.d) : (T)__builtin_amdgcn_exp2f(__builtin_fmaf((float)x[i], LOG2E, t.less));
+    for (int i = 0; i < PIECE<T>; ++i) r[i] = sizeof(T) == 4 ? (T)(power((float)x[i] - t.top) * t.by * -t.d) : (T)__builtin_amdgcn_exp2f(__builtin_fmaf((float)x[i] - t.top, LOG2E, t.more));
     return sizeof(T) == 4 ? r : __builtin_bit_cast(piece<T>, __builtin_bit_cast(u32x4, r) ^ (t.d > 0.0f ? 0x80008000u : 0u));
 }
 
@@ -199,9 +200,9 @@ template <class T, int LANES, int HELD, int WHAT> __global__ void __launch_bound
     if (lane == 0) {
         const Settled s = settle<WHAT != LOGPROBS>(a, row, r, taken);
         if (WHAT == POLICY_GRADIENT) {
-                    const float d = s.d * (a.g ? *a.g : 1.0f);
+            const float d = s.d * (a.g ? *a.g : 1.0f);
             told = {d, (float)(-(double)d * expm1(s.logp)), r.top, (float)(1.0 / r.total),
-                    (float)((double)__builtin_amdgcn_logf(__builtin_fabsf(d)) - s.log_total * 1.4426950408889634 - (double)r.top * (double)LOG2E)};
+                    (float)((double)__builtin_amdgcn_logf(__builtin_fabsf(d)) - s.log_total * 1.4426950408889634)};
         }
     }
     if (WHAT != POLICY_GRADIENT) return;
