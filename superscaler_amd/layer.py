@@ -402,7 +402,8 @@ def window_attention_backward(d_out, q, k, v, out, lse, *, window=None, sinks=0,
 class Packing:
     """Where sequences of different lengths lie one after the other among `tokens` tokens (by default their sum; those behind the last sequence are
     of none). Made once on the host for all the layers that see them: `lengths` are numbers, 0 or more, of the host. It holds a table on
-    `device`, some 72 bytes for every 128 tokens and sequence."""
+    `device`, some 72 bytes for every 128 tokens and sequence, which is there until the calls that read it are done, on whatever streams; a graph that one was
+    captured into reads it at every replay, so keep the packing as long as the graph."""
 
     def __init__(self, lengths, *, tokens=None, device="cuda:0"):
         if isinstance(lengths, torch.Tensor):
@@ -429,13 +430,22 @@ class Packing:
         _, sequences, blocks, self.longest, _ = _PACKING.unpack(head.raw)
         table = np.zeros(max(1, blocks * 16 + sequences * 2), dtype=np.int32)
         self._refused(lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, table.ctypes.data, table.nbytes))
-        self._table = torch.from_numpy(table).to(self.device)
+        self._table, self._streams = torch.from_numpy(table).to(self.device), {_raw_stream(self.device.index)}
         self._args = _PACKING.pack(tokens, sequences, blocks, self.longest, self._table.data_ptr())
 
     @staticmethod
     def _refused(rc):
         if rc != 0:
             raise ValueError(f"ace_packing_table: {load_library().ace_layer_strerror(rc).decode()}")
+
+    def _used(self):
+        """What a call on the current stream takes: the table's memory is not given to anything else before that stream's work on it is done."""
+        index = self.device.index
+        stream = _raw_stream(index)
+        if stream not in self._streams:
+            self._table.record_stream(torch.cuda.current_stream(index))
+            self._streams.add(stream)
+        return self._args
 
 
 def _token_heads(t, what, packing, dtype=None):
@@ -479,7 +489,7 @@ def packed_attention(q, k, v, packing, *, window=None, sinks=0, scale=None):
     q, k, v, head, strides, rows = _packed_args(q, k, v, packing, window, sinks, scale)
     out, lse = q.new_empty(q.shape), q.new_empty(rows, dtype=torch.float32)
     a = _ATTEND.pack(*head, *strides, 0, *out.stride()[:2], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr())
-    _call(q.device, "ace_packed_attend_forward", a, packing._args)
+    _call(q.device, "ace_packed_attend_forward", a, packing._used())
     if _lost(q, k, v):
         out, lse = _untracked("packed_attention", (out, lse), (q, k, v))
     return out, lse
@@ -500,7 +510,7 @@ def packed_attention_backward(d_out, q, k, v, out, lse, packing, *, window=None,
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     size = load_library().ace_packed_attend_backward_workspace_bytes(a, packing._args)
     workspace = q.new_empty(size, dtype=torch.uint8)
-    _call(q.device, "ace_packed_attend_backward", a, packing._args, d_out.data_ptr(), (_i64 * 3)(*d_strides), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+    _call(q.device, "ace_packed_attend_backward", a, packing._used(), d_out.data_ptr(), (_i64 * 3)(*d_strides), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
           workspace.data_ptr(), size)
     return dq, dk, dv
 

@@ -1,0 +1,58 @@
+"""A packing's table and those who use it: other streams, and a packing that goes away while they are at work."""
+import types
+
+import pytest
+import torch
+
+from superscaler_amd import layer
+from tests.test_layer_packed import case, cuda_or_skip
+
+gpu = pytest.mark.gpu
+
+
+def busy(ms=60):
+    """Work for the current stream that takes some `ms` at least."""
+    x = torch.empty(1 << 28, device="cuda")
+    for _ in range(ms * 8):     # (1 GiB takes more than an eighth of a millisecond to fill)
+        x.fill_(1.0)
+
+
+def test_a_table_is_kept_for_every_stream_that_uses_it(monkeypatch):
+    """Without a GPU: a call on a stream that is not the table's tells the allocator so, once, before anything is launched."""
+    asked, current = [], types.SimpleNamespace(cuda_stream=7)
+    p = object.__new__(layer.Packing)
+    p.device, p._args, p._streams = torch.device("cuda:0"), b"args", {3}
+    p._table = types.SimpleNamespace(record_stream=asked.append)
+    monkeypatch.setattr(layer.torch.cuda, "current_stream", lambda index: current)
+    monkeypatch.setattr(layer, "_raw_stream", lambda index: 3)
+    assert p._used() == b"args" and asked == []
+    monkeypatch.setattr(layer, "_raw_stream", lambda index: current.cuda_stream)
+    assert p._used() == b"args" and p._used() == b"args" and asked == [current]
+
+
+@gpu
+def test_a_packing_that_goes_away_under_another_stream_s_work():
+    """Its table's memory is not handed out before that work is done."""
+    device = cuda_or_skip()
+    q, k, v, do = (t.to(device) for t in case(3, 640, 4, 2, 64))
+    lengths = [300, 5, 64, 260]
+
+    def both(packing):
+        out, lse = layer.packed_attention(q, k, v, packing, window=50, sinks=3)
+        return (out, lse) + layer.packed_attention_backward(do, q, k, v, out, lse, packing, window=50, sinks=3)
+    want = both(layer.Packing(lengths, tokens=640))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    packing = layer.Packing(lengths, tokens=640)
+    place, size = packing._table.data_ptr(), packing._table.numel()
+    with torch.cuda.stream(side):
+        busy()
+        got = both(packing)
+        done = torch.cuda.Event()
+        done.record()
+    del packing
+    others = [torch.full((size,), 1 << 20, dtype=torch.int32, device=device) for _ in range(64)]
+    early = not done.query()
+    assert early and all(t.data_ptr() != place for t in others)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
