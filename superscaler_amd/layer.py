@@ -403,7 +403,9 @@ class Packing:
     """Where sequences of different lengths lie one after the other among `tokens` tokens (by default their sum; those behind the last sequence are
     of none). Made once on the host for all the layers that see them: `lengths` are numbers, 0 or more, of the host. It holds a table on
     `device`, some 72 bytes for every 128 tokens and sequence, which is there until the calls that read it are done, on whatever streams; a graph that one was
-    captured into reads it at every replay, so keep the packing as long as the graph."""
+    captured into reads it at every replay, so keep the packing as long as the graph. Making one waits for nothing: its table is
+    on its way on the stream that is current then, and calls on other streams go behind that by themselves. A graph's stream is the caller's to
+    order, as for tensors (torch.cuda.graph waits for the card first); a packing is not made while one is captured."""
 
     def __init__(self, lengths, *, tokens=None, device="cuda:0"):
         if isinstance(lengths, torch.Tensor):
@@ -424,13 +426,17 @@ class Packing:
         if device.type != "cuda":
             raise ValueError(f"device: a GPU expected, not {device}")
         self.device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
+        if torch.cuda.is_current_stream_capturing():
+            raise AceError("a packing is made before the graph that reads it is captured")
         self.lengths, self.tokens = tuple(map(int, sizes)), tokens
         lib, head = load_library(), ctypes.create_string_buffer(_PACKING.size)
         self._refused(lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, None, 0))
         _, sequences, blocks, self.longest, _ = _PACKING.unpack(head.raw)
-        table = np.zeros(max(1, blocks * 16 + sequences * 2), dtype=np.int32)
-        self._refused(lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, table.ctypes.data, table.nbytes))
-        self._table, self._streams = torch.from_numpy(table).to(self.device), {_raw_stream(self.device.index)}
+        table = torch.empty(max(1, blocks * 16 + sequences * 2), dtype=torch.int32, pin_memory=True)
+        self._refused(lib.ace_packing_table(sizes.ctypes.data, len(sizes), tokens, head, table.data_ptr(), table.numel() * 4))
+        made_on = torch.cuda.current_stream(self.device)
+        self._table, self._streams = table.to(self.device, non_blocking=True), {made_on.cuda_stream}
+        self._made = made_on.record_event()
         self._args = _PACKING.pack(tokens, sequences, blocks, self.longest, self._table.data_ptr())
 
     @staticmethod
@@ -439,12 +445,18 @@ class Packing:
             raise ValueError(f"ace_packing_table: {load_library().ace_layer_strerror(rc).decode()}")
 
     def _used(self):
-        """What a call on the current stream takes: the table's memory is not given to anything else before that stream's work on it is done."""
+        """What a call on the current stream takes.  On another stream than the table's it goes behind the table's copy, and the table's memory is not
+        given to anything else before it is done."""
         index = self.device.index
         stream = _raw_stream(index)
         if stream not in self._streams:
-            self._table.record_stream(torch.cuda.current_stream(index))
-            self._streams.add(stream)
+            current = torch.cuda.current_stream(index)
+            self._table.record_stream(current)
+            with torch.cuda.device(index):
+                captured = torch.cuda.is_current_stream_capturing()
+            if not captured:
+                current.wait_event(self._made)
+                self._streams.add(stream)
         return self._args
 
 

@@ -1,4 +1,5 @@
 """A packing's table and those who use it: other streams, and a packing that goes away while they are at work."""
+import contextlib
 import types
 
 import pytest
@@ -18,16 +19,21 @@ def busy(ms=60):
 
 
 def test_a_table_is_kept_for_every_stream_that_uses_it(monkeypatch):
-    """Without a GPU: a call on a stream that is not the table's tells the allocator so, once, before anything is launched."""
-    asked, current = [], types.SimpleNamespace(cuda_stream=7)
+    """Without a GPU: a call on a stream that is not the table's tells the allocator so and goes behind its copy, once, before anything is launched."""
+    asked = []
+    current = types.SimpleNamespace(cuda_stream=7, wait_event=lambda e: asked.append(("wait", e)))
     p = object.__new__(layer.Packing)
-    p.device, p._args, p._streams = torch.device("cuda:0"), b"args", {3}
-    p._table = types.SimpleNamespace(record_stream=asked.append)
+    p.device, p._args, p._streams, p._made = torch.device("cuda:0"), b"args", {3}, "made"
+    p._table = types.SimpleNamespace(record_stream=lambda s: asked.append(("record", s.cuda_stream)))
     monkeypatch.setattr(layer.torch.cuda, "current_stream", lambda index: current)
+    monkeypatch.setattr(layer.torch.cuda, "device", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(layer.torch.cuda, "is_current_stream_capturing", lambda: True)
     monkeypatch.setattr(layer, "_raw_stream", lambda index: 3)
     assert p._used() == b"args" and asked == []
     monkeypatch.setattr(layer, "_raw_stream", lambda index: current.cuda_stream)
-    assert p._used() == b"args" and p._used() == b"args" and asked == [current]
+    assert p._used() == b"args" and asked == [("record", 7)]       # a captured call cannot wait: its caller orders it
+    monkeypatch.setattr(layer.torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert p._used() == b"args" and p._used() == b"args" and asked == [("record", 7), ("record", 7), ("wait", "made")]
 
 
 @gpu
