@@ -444,6 +444,10 @@ class Packing:
         if rc != 0:
             raise ValueError(f"ace_packing_table: {load_library().ace_layer_strerror(rc).decode()}")
 
+    def __reduce__(self):
+        # (a copy, here or in another process, has a table of its own: the arguments hold this one's address)
+        return _packing, (self.lengths, self.tokens, str(self.device))
+
     def _used(self):
         """What a call on the current stream takes.  On another stream than the table's it goes behind the table's copy, and the table's memory is not
         given to anything else before it is done."""
@@ -458,6 +462,10 @@ class Packing:
                 current.wait_event(self._made)
                 self._streams.add(stream)
         return self._args
+
+
+def _packing(lengths, tokens, device):
+    return Packing(lengths, tokens=tokens, device=device)
 
 
 def _token_heads(t, what, packing, dtype=None):

@@ -1,5 +1,8 @@
 """A packing's table and those who use it: other streams, and a packing that goes away while they are at work."""
 import contextlib
+import copy
+import gc
+import pickle
 import types
 
 import pytest
@@ -34,6 +37,29 @@ def test_a_table_is_kept_for_every_stream_that_uses_it(monkeypatch):
     assert p._used() == b"args" and asked == [("record", 7)]       # a captured call cannot wait: its caller orders it
     monkeypatch.setattr(layer.torch.cuda, "is_current_stream_capturing", lambda: False)
     assert p._used() == b"args" and p._used() == b"args" and asked == [("record", 7), ("record", 7), ("wait", "made")]
+
+
+def test_a_copied_packing_has_a_table_of_its_own(monkeypatch):
+    """Without a GPU: copies and pickles are made from the lengths, not from the address that the first one's arguments hold."""
+    made = []
+    monkeypatch.setattr(layer.Packing, "__init__", lambda self, lengths, **how: made.append((lengths, how)))
+    p = object.__new__(layer.Packing)
+    p.lengths, p.tokens, p.device, p._args = (3, 0, 4), 9, torch.device("cuda:0"), b"an address"
+    for other in (copy.copy(p), copy.deepcopy(p), pickle.loads(pickle.dumps(p))):
+        assert not hasattr(other, "_args")
+    assert made == [((3, 0, 4), dict(tokens=9, device="cuda:0"))] * 3
+
+
+@gpu
+def test_a_copied_packing_is_as_good():
+    device = cuda_or_skip()
+    q, k, v, _ = (t.to(device) for t in case(4, 300, 2, 1, 64))
+    packing = layer.Packing([100, 0, 150], tokens=300)
+    want, others = layer.packed_attention(q, k, v, packing), [copy.deepcopy(packing), pickle.loads(pickle.dumps(packing))]
+    del packing
+    gc.collect()
+    for other in others:
+        assert other.lengths == (100, 0, 150) and all(torch.equal(a, b) for a, b in zip(layer.packed_attention(q, k, v, other), want))
 
 
 @gpu
