@@ -36,8 +36,9 @@ struct Args {
     void *dq, *dk, *dv;
     float *part_o, *part_ml;             /* attend_split: [splits][rows][width], [splits][rows][2] */
     int splits, row_blocks;
-    float *far;                          /* attend_far: [batch][kv_heads][far_blocks][far_parts][2][width][32] */
-    int far_blocks, far_parts;
+    float *far;                          /* attend_far: [far_slots][kv_heads][far_parts][2][width][32], a slot for a sequence's block of 32 first keys */
+    int far_blocks, far_parts, far_slots;
+    int far_times, far_per;              /* PACKED: a sequence's slots begin at its first token times far_times / far_per; far_per 0: at its number times far_blocks */
     /* PACKED: queries and keys are all tokens, batch the sequences */
     const ace_packed_block_t *query_blocks, *key_blocks;
     const ace_packed_sequence_t *sequences;
@@ -186,8 +187,8 @@ template <bool PACKED> struct Span {
         const int length = a.length ? a.length[b] : a.keys, start = a.start ? a.start[b] : a.keys - a.queries;
         return {start < -MOST ? -MOST : start > LATEST ? LATEST : start, length < 0 ? 0 : length > a.keys ? a.keys : length};
     }
-    __device__ inline bool has_far(const Args &) const { return true; }
-    __device__ inline int far_index() const { return b; }
+    __device__ inline bool has_far(const Args &, int) const { return true; }
+    __device__ inline int far_slot(const Args &a) const { return b * a.far_blocks; }
 };
 template <> struct Span<true> {
     int first, tokens, index;
@@ -198,8 +199,8 @@ template <> struct Span<true> {
     __device__ inline int64_t first_key(const Args &) const { return first; }
     __device__ inline int64_t values(const Args &a, int head) const { return (int64_t)head * a.queries + first; }
     __device__ inline Sequence sequence(const Args &) const { return {0, index < 0 ? 0 : tokens}; }
-    __device__ inline bool has_far(const Args &a) const { return index >= 0 && tokens > a.window; }   /* queries beyond the first key's window */
-    __device__ inline int far_index() const { return index; }
+    __device__ inline bool has_far(const Args &a, int key) const { return index >= 0 && tokens - a.window > key; }   /* queries beyond a key's window */
+    __device__ inline int far_slot(const Args &a) const { return a.far_per ? (int)((int64_t)first * a.far_times / a.far_per) : index * a.far_blocks; }
 };
 
 /* The order of a run of PRODUCTS matrix products whose operands come from LDS in READS reads each: operands of LEAD products are on
@@ -1361,8 +1362,8 @@ template <class T, int DP, int SHARE, bool PACKED> __global__ void __launch_boun
     }
     if (key >= span.keys(a)) return;
     /* what queries beyond the window have left for a first key */
-    if (a.far_parts > 0 && mine < a.sinks && span.has_far(a)) {
-        const float *part = a.far + ((((int64_t)span.far_index() * a.kv_heads + kv) * a.far_blocks + mine / 32) * a.far_parts) * (2 * 32 * DP) + (lane & 31);
+    if (a.far_parts > 0 && mine < a.sinks && span.has_far(a, mine)) {
+        const float *part = a.far + ((int64_t)(span.far_slot(a) + mine / 32) * a.kv_heads + kv) * a.far_parts * (2 * 32 * DP) + (lane & 31);
         for (int c = 0; c < a.far_parts; ++c, part += 2 * 32 * DP)
 #pragma unroll
             for (int t = 0; t < DP / 32; ++t)
@@ -1391,10 +1392,10 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
     Span<PACKED> span;
     if constexpr (PACKED) span = {__builtin_amdgcn_readfirstlane(a.sequences[b].first), __builtin_amdgcn_readfirstlane(a.sequences[b].tokens), b};
     else span = {b};
-    if (!span.has_far(a)) return;
+    const int k0 = block * 32, key = k0 + (lane & 31);
+    if (!span.has_far(a, k0)) return;
     const Sequence seq = span.sequence(a);
     const int all = span.queries(a);
-    const int k0 = block * 32, key = k0 + (lane & 31);
     const T *krow = (const T *)a.k + span.lead(a.k_stride) + (int64_t)key * a.k_stride[1] + kv * a.k_stride[2];
     const T *vrow = (const T *)a.v + span.lead(a.v_stride) + (int64_t)key * a.v_stride[1] + kv * a.v_stride[2];
     KeyGrads<T, DP> grads;
@@ -1433,7 +1434,7 @@ template <class T, int DP, bool PACKED> __global__ void __launch_bounds__(LANES)
     }
     float *sums = (float *)lds;
     constexpr int HALF = DP * 32;
-    float *to = a.far + ((((int64_t)b * a.kv_heads + kv) * a.far_blocks + block) * a.far_parts + part) * (2 * HALF);
+    float *to = a.far + (((int64_t)(span.far_slot(a) + block) * a.kv_heads + kv) * a.far_parts + part) * (2 * HALF);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         __syncthreads();
@@ -1478,8 +1479,9 @@ Args args_of(const ace_attend_t *a) {
  * 479.  4 heads on 1 of 16,384, a window of 2,048: 344 us in up to 32 parts, 354 in up to 16; 8 on 1 of 32,768, 1,024: 623 and 731.) */
 void far_of(const ace_attend_t *a, int64_t batch, int64_t queries, int64_t keys, int64_t workgroups, Args &k) {
     const int64_t sinks = a->window > 0 ? (a->sinks < keys ? a->sinks : keys) : 0;
-    k.far_blocks = (int)((sinks + 31) / 32), k.far_parts = 0;
+    k.far_blocks = (int)((sinks + 31) / 32), k.far_parts = 0, k.far_slots = 0, k.far_times = k.far_per = 0;
     if (sinks == 0 || batch == 0 || queries == 0) return;
+    k.far_slots = (int)(batch * k.far_blocks);
     const int64_t groups = batch * a->kv_heads * k.far_blocks, tiles = (int64_t)(a->heads / a->kv_heads) * ((queries + 31) / 32);
     int64_t parts = workgroups / groups;
     const int64_t most = (tiles + WAVES * 4 - 1) / (WAVES * 4);
@@ -1489,8 +1491,8 @@ void far_of(const ace_attend_t *a, int64_t batch, int64_t queries, int64_t keys,
 int width_of(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
 int64_t delta_floats(const ace_attend_t *a) { return ((int64_t)a->batch * a->heads * a->queries + 3) / 4 * 4; }
 
-size_t backward_workspace(const ace_attend_t *a, int64_t batch, const Args &k) {
-    return (size_t)(delta_floats(a) + batch * a->kv_heads * k.far_blocks * k.far_parts * 2 * 32 * width_of(a->dim)) * sizeof(float);
+size_t backward_workspace(const ace_attend_t *a, const Args &k) {
+    return (size_t)(delta_floats(a) + (int64_t)k.far_slots * a->kv_heads * k.far_parts * 2 * 32 * width_of(a->dim)) * sizeof(float);
 }
 /* the gradients' part of the arguments */
 int backward_args(const ace_attend_t *a, const void *d_gout, const int64_t *gout_stride, void *d_dq, void *d_dk, void *d_dv, void *d_workspace, Args &k) {

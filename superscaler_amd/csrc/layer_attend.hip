@@ -83,7 +83,7 @@ extern "C" size_t ace_attend_backward_workspace_bytes(const ace_attend_t *a) {
     if (check(a) != ACE_OK || a->batch == 0) return 0;
     Args k = {};
     far_of(a, a->batch, a->queries, a->keys, 256, k);
-    return backward_workspace(a, a->batch, k);
+    return backward_workspace(a, k);
 }
 
 extern "C" int ace_attend_backward(const ace_attend_t *a, const void *d_gout, const int64_t gout_stride[3], void *d_dq, void *d_dk, void *d_dv, void *d_workspace,

@@ -35,14 +35,27 @@ Args packed_args(const ace_attend_t *a, const ace_packing_t *p) {
     return k;
 }
 
-/* attend_far's part of the arguments: none where no sequence is longer than the window */
+/* attend_far's part of the arguments: none where no sequence is longer than the window.
+ *
+ * Slots for what it leaves: a block of first keys has one where a query stands beyond its first key's window, so a sequence of w + 1 + 32 (j - 1) tokens
+ * or more has j, up to far_blocks.  Which sequences are that long is not known here; the most slots per token that any has are the largest of
+ * j / (w + 1 + 32 (j - 1)), which is that of the first or the last j.  With a sequence's slots from its first token times that on, rounded down, no two
+ * sequences' meet (n tokens times it are no fewer than the slots that n tokens need, a whole number).  Where sequences are few, or about as long as first keys and window
+ * together, far_blocks for each are fewer.  (256 sequences of 128 tokens on average, 20 key heads of 128, a window of 256: with 37 first keys 148 MB, for each the same
+ * number 336; with 1,024 first keys and a sequence as long 550 MB and 5.4 GB.) */
 int packed_far(const ace_attend_t *a, const ace_packing_t *p, Args &k) {
     if (p->longest <= a->window) return ACE_OK;
     /* (Of many groups most are short sequences' and end at once: 40 sequences, 4 key heads of 64, 6,143 tokens, a window of 256, all of the backward pass: 74.5 us
      * in one part, 67.6 in three.  Of few, more parts than that are more for attend_dkv to add up: 8 sequences, 4 key heads, 8,192 tokens, a window of 512:
      * 184 in 8 parts, 193 in 16.) */
     far_of(a, p->sequences, p->longest, p->longest, (int64_t)p->sequences * a->kv_heads > 64 ? 512 : 256, k);
-    return (int64_t)p->sequences * a->kv_heads * k.far_blocks > (1 << 22) ? ACE_ETOOBIG : ACE_OK;
+    if ((int64_t)p->sequences * a->kv_heads * k.far_blocks > (1 << 22)) return ACE_ETOOBIG;
+    if (k.far_blocks == 0) return ACE_OK;
+    int64_t times = 1, per = (int64_t)a->window + 1;
+    if (k.far_blocks * per > per + 32 * ((int64_t)k.far_blocks - 1)) times = k.far_blocks, per += 32 * ((int64_t)k.far_blocks - 1);
+    const int64_t slots = (int64_t)p->tokens * times / per;
+    if (slots < k.far_slots) k.far_slots = (int)slots, k.far_times = (int)times, k.far_per = (int)per;
+    return ACE_OK;
 }
 
 }  // namespace
@@ -99,7 +112,7 @@ extern "C" int ace_packed_attend_forward(const ace_attend_t *a, const ace_packin
 
 extern "C" size_t ace_packed_attend_backward_workspace_bytes(const ace_attend_t *a, const ace_packing_t *p) {
     Args k = {};
-    return check(a, p) != ACE_OK || p->tokens == 0 || packed_far(a, p, k) != ACE_OK ? 0 : backward_workspace(a, p->sequences, k);
+    return check(a, p) != ACE_OK || p->tokens == 0 || packed_far(a, p, k) != ACE_OK ? 0 : backward_workspace(a, k);
 }
 
 extern "C" int ace_packed_attend_backward(const ace_attend_t *a, const ace_packing_t *p, const void *d_gout, const int64_t gout_stride[3], void *d_dq, void *d_dk,
@@ -108,7 +121,7 @@ extern "C" int ace_packed_attend_backward(const ace_attend_t *a, const ace_packi
     if (rc != ACE_OK || p->tokens == 0) return rc;
     Args k = packed_args(a, p);
     if ((rc = packed_far(a, p, k)) != ACE_OK) return rc;
-    if (workspace_bytes < backward_workspace(a, p->sequences, k)) return ACE_EINVAL;
+    if (workspace_bytes < backward_workspace(a, k)) return ACE_EINVAL;
     if ((rc = backward_args(a, d_gout, gout_stride, d_dq, d_dk, d_dv, d_workspace, k)) != ACE_OK) return rc;
     const hipStream_t s = (hipStream_t)stream;
     if (a->dtype == ACE_T_BF16) return a->dim <= 64 ? backward<bf16, 64, true>(k, s) : a->dim <= 96 ? backward<bf16, 96, true>(k, s) : backward<bf16, 128, true>(k, s);
