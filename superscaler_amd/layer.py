@@ -152,7 +152,9 @@ class _Untracked(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        raise AceError(f"{ctx.name} is not recorded by automatic differentiation: its gradients come from {ctx.name}_backward (call it under torch.no_grad())")
+        where = {"policy_loss": "policy_loss_gradient", "gradient_norm": None}.get(ctx.name, f"{ctx.name}_backward")
+        raise AceError(f"{ctx.name} is not recorded by automatic differentiation: " + (f"its gradients come from {where}" if where else "there is no gradient of it") +
+                       " (call it under torch.no_grad())")
 
 
 def _lost(*inputs):
