@@ -144,15 +144,19 @@ def _on_gpu(t, what):
 
 
 class _Untracked(torch.autograd.Function):
-    """Results that automatic differentiation cannot go through: the first `n` of the tensors, which depend on the others."""
+    """Results that automatic differentiation cannot go through: the first `n` of the tensors, which depend on the others; `n` 0: the first one, which
+    is changed in place."""
     @staticmethod
     def forward(ctx, name, n, *tensors):
         ctx.name = name
+        if n == 0:
+            ctx.mark_dirty(tensors[0])
+            return tensors[0]
         return tensors[:n]
 
     @staticmethod
     def backward(ctx, *grads):
-        where = {"policy_loss": "policy_loss_gradient", "gradient_norm": None}.get(ctx.name, f"{ctx.name}_backward")
+        where = {"policy_loss": "policy_loss_gradient", "gradient_norm": None, "clip_gradients": None}.get(ctx.name, f"{ctx.name}_backward")
         raise AceError(f"{ctx.name} is not recorded by automatic differentiation: " + (f"its gradients come from {where}" if where else "there is no gradient of it") +
                        " (call it under torch.no_grad())")
 
@@ -168,6 +172,16 @@ def _lost(*inputs):
 def _untracked(name, results, inputs):
     made = iter(_Untracked.apply(name, sum(t is not None for t in results), *(t for t in results + inputs if t is not None)))
     return [None if t is None else next(made) for t in results]
+
+
+def _untracked_in_place(name, changed, inputs):
+    """The same for tensors that are about to be changed.  (What has no graph to lose, a leaf or a view of what carries none, is left as it is.)"""
+    for t in changed:
+        if not t.is_leaf or not (t.requires_grad or t._is_view()):
+            try:
+                _Untracked.apply(name, 0, t, *inputs)
+            except RuntimeError as e:
+                raise AceError(f"{name}: a tensor cannot be changed while automatic differentiation is on (call it under torch.no_grad()): {e}") from None
 
 
 # ---- norms around a block ---------------------------------------------------------------------------------------------------
@@ -819,9 +833,14 @@ def clip_gradients(grads, max_norm, *, grad_scale=None) -> GradientNorm:
     if any(end > begin for (_, end), (begin, _) in zip(places, places[1:])):
         raise ValueError("grads: two of them overlap")
     r = _norm_of(grads, table, max_norm, grad_scale)
+    made = r
+    if _lost(*grads, grad_scale):
+        inputs = [t for t in (*grads, grad_scale) if t is not None and t.requires_grad]
+        made = GradientNorm(*_untracked("clip_gradients", tuple(r), tuple(inputs)))
+        _untracked_in_place("clip_gradients", grads, inputs)
     _call(grads[0].device, "ace_gradient_scale", table.buffer_info()[0], len(grads), r.scale.data_ptr())
     torch.autograd.graph.increment_version(grads)
-    return r
+    return made
 
 
 # ---- AdamW over many tensors ------------------------------------------------------------------------------------------------

@@ -22,3 +22,45 @@ def test_the_message_names_calls_that_are_there(name):
         made.sum().backward()
     words = [w.strip("():") for w in str(e.value).split() if "_" in w and "." not in w]
     assert name in words and all(hasattr(layer, w) for w in words)
+
+
+def test_what_is_changed_in_place_is_told():
+    """Without a GPU: tensors with a graph and those that depend on them; leaves and views of what has none stay as they are."""
+    a = torch.ones(3, requires_grad=True)
+    g, plain, whole = a * 2, torch.ones(3), torch.ones(4)
+    with torch.no_grad():
+        part = whole[:3]
+    layer._untracked_in_place("clip_gradients", [g, plain, part, a], [g, a])
+    for t in (g, plain):
+        with pytest.raises(AceError, match="clip_gradients"):
+            t.sum().backward()
+    assert not part.requires_grad and a.is_leaf
+    with pytest.raises(AceError, match="no_grad"):
+        layer._untracked_in_place("clip_gradients", [(a * 2).split(1)[0]], [a])
+
+
+@gpu
+def test_clipped_gradients_that_carry_a_graph():
+    """As with gradient_norm, going backward through what comes back, or through what was clipped, is an error; the values are as without a graph."""
+    device = cuda_or_skip()
+    x = torch.arange(1.0, 11.0, device=device, requires_grad=True)
+
+    def fresh():
+        y = torch.ones(5, device=device)
+        return [torch.autograd.grad((x ** 3).sum(), x, create_graph=True)[0], y]
+    with torch.no_grad():
+        want = [t.detach() for t in [3 * x ** 2, torch.ones(5, device=device)]]
+        r0 = layer.clip_gradients(want, 0.5)
+        assert not any(t.requires_grad for t in r0)
+    for through in (lambda g, r: r.norm.sum(), lambda g, r: r.scale.sum(), lambda g, r: r.norms.sum(), lambda g, r: g[0].sum(), lambda g, r: g[1].sum()):
+        grads = fresh()
+        r = layer.clip_gradients(grads, 0.5)
+        assert all(torch.equal(a, b) for a, b in zip(grads, want)) and all(torch.equal(a, b) for a, b in zip(r, r0))
+        with pytest.raises(AceError, match="clip_gradients"):
+            through(grads, r).backward()
+    scale = torch.ones(1, device=device, requires_grad=True)
+    with pytest.raises(AceError, match="clip_gradients"):
+        layer.clip_gradients([torch.ones(5, device=device)], 0.5, grad_scale=scale).norm.backward()
+    p = torch.ones(5, device=device, requires_grad=True)      # a leaf has no graph to lose
+    layer.clip_gradients([p], 0.5)
+    assert p.is_leaf and float(p.detach().norm()) < 0.51
