@@ -715,13 +715,8 @@ def policy_loss(logits, targets, old_logp, advantages, *, ref_logp=None, weights
     gradient of logits is token_logprobs_backward(d_loss * d_logp, logits, targets, stats), or comes along from policy_loss_gradient."""
     a, z, keep, made, workspace = _policy_args(logits, targets, old_logp, advantages, ref_logp, weights, clip, kl_weight)
     _call(z.device, "ace_policy_loss", a, *map(_pointer, (made.loss, made.logp, made.stats, made.d_logp, workspace)), workspace.numel() * 8)
-    return _policy_result("policy_loss", made, logits, old_logp, advantages, ref_logp, weights)
-
-
-def _policy_result(name, made, *inputs):
-    if _lost(*inputs):
-        made = PolicyLoss(*_untracked(name, tuple(made), inputs))
-    return made
+    inputs = (logits, old_logp, advantages, ref_logp, weights)
+    return PolicyLoss(*_untracked("policy_loss", tuple(made), inputs)) if _lost(*inputs) else made
 
 
 def policy_loss_gradient(logits, targets, old_logp, advantages, *, ref_logp=None, weights=None, clip=(0.2, 0.2), kl_weight=0.0, d_loss=None, out=None):
@@ -736,9 +731,12 @@ def policy_loss_gradient(logits, targets, old_logp, advantages, *, ref_logp=None
     grad, stride = _gradient_of(z, out)
     _call(z.device, "ace_policy_loss_gradient", a, _pointer(d_loss), *map(_pointer, (made.loss, made.logp, made.stats, made.d_logp, grad)), stride, workspace.data_ptr(),
           workspace.numel() * 8)
-    made = _policy_result("policy_loss", made, logits, old_logp, advantages, ref_logp, weights)
     if out is not None:
         torch.autograd.graph.increment_version(out)
+    inputs = tuple(t for t in (logits, old_logp, advantages, ref_logp, weights, d_loss) if t is not None)
+    if _lost(*inputs):      # (`out` is left as it is: its memory comes back as another tensor)
+        made = PolicyLoss(*_untracked("policy_loss", tuple(made), inputs))
+        grad = _Untracked.apply("policy_loss", 0, grad.detach(), *inputs)
     return made, grad
 
 
@@ -820,8 +818,8 @@ def gradient_norm(grads, *, max_norm=None, grad_scale=None) -> GradientNorm:
     given = list(grads)
     grads, table = _gradients(given, False)
     made = _norm_of(grads, table, max_norm, grad_scale)
-    if _lost(*given):
-        made = GradientNorm(*_untracked("gradient_norm", tuple(made), tuple(given)))
+    if _lost(*given, grad_scale):
+        made = GradientNorm(*_untracked("gradient_norm", tuple(made), (*given, grad_scale)))
     return made
 
 

@@ -64,3 +64,40 @@ def test_clipped_gradients_that_carry_a_graph():
     p = torch.ones(5, device=device, requires_grad=True)      # a leaf has no graph to lose
     layer.clip_gradients([p], 0.5)
     assert p.is_leaf and float(p.detach().norm()) < 0.51
+
+
+@gpu
+def test_a_policy_s_gradient_is_not_gone_through():
+    """Second derivatives are lost, whichever input they are by; the logits' own graph still takes the gradient, also where they hold it."""
+    device = cuda_or_skip()
+    gen = torch.Generator(device=device).manual_seed(1)
+    w = torch.randn(8, 64, device=device, generator=gen)
+    h, t, old, A = torch.randn(6, 8, device=device, generator=gen), torch.arange(6, device=device), torch.full((6,), -4.0, device=device), torch.ones(6, device=device)
+    want = layer.policy_loss_gradient(h @ w, t, old, A)[1]
+    for in_place in (False, True):
+        p = w.clone().requires_grad_()
+        logits = h @ p
+        r, g = layer.policy_loss_gradient(logits, t, old, A, out=logits if in_place else None)
+        assert torch.equal(g, want) and (not in_place or g.data_ptr() == logits.data_ptr())
+        with pytest.raises(AceError, match="policy_loss_gradient"):
+            g.sum().backward(retain_graph=True)
+        g.mul_(2.0)             # a program's own work on it
+        logits.backward(g)
+        assert torch.equal(p.grad, h.t() @ (2 * want))
+    given = dict(logits=h @ w, targets=t, old_logp=old, advantages=A, ref_logp=old + 0.1, weights=A / 6, d_loss=torch.ones(1, device=device))
+    for name in ("logits", "old_logp", "advantages", "ref_logp", "weights", "d_loss"):
+        how = dict(given, **{name: given[name].clone().requires_grad_()})
+        for each in layer.policy_loss_gradient(**how, kl_weight=0.1)[1], layer.policy_loss_gradient(**how, kl_weight=0.1)[0].loss:
+            with pytest.raises(AceError):
+                each.sum().backward()
+        with torch.no_grad():
+            assert not layer.policy_loss_gradient(**how, kl_weight=0.1)[1].requires_grad
+
+
+@gpu
+def test_a_factor_that_has_a_gradient():
+    device = cuda_or_skip()
+    scale = torch.ones(1, device=device, requires_grad=True)
+    for result in layer.gradient_norm([torch.ones(5, device=device)], max_norm=0.5, grad_scale=scale):
+        with pytest.raises(AceError, match="gradient_norm"):
+            result.sum().backward()
