@@ -16,7 +16,8 @@ another stream is the caller's to order.  Where a row's elements are not adjacen
 sizes raise ValueError, other types TypeError, a missing library or a HIP failure AceError.  There is no other form behind these calls.
 
 Gradients come from the *_backward calls; torch's automatic differentiation records nothing of these operators.  Where it is on and an
-input requires a gradient, so do the results, and going backward through them raises AceError: no gradient is lost unnoticed.
+input requires a gradient, so do the results, and going backward through them raises AceError: no gradient is lost unnoticed.  Tensors that
+carry a tangent of forward-mode differentiation raise it at once.
 """
 import array
 import ctypes
@@ -27,6 +28,7 @@ from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .evaluator import ACE_ETOOBIG, AceError
 
@@ -161,6 +163,14 @@ class _Untracked(torch.autograd.Function):
                        " (call it under torch.no_grad())")
 
 
+def _no_tangents(*tensors):
+    """Raises where forward-mode differentiation would lose a tangent of these."""
+    if forward_ad._current_level >= 0:      # (a level is entered)
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise AceError("forward-mode differentiation: these operators have no tangents (hand them forward_ad.unpack_dual(t).primal)")
+
+
 def _lost(*inputs):
     """Whether automatic differentiation would miss a gradient of these."""
     for t in inputs:
@@ -246,6 +256,7 @@ def _refuse_block_norm(x, block, residual_scale, gate, exit_weight, exit_bias, e
 
 def _block_norm_args(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind, eps):
     """(packed arguments, the tensors whose addresses they hold, rows)"""
+    _no_tangents(x, block, gate, exit_weight, exit_bias, entry_weight, entry_bias)
     if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _TYPES and x.dim() > 0 and 1 <= x.shape[-1] <= MAX_WIDTH and kind in ("layer", "rms")):
         _refuse_block_norm(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind)
     dtype, device, shape = x.dtype, x.device, x.shape
@@ -295,6 +306,7 @@ def block_norm_backward(d_residual, d_normed, x, block, stats, *, residual_scale
     """Gradients of what block_norm was given, from those of its two results (either may be None) and its `stats`.  Sums over rows
     are in 32 bits and in an order that the sizes alone decide: the same call gives the same bits."""
     a, keep, rows = _block_norm_args(x, block, residual_scale, gate, exit_weight, exit_bias, entry_weight, entry_bias, kind, 0.0)
+    _no_tangents(d_residual, d_normed)
     if d_normed is not None and entry_weight is None:
         raise ValueError("d_normed goes with an entry norm")
     grads = []
@@ -355,6 +367,7 @@ def _attend_head(batch, queries, keys, heads, kv_heads, dim, dtype, window, sink
 
 def _attend_args(q, k, v, window, sinks, scale, start, lengths):
     """(q, k and v as the kernels read them, the arguments' part before the strides, q's, k's and v's strides, (batch, heads, queries))"""
+    _no_tangents(q, k, v)
     q, q_strides = _heads(q, "q")
     (k, k_strides), (v, v_strides) = _heads(k, "k", q), _heads(v, "v", q)
     (batch, queries, heads, dim), (_, keys, kv_heads, _) = q.shape, k.shape
@@ -401,6 +414,7 @@ def window_attention_backward(d_out, q, k, v, out, lse, *, window=None, sinks=0,
     """Gradients (dq, dk, dv) of window_attention's q, k and v from that of its `out`; `out` and `lse` are what it returned.  The
     same call gives the same bits."""
     q, k, v, head, strides, rows = _attend_args(q, k, v, window, sinks, scale, start, lengths)
+    _no_tangents(d_out, out, lse)
     (d_out, d_strides), (out, out_strides) = _heads(d_out, "d_out", q), _heads(out, "out", q)
     if d_out.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"d_out and out: {tuple(q.shape)} expected, got {tuple(d_out.shape)} and {tuple(out.shape)}")
@@ -504,6 +518,7 @@ def _token_heads(t, what, packing, dtype=None):
 
 def _packed_args(q, k, v, packing, window, sinks, scale):
     """As _attend_args, with the tokens as those of one sequence."""
+    _no_tangents(q, k, v)
     if not isinstance(packing, Packing):
         raise TypeError(f"packing: a Packing expected, not {type(packing).__name__}")
     q, q_strides = _token_heads(q, "q", packing)
@@ -536,6 +551,7 @@ def packed_attention_backward(d_out, q, k, v, out, lse, packing, *, window=None,
     sequence are 0. Up to 2^22 of sequences * kv_heads * (blocks of 32 first keys) where a sequence is longer than the window. The same call gives the
     same bits."""
     q, k, v, head, strides, rows = _packed_args(q, k, v, packing, window, sinks, scale)
+    _no_tangents(d_out, out, lse)
     (d_out, d_strides), (out, out_strides) = _token_heads(d_out, "d_out", packing, q.dtype), _token_heads(out, "out", packing, q.dtype)
     if d_out.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"d_out and out: {tuple(q.shape)} expected, got {tuple(d_out.shape)} and {tuple(out.shape)}")
@@ -613,6 +629,7 @@ def _refuse_token_loss(logits, targets, rows):
 def _token_loss_args(logits, targets, *rows, bounds=(0.0, 1.0), kl_weight=0.0):
     """(packed arguments, logits as the kernels read them, the other tensors whose addresses the arguments hold); `rows`: old_logp, advantages,
     ref_logp and weights, or none of them"""
+    _no_tangents(logits, *rows)
     if not (isinstance(logits, torch.Tensor) and isinstance(targets, torch.Tensor) and logits.is_cuda and logits.dtype in _TYPES and logits.dim() > 0 and
             1 <= logits.shape[-1] <= MAX_VOCAB and targets.dtype in _TARGETS):
         _refuse_token_loss(logits, targets, rows)
@@ -672,6 +689,7 @@ def token_logprobs_backward(d_logp, logits, targets, stats, *, out=None):
     if out is logits and _flat_rows(logits) is None:
         raise ValueError("out: logits of rows that lie evenly expected")
     a, z, keep = _token_loss_args(logits, targets)
+    _no_tangents(d_logp, stats)
     _on_gpu(d_logp, "d_logp")
     if d_logp.dtype != torch.float32:
         raise TypeError(f"d_logp: float32 expected, not {d_logp.dtype}")
@@ -749,6 +767,7 @@ class GradientNorm(NamedTuple):
 
 
 def _one_float(t, what, device):
+    _no_tangents(t)
     _on_gpu(t, what)
     if t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
         raise ValueError(f"{what}: one float32 on {device} expected")
@@ -769,6 +788,7 @@ def _dense(t):
 def _gradients(grads, in_place):
     """(the tensors, ace_gradient_t for each as 64-bit numbers)"""
     grads = list(grads)
+    _no_tangents(*grads)
     if not grads:
         raise ValueError("no gradients")
     try:
@@ -921,6 +941,7 @@ class AdamW:
         if not (0 <= b1 < 1 and 0 <= b2 < 1) or step < 1 or eps < 0:
             raise ValueError(f"betas in [0, 1), a step from 1 and eps >= 0 expected, got {betas}, {step}, {eps}")
         grads = list(grads)
+        _no_tangents(*grads)
         if len(grads) != len(self._shapes):
             raise ValueError(f"{len(grads)} gradients for {len(self._shapes)} parameters")
         kind, device = getattr(grads[0], "dtype", None), self.device

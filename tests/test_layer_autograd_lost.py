@@ -1,6 +1,7 @@
 """Where automatic differentiation would lose a gradient of the packed step's operators, it is told, and what to call instead."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from superscaler_amd import layer
 from superscaler_amd.evaluator import AceError
@@ -101,3 +102,44 @@ def test_a_factor_that_has_a_gradient():
     for result in layer.gradient_norm([torch.ones(5, device=device)], max_norm=0.5, grad_scale=scale):
         with pytest.raises(AceError, match="gradient_norm"):
             result.sum().backward()
+
+
+def test_tangents():
+    """Without a GPU: what carries one is refused before anything else is looked at."""
+    x, d = torch.ones(2, 4), torch.ones(2, 4)
+    layer._no_tangents(x, None)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, d)
+        layer._no_tangents(x, None)
+        with pytest.raises(AceError, match="forward-mode"):
+            layer._no_tangents(None, x, dual)
+        t, f, other = torch.zeros(2, dtype=torch.int64), torch.zeros(2), forward_ad.make_dual(torch.zeros(2), torch.ones(2))
+        packing = object.__new__(layer.Packing)
+        for call in (lambda: layer.block_norm(dual, entry_weight=x[0]), lambda: layer.block_norm(x, dual, entry_weight=x[0]), lambda: layer.window_attention(x, dual, x),
+                     lambda: layer.packed_attention(x, x, dual, packing), lambda: layer.token_logprobs(dual, t), lambda: layer.policy_loss(x, t, other, f),
+                     lambda: layer.policy_loss_gradient(x, t, f, f, weights=other), lambda: layer.gradient_norm([x, dual]), lambda: layer.clip_gradients([dual], 1.0),
+                     lambda: layer.token_logprobs_backward(f, dual, t, x)):
+            with pytest.raises(AceError, match="forward-mode"):
+                call()
+        layer._no_tangents(forward_ad.unpack_dual(dual).primal)
+    layer._no_tangents(x)
+
+
+@gpu
+def test_tangents_on_the_gpu():
+    """Of the tensors that come in beside the first ones; a call without any is as it is outside."""
+    device = cuda_or_skip()
+    z, t, f = torch.randn(4, 30, device=device), torch.arange(4, device=device), torch.full((4,), -3.0, device=device)
+    one, q = torch.ones(1, device=device), torch.ones(6, 2, 64, dtype=torch.bfloat16, device=device)
+    packing = layer.Packing([6])
+    out, lse = layer.packed_attention(q, q, q, packing)
+    stats, want = layer.token_logprobs(z, t).stats, layer.policy_loss_gradient(z, t, f, f, d_loss=one)[1]
+    with forward_ad.dual_level():
+        def dual(x):
+            return forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: layer.packed_attention_backward(dual(q), q, q, q, out, lse, packing), lambda: layer.token_logprobs_backward(dual(f), z, t, stats),
+                     lambda: layer.policy_loss_gradient(z, t, f, f, d_loss=dual(one)), lambda: layer.gradient_norm([z], grad_scale=dual(one)),
+                     lambda: layer.clip_gradients([z], 1.0, grad_scale=dual(one)), lambda: layer.window_attention_backward(*[dual(q[None])] + [q[None]] * 4, lse[None])):
+            with pytest.raises(AceError, match="forward-mode"):
+                call()
+        assert torch.equal(layer.policy_loss_gradient(z, t, f, f, d_loss=one)[1], want)
