@@ -647,6 +647,16 @@ def _token_loss_args(logits, targets, *rows, bounds=(0.0, 1.0), kl_weight=0.0):
     return a, logits, keep
 
 
+def _meet(a, a_step, b, b_step, rows, size):
+    """Whether some of `rows` rows of `size` bytes from a on, a_step apart, share bytes with such rows from b on, but for being the same ones row for row."""
+    if a + (rows - 1) * a_step + size <= b or b + (rows - 1) * b_step + size <= a:
+        return False
+    if rows == 1 or a_step == b_step:
+        # (rows that lie between the other's rows, as of two halves of wider ones, are their own)
+        return a != b and (rows == 1 or not size <= (b - a) % a_step <= a_step - size)
+    return True
+
+
 def _gradient_of(logits, out):
     """Where the logits' gradient goes: (tensor, elements between its rows)"""
     if out is None:
@@ -659,11 +669,7 @@ def _gradient_of(logits, out):
     if out.shape != logits.shape or out.device != logits.device or stride is None:
         raise ValueError(f"out: rows {tuple(logits.shape)} on {logits.device} expected, got {tuple(out.shape)} on {out.device}")
     rows, size = math.prod(out.shape[:-1]), out.element_size()
-
-    def end(t, step):
-        return t.data_ptr() + ((rows - 1) * step + t.shape[-1]) * size
-    own = _flat_rows(logits)
-    if rows and not (out.data_ptr() == logits.data_ptr() and (stride == own or rows == 1)) and out.data_ptr() < end(logits, own) and logits.data_ptr() < end(out, stride):
+    if rows and _meet(out.data_ptr(), stride * size, logits.data_ptr(), _flat_rows(logits) * size, rows, out.shape[-1] * size):
         raise ValueError("out: the logits themselves or memory of its own expected")
     return out, stride
 
