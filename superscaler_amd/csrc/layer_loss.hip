@@ -306,7 +306,7 @@ template <class T> __global__ void __launch_bounds__(BACK_LANES) loss_back(const
         auto grad = [&](float x) { return (T)(-d * (power(x - top) * by)); };
         /* (read before anything is written: the gradient may go where the logits are) */
         const bool mine = lane == layout.owner((int)target, BACK_LANES) && layout.piece_of((int)target) / (BACK_LANES * BACK_HELD) == part;
-        const float taken = mine ? (float)z[target] : 0.0f, edge = part == 0 && lane < layout.rest ? (float)z[layout.edge(lane)] : 0.0f;
+        const float logp = mine && a.logp ? a.logp[row] : 0.0f, taken = mine && !a.logp ? (float)z[target] : 0.0f, edge = part == 0 && lane < layout.rest ? (float)z[layout.edge(lane)] : 0.0f;
         piece<T> v[BACK_HELD];
 #pragma unroll
         for (int k = 0; k < BACK_HELD; ++k)
@@ -320,8 +320,9 @@ template <class T> __global__ void __launch_bounds__(BACK_LANES) loss_back(const
             out.put(k, r);
         }
         if (part == 0 && lane < layout.rest) to[layout.edge(lane)] = grad(edge);
-        /* the target's own, by the lane that has just left it as another's */
-        if (mine) to[target] = (T)(d * (1.0f - power(taken - top) * by));
+        /* the target's own, by the lane that has just left it as another's.  (Next to 1 a probability has no digits left for what it lacks; its logarithm
+         * has them all.) */
+        if (mine) to[target] = (T)(a.logp ? -d * expm1f(logp) : d * (1.0f - power(taken - top) * by));
     }
 }
 
@@ -435,7 +436,7 @@ extern "C" int ace_token_logprobs_backward(const ace_token_loss_t *a, const floa
     if (rc != ACE_OK || a->rows == 0) return rc;
     if (!g_logp || !d_stats || (rc = check_out(a, d_dlogits, out_stride)) != ACE_OK) return ACE_EINVAL;
     Loss k = args_of(a);
-    k.g = g_logp, k.stats = (float *)d_stats, k.d_logits = d_dlogits, k.out_stride = out_stride;
+    k.logp = (float *)a->d_old, k.g = g_logp, k.stats = (float *)d_stats, k.d_logits = d_dlogits, k.out_stride = out_stride;
     return backward(k, a->dtype, false, (hipStream_t)stream);
 }
 

@@ -688,13 +688,20 @@ def token_logprobs(logits, targets) -> TokenLogprobs:
     return TokenLogprobs(logp, stats)
 
 
-def token_logprobs_backward(d_logp, logits, targets, stats, *, out=None):
+def token_logprobs_backward(d_logp, logits, targets, stats, *, logp=None, out=None):
     """Gradient of token_logprobs' logits from that of its `logp` (float32) and its `stats`: d_logp ([target] - softmax), 0 where d_logp is or
     there is no target.  Cross entropy, averaged over n tokens, has d_logp = -1 / n; policy_loss has d_loss times its own `d_logp`.
-    `out`: None, or where the gradient goes, which may be the logits themselves."""
+    `logp`: None, or what token_logprobs returned: with it a target's own gradient, d_logp (1 - p), keeps its digits where its probability p is next to 1 (without,
+    it is off by up to 2^-22 d_logp).  `out`: None, or where the gradient goes, which may be the logits themselves."""
     if out is logits and _flat_rows(logits) is None:
         raise ValueError("out: logits of rows that lie evenly expected")
-    a, z, keep = _token_loss_args(logits, targets)
+    if logp is not None:
+        _on_gpu(logp, "logp")
+        if logp.dtype != torch.float32:
+            raise TypeError(f"logp: float32 expected, not {logp.dtype}")
+        if not isinstance(targets, torch.Tensor) or logp.shape != targets.shape or logp.device != targets.device:
+            raise ValueError(f"logp: what token_logprobs returned for these targets expected, got {tuple(logp.shape)} on {logp.device}")
+    a, z, keep = _token_loss_args(logits, targets, logp)     # (where the policy's have those of an earlier one)
     _no_tangents(d_logp, stats)
     _on_gpu(d_logp, "d_logp")
     if d_logp.dtype != torch.float32:

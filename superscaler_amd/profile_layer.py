@@ -262,10 +262,10 @@ def measure(w, micro_batch, tp, window=None, sinks=0, vocab=51200, reps=10, devi
         return out
     a, even = x.flatten(0, -2), torch.full((micro_batch * s,), -1.0 / (micro_batch * s), device=device)
     logits = a @ table.t()
-    stats = layer.token_logprobs(logits, tokens).stats
+    logp, stats = layer.token_logprobs(logits, tokens)
 
     def back():
-        g = layer.token_logprobs_backward(even, logits, tokens, stats)
+        g = layer.token_logprobs_backward(even, logits, tokens, stats, logp=logp)
         return g @ table, a.t() @ g
     both("gpt-post-process", lambda: layer.token_logprobs(a @ table.t(), tokens), back)
     return out
