@@ -75,7 +75,7 @@ __device__ inline float around(float top) { return top == -__builtin_inff() ? 0.
 __device__ inline float power(float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, LOG2E, x * LOG2E_REST)); }
 
 /* Joins the lanes' maxima and sums; all lanes know the result.  `tops`, `sums`: one for each wavefront, not in use. */
-template <int LANES> __device__ inline Row join(float top, float total, float *tops, double *sums) {
+template <int LANES, class S> __device__ inline Row join(float top, S total, float *tops, double *sums) {
     float most = top;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
@@ -252,21 +252,25 @@ template <class T, int LANES, bool POLICY> __global__ void __launch_bounds__(LAN
                 for (int e = 0; e < PIECE<T>; ++e) v[i][e] = (T)-inf;
         }
     };
-    float top = lane < layout.rest ? (float)z[layout.edge(lane)] : -inf, total = lane < layout.rest ? power(top - around(top)) : 0.0f;
+    float top = lane < layout.rest ? (float)z[layout.edge(lane)] : -inf;
+    /* (a lane has up to half a million elements: their sum is of 64 bits, that of the pieces of a turn of 32) */
+    double total = lane < layout.rest ? (double)power(top - around(top)) : 0.0;
     auto use = [&](piece<T> (&v)[AHEAD]) {
         float most = -inf;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
             for (int e = 0; e < PIECE<T>; ++e) most = fmaxf(most, (float)v[i][e]);
-        if (most > top) total *= power(top - most), top = most;
+        if (most > top) total *= (double)power(top - most), top = most;
         const float base = around(top);
+        float turn = 0.0f;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             keep(v[i]);
 #pragma unroll
-            for (int e = 0; e < PIECE<T>; ++e) total += power((float)v[i][e] - base);
+            for (int e = 0; e < PIECE<T>; ++e) turn += power((float)v[i][e] - base);
         }
+        total += (double)turn;
     };
     piece<T> x[AHEAD], y[AHEAD];
     ask(x, 0);
