@@ -2,8 +2,9 @@
  * Log-probabilities of taken tokens and the clipped policy loss (ace_token_logprobs, ace_policy_loss), with gradients.
  *
  * Rows of logits, thousands to a hundred thousand elements each, are read once. A lane keeps a maximum of its own and the sum of exponentials
- * around it, 32 bits each; lanes and wavefronts are joined in 64 bits, and one lane goes on in 64 bits from the row's maximum and sum to its
- * log-probability, loss and derivative: a ratio that stands next to the border of its clipping falls on the side that it belongs to.
+ * around it, 32 bits each (of rows too large to be held, 32 terms at a time); lanes and wavefronts are joined in 64 bits, and one lane goes on in 64 bits from the row's
+ * maximum and sum to its log-probability, loss and derivative. So nothing but the lanes' sums is rounded before a ratio is held against the border of its clipping: it
+ * falls on the side that it belongs to unless it is nearer to the border than those sums are exact (2^-24 of a ratio for each term of a lane, some hundreds at most).
  *
  * Bound by memory.  A workgroup's registers hold a whole row (held_rows), so that the gradient needs no second look at the logits: 8,192 rows of
  * 51,200 in bfloat16, a fifth of them without a target, 294 us, 5.2 TB/s of what is read and written, as a large copy does; with a second look (loss_rows,
