@@ -355,8 +355,8 @@ def main(argv=None):
     for what, asked, there in (("--micro-batches", args.micro_batches, base.mbs_list), ("--tp", args.tp, [t for t in base.tp_list if heads % t == 0])):
         if any(v not in there for v in asked or ()):
             ap.error(f"{what}: of workload {w.name} there are {there}")
-    if args.documents < 0 or (args.clip is not None and not args.clip > 0):
-        ap.error("--documents: 0 or more, and --clip: a positive number expected")
+    if args.documents < 0 or args.steps < 0 or args.policy_steps < 0 or (args.clip is not None and not args.clip > 0):
+        ap.error("--documents, --steps and --policy-steps: 0 or more, and --clip: a positive number expected")
     measured = {(b, tp): measure(w, b, tp, args.window, args.sinks, reps=args.reps, documents=args.documents, loss=args.loss)
                 for b in (args.micro_batches or base.mbs_list) for tp in (args.tp or base.tp_list) if heads % tp == 0}
     db = database(w, graph, measured, base)
