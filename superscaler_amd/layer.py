@@ -933,6 +933,7 @@ class AdamW:
         if state_bits == 8:
             for name in ("m_scale", "v_scale"):
                 self.state[name] = torch.zeros(self.size // ADAMW_BLOCK, dtype=torch.float32, device=self.device)
+        self._streams = {_raw_stream(self.device.index)}
         self._shapes = [p.shape for p in params]
         self._places = table[:, 0].tolist(), table[:, 1].tolist()
         self._args = _AdamW(self._tensors.data_ptr(), self._chunk_tensor.data_ptr(), len(params), int(self._first_chunks[-1]), state_bits, 0,
@@ -975,6 +976,11 @@ class AdamW:
             _on_gpu(grad_scale, "grad_scale")
             if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != device:
                 raise ValueError(f"grad_scale: one float32 on {device} expected")
+        stream = _raw_stream(device.index)
+        if stream not in self._streams:      # (the memory of what is this object's own goes to nothing else before that stream's work on it is done)
+            for t in (self._tensors, self._chunk_tensor, *self.state.values()):
+                t.record_stream(torch.cuda.current_stream(device))
+            self._streams.add(stream)
         a = self._args
         a.grad_type = _TYPES[kind]
         a.d_m, a.d_v, a.d_m_scale, a.d_v_scale = map(_pointer, self._held())
