@@ -200,9 +200,12 @@ typedef struct ace_token_loss {
 
 /* d_logp: float[rows]; d_stats: float[rows][2] = top and total. */
 int ace_token_logprobs(const ace_token_loss_t *a, float *d_logp, float *d_stats, void *stream);
-/* d_dlogits: of the logits' type, rows out_stride elements apart; may be the logits themselves, row for row.  g_logp: float[rows].  a->d_old: NULL, or the
- * d_logp of ace_token_logprobs: the target's d_z then keeps its digits where its probability is next to 1 (otherwise it is off by up to 2^-22 g). */
+/* d_dlogits: of the logits' type, rows out_stride elements apart; may be the logits themselves, row for row.  g_logp: float[rows]. */
 int ace_token_logprobs_backward(const ace_token_loss_t *a, const float *g_logp, const float *d_stats, void *d_dlogits, int64_t out_stride, void *stream);
+/* The same with the d_logp of ace_token_logprobs, or NULL: the target's d_z keeps its digits where its probability is next to 1 (without, it is off by up to
+ * 2^-22 g). */
+int ace_token_logprobs_gradient(const ace_token_loss_t *a, const float *g_logp, const float *d_logp, const float *d_stats, void *d_dlogits, int64_t out_stride,
+                                void *stream);
 /* d_loss: one float; d_dlogp: float[rows], for g = 1.  d_workspace: ace_policy_loss_workspace_bytes(a) bytes, a multiple of 8. */
 size_t ace_policy_loss_workspace_bytes(const ace_token_loss_t *a);
 int ace_policy_loss(const ace_token_loss_t *a, float *d_loss, float *d_logp, float *d_stats, float *d_dlogp, void *d_workspace, size_t workspace_bytes, void *stream);

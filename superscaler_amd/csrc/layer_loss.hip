@@ -436,13 +436,18 @@ extern "C" int ace_token_logprobs(const ace_token_loss_t *a, float *d_logp, floa
     return forward<false>(k, a->dtype, (hipStream_t)stream);
 }
 
-extern "C" int ace_token_logprobs_backward(const ace_token_loss_t *a, const float *g_logp, const float *d_stats, void *d_dlogits, int64_t out_stride, void *stream) {
+extern "C" int ace_token_logprobs_gradient(const ace_token_loss_t *a, const float *g_logp, const float *d_logp, const float *d_stats, void *d_dlogits, int64_t out_stride,
+                                           void *stream) {
     int rc = check(a, false);
     if (rc != ACE_OK || a->rows == 0) return rc;
     if (!g_logp || !d_stats || (rc = check_out(a, d_dlogits, out_stride)) != ACE_OK) return ACE_EINVAL;
     Loss k = args_of(a);
-    k.logp = (float *)a->d_old, k.g = g_logp, k.stats = (float *)d_stats, k.d_logits = d_dlogits, k.out_stride = out_stride;
+    k.logp = (float *)d_logp, k.g = g_logp, k.stats = (float *)d_stats, k.d_logits = d_dlogits, k.out_stride = out_stride;
     return backward(k, a->dtype, false, (hipStream_t)stream);
+}
+
+extern "C" int ace_token_logprobs_backward(const ace_token_loss_t *a, const float *g_logp, const float *d_stats, void *d_dlogits, int64_t out_stride, void *stream) {
+    return ace_token_logprobs_gradient(a, g_logp, nullptr, d_stats, d_dlogits, out_stride, stream);
 }
 
 extern "C" size_t ace_policy_loss_workspace_bytes(const ace_token_loss_t *a) { return check(a, true) == ACE_OK ? (size_t)a->rows * sizeof(double) : 0; }

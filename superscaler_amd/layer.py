@@ -38,7 +38,7 @@ _lib = None
 EXPORTS = ["ace_layer_abi_version", "ace_layer_strerror", "ace_layer_last_hip_error", "ace_block_norm_forward", "ace_block_norm_workspace_bytes",
            "ace_block_norm_backward", "ace_attend_workspace_bytes", "ace_attend_forward", "ace_attend_backward_workspace_bytes",
            "ace_attend_backward", "ace_adamw_step", "ace_adamw_moments", "ace_gradient_norm_workspace_bytes", "ace_gradient_norm", "ace_gradient_scale",
-           "ace_token_logprobs", "ace_token_logprobs_backward", "ace_policy_loss_workspace_bytes", "ace_policy_loss", "ace_policy_loss_gradient",
+           "ace_token_logprobs", "ace_token_logprobs_backward", "ace_token_logprobs_gradient", "ace_policy_loss_workspace_bytes", "ace_policy_loss", "ace_policy_loss_gradient",
            "ace_packing_table", "ace_packed_attend_forward", "ace_packed_attend_backward_workspace_bytes", "ace_packed_attend_backward"]
 ABI_VERSION = 2
 MAX_WIDTH = 32768       # ACE_NORM_MAX_WIDTH
@@ -107,6 +107,7 @@ def load_library():
     lib.ace_gradient_scale.argtypes = [_vp, _i64, _vp, _vp]
     lib.ace_token_logprobs.argtypes = [_vp] * 4
     lib.ace_token_logprobs_backward.argtypes = [_vp] * 4 + [_i64, _vp]
+    lib.ace_token_logprobs_gradient.argtypes = [_vp] * 5 + [_i64, _vp]
     lib.ace_policy_loss_workspace_bytes.argtypes = [_vp]
     lib.ace_policy_loss.argtypes = [_vp] * 6 + [_size, _vp]
     lib.ace_policy_loss_gradient.argtypes = [_vp] * 7 + [_i64, _vp, _size, _vp]
@@ -701,19 +702,19 @@ def token_logprobs_backward(d_logp, logits, targets, stats, *, logp=None, out=No
             raise TypeError(f"logp: float32 expected, not {logp.dtype}")
         if not isinstance(targets, torch.Tensor) or logp.shape != targets.shape or logp.device != targets.device:
             raise ValueError(f"logp: what token_logprobs returned for these targets expected, got {tuple(logp.shape)} on {logp.device}")
-    a, z, keep = _token_loss_args(logits, targets, logp)     # (where the policy's have those of an earlier one)
-    _no_tangents(d_logp, stats)
+    a, z, keep = _token_loss_args(logits, targets)
+    _no_tangents(d_logp, logp, stats)
     _on_gpu(d_logp, "d_logp")
     if d_logp.dtype != torch.float32:
         raise TypeError(f"d_logp: float32 expected, not {d_logp.dtype}")
     if d_logp.shape != targets.shape or d_logp.device != z.device:
         raise ValueError(f"d_logp: {tuple(targets.shape)} on {z.device} expected, got {tuple(d_logp.shape)} on {d_logp.device}")
-    d_logp = d_logp.contiguous()
+    d_logp, logp = d_logp.contiguous(), None if logp is None else logp.contiguous()
     _on_gpu(stats, "stats")
     if stats.dtype != torch.float32 or stats.shape != targets.shape + (2,) or not stats.is_contiguous() or stats.device != z.device:
         raise ValueError("stats: what token_logprobs returned expected")
     grad, stride = _gradient_of(z, out)
-    _call(z.device, "ace_token_logprobs_backward", a, d_logp.data_ptr(), stats.data_ptr(), grad.data_ptr(), stride)
+    _call(z.device, "ace_token_logprobs_gradient", a, d_logp.data_ptr(), _pointer(logp), stats.data_ptr(), grad.data_ptr(), stride)
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return grad

@@ -19,6 +19,15 @@ def rows(vocab, rest, dtype):
     return z, targets, float(others / (1 + others))
 
 
+def test_refusals_of_the_c_entry():
+    lib = layer.load_library()
+    a = layer._TOKEN_LOSS.pack(4, 16, 16, 1, 64, 64, 64, 0, 0, 0, 0, 0.0, 1.0, 0.0, 0.25)
+    for logp in (None, 64):
+        assert lib.ace_token_logprobs_gradient(a, None, logp, 64, 128, 16, None) == -1 and lib.ace_token_logprobs_gradient(a, 64, logp, None, 128, 16, None) == -1
+        assert lib.ace_token_logprobs_gradient(a, 64, logp, 64, None, 16, None) == -1 and lib.ace_token_logprobs_gradient(a, 64, logp, 64, 128, 15, None) == -1
+    assert lib.ace_token_logprobs_gradient(None, 64, 64, 64, 128, 16, None) == -1
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("vocab", [600, 4099, 51200, 100003, 140001])
@@ -60,3 +69,15 @@ def test_log_probabilities_that_are_no_numbers_and_refusals():
     for bad, kind in ((r.logp.double(), TypeError), (r.logp[:5], ValueError), (r.logp.cpu(), ValueError), (1.0, TypeError)):
         with pytest.raises(kind):
             layer.token_logprobs_backward(d, z, t, r.stats, logp=bad)
+
+
+@gpu
+def test_a_policy_s_numbers_are_not_taken_for_log_probabilities():
+    """By the C entries: one structure for the policy's loss and for the gradients after it, with the earlier policy's log-probabilities in it."""
+    device = cuda_or_skip()
+    z, t = torch.randn(5, 900, device=device, generator=torch.Generator(device=device).manual_seed(1)), torch.arange(5, device=device)
+    r, old = layer.token_logprobs(z, t), torch.full((5,), -1.0, device=device)
+    d, out = torch.ones(5, device=device), torch.empty_like(z)
+    a = layer._TOKEN_LOSS.pack(5, 900, 900, 0, 64, z.data_ptr(), t.data_ptr(), old.data_ptr(), d.data_ptr(), 0, 0, 0.8, 1.2, 0.0, 0.2)
+    layer._call(device, "ace_token_logprobs_backward", a, d.data_ptr(), r.stats.data_ptr(), out.data_ptr(), 900)
+    assert torch.equal(out, layer.token_logprobs_backward(d, z, t, r.stats))
