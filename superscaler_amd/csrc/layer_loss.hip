@@ -7,10 +7,11 @@
  * falls on the side that it belongs to unless it is nearer to the border than those sums are exact (2^-24 of a ratio for each term of a lane, some hundreds at most).
  *
  * Bound by memory.  A workgroup's registers hold a whole row (held_rows), so that the gradient needs no second look at the logits: 8,192 rows of
- * 51,200 in bfloat16, a fifth of them without a target, 294 us, 5.2 TB/s of what is read and written, as a large copy does; with a second look (loss_rows,
+ * 51,200 in bfloat16, a fifth of them without a target, 293 us, 5.2 TB/s of what is read and written, as a large copy does; with a second look (loss_rows,
  * loss_back) 414.  Two workgroups of 512 lanes are resident on a CU with rows of up to 53,248 elements of 16 bits (half as many of 32), one with up to
- * 131,072 (98,304), past which a row is looked at twice.  800 MB of log-probabilities alone, from 8,192 to 65,536 elements a row: 127 to 145 us, 5.5 to 6.3 TB/s, which
- * is what reads alone reach; rows of 1,000, by a wavefront each, 246 (by four: 480).
+ * 131,072 (98,304), past which a row is looked at twice.  800 MB of log-probabilities alone, two inputs in turn, from 8,192 to 65,536 elements a row: 136 to 161 us, 5.0 to
+ * 5.9 TB/s, slowest in half precision; of 100,000 and 131,072 of 16 bits, one workgroup on a CU, 200 to 211 and 172 to 178; of 1,000, by a wavefront each, 197 to 209 (with four
+ * for each it was twice that).
  */
 #include <type_traits>
 #include "layer_common.h"
@@ -226,7 +227,7 @@ template <class T, int LANES, int HELD, int WHAT> __global__ void __launch_bound
     if (lane == layout.owner((int)target, LANES)) to[target] = (T)t.at_target;
 }
 
-/* A row per workgroup, AHEAD pieces for each lane on their way while as many are worked on.  8 rows of 200,000 in bfloat16 19.5 us, 1,225 98, 5.0 TB/s (256 lanes: 22.9 and
+/* A row per workgroup, AHEAD pieces for each lane on their way while as many are worked on.  8 rows of 200,000 in bfloat16 19.6 us, 1,225 97, 5.1 TB/s (256 lanes: 22.9 and
  * 97; 1,024: 20.5 and 121). */
 constexpr int AHEAD = 4;
 template <class T, int LANES, bool POLICY> __global__ void __launch_bounds__(LANES) loss_rows(const Loss a, int64_t first) {

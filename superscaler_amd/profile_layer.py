@@ -8,7 +8,8 @@ The times go into a database of the form that ProfileDB.from_directory loads; se
 optimizer's moments in 32 bits and in 8.  `--steps` trains the layer for that many steps with both, as a check that what was
 timed works together.  Collectives and bandwidths between GPUs cannot be taken on one card: they are those of the synthetic database.
 `--documents` fills every row of tokens with so many documents of different lengths, one after the other, whose tokens do not see each other's;
-`--loss` measures the output layer with the log-probabilities of its targets, forward and backward; `--clip` clips the gradients' norm in `--steps`.
+`--loss` measures the output layer with the log-probabilities of its targets, forward and backward (of a shard of the vocabulary,
+without what joins the shards); `--clip` clips the gradients' norm in `--steps`.
 `--policy-steps` trains a layer with an output layer as a policy: packed documents, the clipped loss on what it took, gradients clipped to `--clip` or 1.
 Where only some sizes and degrees are measured, the others are the synthetic database's, too: the line names them and no best plan.
 Prints one JSON line; `--out` writes the database as files, and beside them which of them were measured.
@@ -222,7 +223,7 @@ def _reserved_mb(call, device="cuda:0", left=None):
 def measure(w, micro_batch, tp, window=None, sinks=0, vocab=51200, reps=10, device="cuda:0", documents=0, loss=False):
     """{operator name: (forward us, backward us, reserved forward MB, backward MB)} of a layer's shard of workload `w`, for the rows of
     opgraph.GPT_TYPES.  `documents`: how many fill a row of tokens (0: it is one sequence); `loss`: the output layer's row has the
-    log-probabilities of its targets, too."""
+    log-probabilities of its targets, too (over a shard of the vocabulary they are of its part alone: what joins the parts is left out, as sums of a group are)."""
     net, h, s = GptLayer(w.hidden, tp, window, sinks, device), w.hidden, w.seq
     x = torch.randn(micro_batch, s, h, device=device).bfloat16()
     block, d = torch.randn_like(x), torch.randn_like(x)
